@@ -41,7 +41,7 @@ enum nf4b_status {
   NF4B_ERR_DEVICE = 5        /* current device is not an sm_100 part */
 };
 
-enum nf4b_dtype { NF4B_F16 = 0, NF4B_F32 = 1 };
+enum nf4b_dtype { NF4B_F16 = 0, NF4B_F32 = 1, NF4B_BF16 = 2 /* attention and gradient clipping (stew_step.h) only */ };
 
 /* The fields of a bitsandbytes QuantState the unpack reads (nf4.py:61-70, :80-91).
  * Nested (double-quantized) state:

@@ -11,7 +11,8 @@
  *                                       for the backward) applied to q and k in one launch
  *   nf4b_swiglu_fwd / _bwd           <- solution/swiglu.py:15-40
  *   nf4b_ce_fwd / _bwd               <- solution/head_loss.py (loss, then softmax - onehot)
- * Activations are fp16, row-major.
+ *   nf4b_attn_fwd / _bwd             <- the per-row SDPA of solution/unpad.py:177-219
+ * Activations are fp16, row-major (attention: fp16 or bf16, strided).
  */
 #ifndef STEW_STEP_H
 #define STEW_STEP_H
@@ -64,6 +65,70 @@ int nf4b_ce_fwd(const void* logits, const int64_t* labels, float* loss, float* l
                 int64_t vocab, void* stream);
 int nf4b_ce_bwd(void* logits, const int64_t* labels, const float* lse, const float* gscale,
                 int64_t rows, int64_t vocab, void* stream);
+
+/* Attention over packed token rows.  q [tokens, heads, head_dim] and k, v [tokens, kv_heads,
+ * head_dim] (fp16 or bf16) hold `rows` sequences one after the other: sequence b is tokens
+ * [cu[b], cu[b+1]) (device int32 [rows + 1], cu[0] = 0, ascending, cu[rows] <= tokens; an empty
+ * sequence is allowed).  Inside a sequence token i sees the tokens j with
+ * i - left <= j <= i + right; a negative bound is no bound ((-1, 0) is causal attention).  Query
+ * head h reads key/value head h / (heads / kv_heads).  With s_ij = scale q_i.k_j:
+ *   p_ij = exp(s_ij) / sum_j exp(s_ij),   o_i = sum_j p_ij v_j,   lse_i = log sum_j exp(s_ij)
+ * head_dim: a multiple of 8, at most 128.  The last dimension is contiguous; token and head
+ * strides (in elements) are multiples of 8 and at least head_dim, pointers are 16-byte aligned.
+ * cu is read on the device: values outside [0, tokens] are clamped there.  */
+typedef struct nf4b_attn {
+  const void* q;
+  const void* k;
+  const void* v;
+  const int32_t* cu;
+  int64_t tokens;
+  int64_t q_stride, q_head_stride;
+  int64_t k_stride, k_head_stride;
+  int64_t v_stride, v_head_stride;
+  int32_t rows, heads, kv_heads, head_dim;
+  int32_t dtype;         /* NF4B_F16 or NF4B_BF16 */
+  int32_t left, right;
+  float scale;           /* > 0 */
+} nf4b_attn;
+
+/* out [tokens, heads, head_dim] contiguous, of q's type; lse fp32 [heads, tokens] (natural log).
+ * Tokens at and behind cu[rows] get zeros (lse -inf).  */
+int nf4b_attn_fwd(const nf4b_attn* a, void* out, float* lse, void* stream);
+
+/* Gradients from dout, out (contiguous, as nf4b_attn_fwd wrote it) and lse:
+ *   dv_j = sum_i p_ij do_i,   ds_ij = p_ij (do_i.v_j - do_i.o_i),
+ *   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,
+ * k's and v's summed over the query heads that share them.  The probabilities are recomputed
+ * from lse; every sum is taken in a fixed order (the same bits on every run).  dout, dq
+ * [tokens, heads, head_dim] and dk, dv [tokens, kv_heads, head_dim] are contiguous, of q's type;
+ * tokens at and behind cu[rows] get zeros.  work: nf4b_attn_bwd_work_bytes() bytes of device
+ * scratch, 16-byte aligned, of any content; -1 for sizes outside the envelope.  */
+int64_t nf4b_attn_bwd_work_bytes(int64_t tokens, int32_t rows, int32_t heads, int32_t kv_heads);
+int nf4b_attn_bwd(const nf4b_attn* a, const void* out, const float* lse, const void* dout, void* dq,
+                  void* dk, void* dv, void* work, int64_t work_bytes, void* stream);
+
+/* One gradient of a list: src and dst hold `numel` contiguous values of `dtype` (NF4B_F16,
+ * NF4B_BF16 or NF4B_F32; the element's own alignment is enough).  dst == src scales in place;
+ * dst == NULL reads it for the norm only.  numel 0 is allowed (pointers may then be NULL).  */
+typedef struct nf4b_grad {
+  const void* src;
+  void* dst;
+  int64_t numel;
+  int32_t dtype;
+  int32_t reserved;
+} nf4b_grad;
+
+/* Global 2-norm of a list of gradients and clipping to max_norm (>= 0, or infinity):
+ *   *norm = || src / *divisor ||_2 over all n gradients (device fp32; divisor: device fp32, NULL = 1)
+ *   dst   = src * (1 / *divisor) * min(1, max_norm / (*norm + 1e-6))
+ * The squares are summed in 64 bits in a fixed order.  A norm that is infinite gives zeros (NaN
+ * where src is infinite), a NaN norm gives NaN everywhere.  An in-place list under the limit with
+ * no divisor is not written.  No dst may overlap another gradient's src or dst.  `grads` is a host
+ * array, read before the call returns.  work: nf4b_clip_grads_work_bytes(n) bytes of device
+ * scratch, 8-byte aligned, of any content.  */
+int64_t nf4b_clip_grads_work_bytes(int32_t n);
+int nf4b_clip_grads(const nf4b_grad* grads, int32_t n, float max_norm, const float* divisor, float* norm,
+                    void* work, int64_t work_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -20,6 +20,7 @@ NF4B_ERR_CUDA = 4
 NF4B_ERR_DEVICE = 5
 NF4B_F16 = 0
 NF4B_F32 = 1
+NF4B_BF16 = 2
 
 c_void_p = ctypes.c_void_p
 c_int32 = ctypes.c_int32
@@ -64,6 +65,21 @@ class LoraGradsItemC(ctypes.Structure):
     _fields_ = [("x", c_void_p), ("dy", c_void_p), ("xa", c_void_p), ("dyb", c_void_p),
                 ("scale", c_float), ("da", c_void_p), ("db", c_void_p), ("in_features", c_int64),
                 ("out_features", c_int64)]
+
+
+class AttnC(ctypes.Structure):
+    """nf4b_attn."""
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("cu", c_void_p), ("tokens", c_int64),
+                ("q_stride", c_int64), ("q_head_stride", c_int64), ("k_stride", c_int64),
+                ("k_head_stride", c_int64), ("v_stride", c_int64), ("v_head_stride", c_int64),
+                ("rows", c_int32), ("heads", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32),
+                ("dtype", c_int32), ("left", c_int32), ("right", c_int32), ("scale", c_float)]
+
+
+class GradC(ctypes.Structure):
+    """nf4b_grad."""
+    _fields_ = [("src", c_void_p), ("dst", c_void_p), ("numel", c_int64), ("dtype", c_int32),
+                ("reserved", c_int32)]
 
 
 # name -> (restype, argtypes); every symbol include/*.h declares
@@ -113,6 +129,12 @@ SIGNATURES = {
     "nf4b_swiglu_bwd": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     "nf4b_ce_fwd": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p]),
     "nf4b_ce_bwd": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p]),
+    "nf4b_attn_fwd": (c_int32, [ctypes.POINTER(AttnC), c_void_p, c_void_p, c_void_p]),
+    "nf4b_attn_bwd_work_bytes": (c_int64, [c_int64, c_int32, c_int32, c_int32]),
+    "nf4b_attn_bwd": (c_int32, [ctypes.POINTER(AttnC), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                c_void_p, c_void_p, c_int64, c_void_p]),
+    "nf4b_clip_grads_work_bytes": (c_int64, [c_int32]),
+    "nf4b_clip_grads": (c_int32, [c_void_p, c_int32, c_float, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     "nf4b_lora_grads": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_void_p,
                                   c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int32, c_void_p]),
     "nf4b_lora_grads_noalloc": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_void_p,

@@ -13,14 +13,78 @@ from __future__ import annotations
 
 import math
 
+import ctypes
+from itertools import chain
+
 import torch
 import torch.distributed as dist
+
+from . import _lib
 
 
 def _world(group) -> int:
     if not (dist.is_available() and dist.is_initialized()):
         return 1
     return dist.get_world_size(group)
+
+
+_GRAD_DTYPE = {torch.float32: _lib.NF4B_F32, torch.float16: _lib.NF4B_F16, torch.bfloat16: _lib.NF4B_BF16}
+
+
+def clip_grads(grads, max_norm: float, divisor: torch.Tensor | None = None, out=None) -> torch.Tensor:
+    """Global 2-norm over a list of gradients and clipping to max_norm, without a host
+    synchronisation (so a captured step can hold it):
+        norm = || g / divisor ||_2 over all of them,  out = g / divisor * min(1, max_norm / (norm + 1e-6))
+    Returns the norm before clipping (0-d fp32 device tensor).  grads: contiguous CUDA tensors of
+    one device, fp32 / fp16 / bf16, each type its own.  out: where the results go, tensors of the
+    same sizes and types (for instance the parameters' gradients, for grads that are views of an
+    all-reduced flat buffer); None scales in place, and an in-place list that is under the limit
+    and has no divisor is only read.  divisor: one fp32 on the device (the labelled-token count),
+    None for 1.  max_norm: >= 0; infinity never clips.  A norm that is not finite behaves as
+    max_norm / norm does: infinite gives zeros (NaN where g is infinite), NaN gives NaN."""
+    grads = list(grads)
+    dst = grads if out is None else list(out)
+    if not grads:
+        raise ValueError("clip_grads: no gradients")
+    if len(dst) != len(grads):
+        raise ValueError(f"clip_grads: {len(dst)} outputs for {len(grads)} gradients")
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"clip_grads: max_norm must be >= 0, got {max_norm}")
+    dev = grads[0].device
+    if dev.type != "cuda":
+        raise _lib.NF4Unsupported(_lib.NF4B_ERR_UNSUPPORTED, f"clip_grads: gradients on {dev} (CUDA only)")
+    table = []
+    for g, o in zip(grads, dst):
+        dt = _GRAD_DTYPE.get(g.dtype)
+        if dt is None:
+            raise _lib.NF4Unsupported(_lib.NF4B_ERR_UNSUPPORTED, f"clip_grads: {g.dtype} gradient")
+        n = g.numel()
+        if g.device != dev or not g.is_contiguous():
+            raise ValueError("clip_grads: gradients must be contiguous and on one device")
+        if o is not g and (o.dtype != g.dtype or o.numel() != n or o.device != dev or not o.is_contiguous()):
+            raise ValueError("clip_grads: an output must be contiguous, of its gradient's type, size and device")
+        table.append((g.data_ptr(), o.data_ptr(), n, dt))
+    used = [t[1] for t in table if t[2]]
+    if len(set(used)) != len(used):
+        raise ValueError("clip_grads: one tensor is the output of two gradients")
+    if out is not None:
+        read = {t[0] for t in table if t[2]}
+        if any(t[1] != t[0] and t[1] in read for t in table if t[2]):
+            raise ValueError("clip_grads: an output is another gradient of the list")
+    if divisor is not None and (divisor.dtype != torch.float32 or divisor.numel() != 1 or divisor.device != dev):
+        raise ValueError("clip_grads: divisor must be one fp32 value on the gradients' device")
+    L = _lib.lib()
+    wb = int(L.nf4b_clip_grads_work_bytes(len(table)))
+    # nf4b_grad is four 64-bit words: src, dst, numel, and dtype beside a reserved half
+    arr = (ctypes.c_int64 * (4 * len(table)))(*chain.from_iterable(table))
+    with torch.cuda.device(dev):
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        work = torch.empty(wb, dtype=torch.uint8, device=dev)
+        _lib.check(L.nf4b_clip_grads(arr, len(table), max_norm, None if divisor is None else divisor.data_ptr(),
+                                     norm.data_ptr(), work.data_ptr(), wb, torch.cuda.current_stream(dev).cuda_stream),
+                   "nf4b_clip_grads")
+    return norm
 
 
 def flatten_grads(params, extra: float) -> torch.Tensor:

@@ -1,12 +1,17 @@
 """Autograd wrappers of the layer kernels of the packed-token QLoRA step (C ABI
 include/stew_step.h): RMSNorm, RMSNorm fused with the residual add, rotary embedding of q and
-k, SwiGLU and the LM head's cross-entropy -- the counterparts of the reference's
+k, attention over packed rows, SwiGLU and the LM head's cross-entropy -- the counterparts of the
+reference's
 solution/rmsnorm.py (RMSNormFn :59-92, AddRMSNormFn :192-233), solution/rope.py (:71-92),
 solution/swiglu.py (:42-66) and solution/head_loss.py.  fp16 activations, fp32 math; the CUDA
 kernels are the only implementation (no torch fallback)."""
 from __future__ import annotations
 
+import ctypes
+import math
+
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .nf4 import _stream
@@ -148,6 +153,134 @@ def rope_qk(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tens
 def swiglu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     """fp16(gate * sigmoid(gate) * up), fp32 inside (the reference's SwiGLU kernel)."""
     return _SwiGLU.apply(gate, up)
+
+
+ATTN_MAX_HEAD_DIM = 128
+_ATTN_DTYPE = {torch.float16: _lib.NF4B_F16, torch.bfloat16: _lib.NF4B_BF16}
+
+
+def _attn_layout(t: torch.Tensor) -> torch.Tensor:
+    """t [tokens, heads, head_dim] as the kernels read it: contiguous features, strides that are
+    multiples of 8 elements, a 16-byte aligned base (slices of one projection output stay as they
+    are; anything else, a broadcast view too, is copied)."""
+    n, h, d = t.shape
+    if (t.stride(2) == 1 and (n == 1 or (t.stride(0) >= d and t.stride(0) % 8 == 0))
+            and (h == 1 or (t.stride(1) >= d and t.stride(1) % 8 == 0)) and t.data_ptr() % 16 == 0):
+        return t
+    return _aligned_c(t)
+
+
+def _aligned_c(t: torch.Tensor) -> torch.Tensor:
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _attn_c(q, k, v, cu, left, right, scale) -> _lib.AttnC:
+    n, hq, d = q.shape
+    hk = k.shape[1]
+    a = _lib.AttnC()
+    a.q, a.k, a.v, a.cu = q.data_ptr(), k.data_ptr(), v.data_ptr(), cu.data_ptr()
+    a.tokens, a.rows, a.heads, a.kv_heads, a.head_dim = n, cu.numel() - 1, hq, hk, d
+    # a dimension of one element may carry any stride
+    a.q_stride, a.q_head_stride = (q.stride(0) if n > 1 else hq * d), (q.stride(1) if hq > 1 else d)
+    a.k_stride, a.k_head_stride = (k.stride(0) if n > 1 else hk * d), (k.stride(1) if hk > 1 else d)
+    a.v_stride, a.v_head_stride = (v.stride(0) if n > 1 else hk * d), (v.stride(1) if hk > 1 else d)
+    a.dtype, a.left, a.right, a.scale = _ATTN_DTYPE[q.dtype], left, right, scale
+    return a
+
+
+def _attn_forward(q, k, v, cu, left, right, scale):
+    q, k, v = _attn_layout(q), _attn_layout(k), _attn_layout(v)
+    n, hq, d = q.shape
+    dev = q.device
+    out = torch.empty(n, hq, d, dtype=q.dtype, device=dev)
+    lse = torch.empty(hq, n, dtype=torch.float32, device=dev)
+    if n:
+        with torch.cuda.device(dev):
+            a = _attn_c(q, k, v, cu, left, right, scale)
+            _lib.check(_lib.lib().nf4b_attn_fwd(ctypes.byref(a), out.data_ptr(), lse.data_ptr(), _stream(dev)),
+                       "nf4b_attn_fwd")
+    return q, k, v, out, lse
+
+
+class _PackedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu, left, right, scale):
+        q, k, v, out, lse = _attn_forward(q, k, v, cu, left, right, scale)
+        ctx.save_for_backward(q, k, v, cu, out, lse)
+        ctx.args = (left, right, scale)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, cu, out, lse = ctx.saved_tensors
+        n, hq, d = q.shape
+        hk = k.shape[1]
+        dev = q.device
+        dout = _aligned_c(dout.to(q.dtype))
+        dq = torch.empty(n, hq, d, dtype=q.dtype, device=dev)
+        dk = torch.empty(n, hk, d, dtype=q.dtype, device=dev)
+        dv = torch.empty(n, hk, d, dtype=q.dtype, device=dev)
+        if n:
+            L = _lib.lib()
+            with torch.cuda.device(dev):
+                a = _attn_c(q, k, v, cu, *ctx.args)
+                wb = int(L.nf4b_attn_bwd_work_bytes(n, a.rows, hq, hk))
+                work = torch.empty(max(wb, 16), dtype=torch.uint8, device=dev)
+                _lib.check(L.nf4b_attn_bwd(ctypes.byref(a), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
+                                           dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), work.data_ptr(), wb,
+                                           _stream(dev)), "nf4b_attn_bwd")
+        return dq, dk, dv, None, None, None, None
+
+
+def packed_attention_supported(q: torch.Tensor) -> bool:
+    """Whether packed_attention's kernels take q's type and head size."""
+    return (q.is_cuda and q.dtype in _ATTN_DTYPE and q.shape[-1] % 8 == 0
+            and 0 < q.shape[-1] <= ATTN_MAX_HEAD_DIM)
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor, window=(-1, 0),
+                     scale: float | None = None) -> torch.Tensor:
+    """Attention inside each of the sequences packed one after the other in q [N, Hq, D] and
+    k, v [N, Hk, D] (fp16 or bf16; D a multiple of 8 up to 128; Hq a multiple of Hk, query head h
+    reading key/value head h // (Hq / Hk)).  cu: int32 [B + 1] on the same device, sequence b is
+    tokens [cu[b], cu[b+1]), cu[0] = 0, ascending; empty sequences are allowed.  Its values are
+    not read on the host: the kernels cut them to [0, N].
+    window = (left, right): token i sees the tokens i - left <= j <= i + right of its sequence, -1
+    for no bound; (-1, 0) is causal, (-1, -1) sees everything.  scale: of the scores, default
+    1 / sqrt(D).
+    Returns [N, Hq, D]; tokens behind cu[B] get zeros, and zero gradients.  Any strides with
+    contiguous features are read in place when they are multiples of 8 elements, else copied.
+    The backward recomputes the probabilities from the saved log-sum-exp; forward and backward
+    give the same bits on every run.  Second derivatives are refused."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 3:
+            raise ValueError(f"packed_attention: {name} must be [tokens, heads, head_dim], got {tuple(t.shape)}")
+        if t.dtype != q.dtype or t.device != q.device:
+            raise ValueError("packed_attention: q, k and v must share one type and device")
+    n, hq, d = q.shape
+    if k.shape != v.shape or k.shape[0] != n or k.shape[2] != d:
+        raise ValueError(f"packed_attention: k {tuple(k.shape)} and v {tuple(v.shape)} do not fit q {tuple(q.shape)}")
+    hk = k.shape[1]
+    if hk == 0 or hq == 0 or hq % hk:
+        raise ValueError(f"packed_attention: {hq} query heads are not a multiple of {hk} key/value heads")
+    if not packed_attention_supported(q):
+        raise _lib.NF4Unsupported(_lib.NF4B_ERR_UNSUPPORTED,
+                                  f"packed_attention: {q.dtype} head_dim {d} on {q.device} (fp16 or bf16 CUDA "
+                                  "tensors, head_dim a multiple of 8 up to 128)")
+    if cu.dtype != torch.int32 or cu.dim() != 1 or cu.numel() < 1 or cu.device != q.device or not cu.is_contiguous():
+        raise ValueError("packed_attention: cu must be a contiguous int32 vector of B + 1 row starts on q's device")
+    left, right = (int(x) for x in window)
+    if left < -1 or right < -1:
+        raise ValueError(f"packed_attention: window {tuple(window)}: bounds are >= 0, or -1 for none")
+    left, right = min(left, n), min(right, n)  # further than the longest sequence: no bound
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise ValueError(f"packed_attention: scale must be positive and finite, got {scale}")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _PackedAttention.apply(q, k, v, cu, left, right, scale)
+    return _attn_forward(q, k, v, cu, left, right, scale)[3]
 
 
 # The backward's softmax - onehot is written as fp16 times this power of two (exact to divide
