@@ -107,6 +107,11 @@ int64_t nf4b_attn_bwd_work_bytes(int64_t tokens, int32_t rows, int32_t heads, in
 int nf4b_attn_bwd(const nf4b_attn* a, const void* out, const float* lse, const void* dout, void* dq,
                   void* dk, void* dv, void* work, int64_t work_bytes, void* stream);
 
+/* Reads (and with reset != 0 clears) the device-side flag the attention kernels set when a pipeline
+ * wait ran out of time (the kernel then ends early instead of hanging).  0 = no timeout since the
+ * last reset.  Synchronous.  */
+int nf4b_attn_error_flag(int* value, int reset);
+
 /* One gradient of a list: src and dst hold `numel` contiguous values of `dtype` (NF4B_F16,
  * NF4B_BF16 or NF4B_F32; the element's own alignment is enough).  dst == src scales in place;
  * dst == NULL reads it for the norm only.  numel 0 is allowed (pointers may then be NULL).  */

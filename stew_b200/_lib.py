@@ -133,6 +133,7 @@ SIGNATURES = {
     "nf4b_attn_bwd_work_bytes": (c_int64, [c_int64, c_int32, c_int32, c_int32]),
     "nf4b_attn_bwd": (c_int32, [ctypes.POINTER(AttnC), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                 c_void_p, c_void_p, c_int64, c_void_p]),
+    "nf4b_attn_error_flag": (c_int32, [ctypes.POINTER(c_int32), c_int32]),
     "nf4b_clip_grads_work_bytes": (c_int64, [c_int32]),
     "nf4b_clip_grads": (c_int32, [c_void_p, c_int32, c_float, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     "nf4b_lora_grads": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_void_p,
@@ -212,6 +213,12 @@ def gemm_error_flag(reset: bool = True) -> int:
 def dequant_error_flag(reset: bool = True) -> int:
     v = c_int32(0)
     check(lib().nf4b_dequant_error_flag(ctypes.byref(v), 1 if reset else 0), "nf4b_dequant_error_flag")
+    return int(v.value)
+
+
+def attn_error_flag(reset: bool = True) -> int:
+    v = c_int32(0)
+    check(lib().nf4b_attn_error_flag(ctypes.byref(v), 1 if reset else 0), "nf4b_attn_error_flag")
     return int(v.value)
 
 

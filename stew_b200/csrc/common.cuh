@@ -46,6 +46,11 @@ inline int ilog2_exact(int64_t v) {
   return s;
 }
 
+// Tensor map of a tiled TMA tensor of up to 5 dimensions (innermost first; `strides` in bytes, of
+// the dimensions after the first).
+int make_tmap_tiled(CUtensorMap* m, CUtensorMapDataType dt, int rank, const void* base, const uint64_t* dims,
+                    const uint64_t* strides, const uint32_t* box, CUtensorMapSwizzle sw);
+
 // Checks the device once per thread and device: sm_100 family only.
 int check_device();
 

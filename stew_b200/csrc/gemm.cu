@@ -1255,19 +1255,22 @@ static EncodeTiledFn encode_fn() {
   return fn;
 }
 
-static int make_tmap_2d(CUtensorMap* m, CUtensorMapDataType dt, const void* base, uint64_t inner,
-                        uint64_t outer, uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer,
-                        CUtensorMapSwizzle sw) {
+int make_tmap_tiled(CUtensorMap* m, CUtensorMapDataType dt, int rank, const void* base, const uint64_t* dims,
+                    const uint64_t* strides, const uint32_t* box, CUtensorMapSwizzle sw) {
   EncodeTiledFn enc = encode_fn();
   if (!enc) {
     record_driver_error("cudaGetDriverEntryPoint(cuTensorMapEncodeTiled)", -1);
     return NF4B_ERR_CUDA;
   }
-  cuuint64_t dims[2] = {inner, outer};
-  cuuint64_t strides[1] = {row_bytes};
-  cuuint32_t box[2] = {box_inner, box_outer};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = enc(m, dt, 2, const_cast<void*>(base), dims, strides, box, estr,
+  cuuint64_t d[5], st[4];
+  cuuint32_t bx[5], estr[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    bx[i] = box[i];
+    estr[i] = 1;
+    if (i + 1 < rank) st[i] = strides[i];
+  }
+  CUresult r = enc(m, dt, cuuint32_t(rank), const_cast<void*>(base), d, st, bx, estr,
                    CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
@@ -1275,6 +1278,14 @@ static int make_tmap_2d(CUtensorMap* m, CUtensorMapDataType dt, const void* base
     return NF4B_ERR_CUDA;
   }
   return NF4B_OK;
+}
+
+static int make_tmap_2d(CUtensorMap* m, CUtensorMapDataType dt, const void* base, uint64_t inner,
+                        uint64_t outer, uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer,
+                        CUtensorMapSwizzle sw) {
+  const uint64_t dims[2] = {inner, outer}, strides[1] = {row_bytes};
+  const uint32_t box[2] = {box_inner, box_outer};
+  return make_tmap_tiled(m, dt, 2, base, dims, strides, box, sw);
 }
 
 static int sm_count_cached() {
