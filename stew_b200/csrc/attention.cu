@@ -4,63 +4,14 @@
 //   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i
 // over the pairs (i, j) of one sequence inside the window i - left <= j <= i + right.
 //
-// One warp owns one (token, head): forward and dq walk the token's keys, dk/dv walk the queries
-// that see the key, over every query head of its group.  A lane holds head_dim / 32 consecutive
-// features (rounded up to 4); all sums are fp32 in registers and in a fixed order.
+// Every product runs on tcgen05 over 128-token tiles that TMA brings in; a ragged tile's rows of other
+// sequences are zeroed in shared memory where a product sums over them, and masked elsewhere.
+// Sums and softmax statistics are fp32 (TMEM, registers), in a fixed order.
 #include <mutex>
 
 #include "attn_common.cuh"
 
 namespace nf4b {
-
-constexpr int AT_WARPS = 4;
-
-template <typename T>
-__device__ __forceinline__ float at_to_f(T v);
-template <>
-__device__ __forceinline__ float at_to_f<__half>(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float at_to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-__device__ __forceinline__ T at_from_f(float v);
-template <>
-__device__ __forceinline__ __half at_from_f<__half>(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 at_from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
-// Four features of a lane (zeros behind head_dim).
-template <typename T>
-__device__ __forceinline__ void at_load(const T* row, int lane, int head_dim, float (&f)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = lane * 4 + i < head_dim ? at_to_f(row[lane * 4 + i]) : 0.f;
-}
-template <typename T>
-__device__ __forceinline__ void at_store(T* row, int lane, int head_dim, const float (&f)[4], float s) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane * 4 + i < head_dim) row[lane * 4 + i] = at_from_f<T>(f[i] * s);
-}
-__device__ __forceinline__ float at_dot(const float (&a)[4], const float (&b)[4]) {
-  float s = fmaf(a[0], b[0], fmaf(a[1], b[1], fmaf(a[2], b[2], a[3] * b[3])));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  return s;
-}
-
-// The sequence [a, b) that holds token t; false behind the last one.  cu's values are clamped
-// to [0, tokens], so nothing outside the tensors is ever addressed.
-__device__ __forceinline__ bool at_sequence(const nf4b_attn& p, int64_t t, int64_t& a, int64_t& b) {
-  auto at = [&](int i) { return i == 0 ? int64_t(0) : max(int64_t(0), min64(p.cu[i], p.tokens)); };
-  if (p.rows == 0 || t >= at(p.rows)) return false;
-  int lo = 0, hi = p.rows;  // cu[lo] <= t < cu[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (at(mid) <= t) lo = mid; else hi = mid;
-  }
-  a = at(lo);
-  b = at(hi);
-  return true;
-}
 
 // ------------------------------------------------------------------- forward
 // One CTA per (128-token query tile, head); two CTAs on an SM, so one's softmax runs beside the
@@ -328,76 +279,533 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
   if (warp == 5) tmem_dealloc(tmem, 256);
 }
 
-// dq, and delta_i = do_i.o_i for the dk/dv kernel.
-template <typename T>
-__global__ void __launch_bounds__(32 * AT_WARPS)
-    attn_dq_kernel(const nf4b_attn p, const T* __restrict__ out, const float* __restrict__ lse, const T* __restrict__ dout,
-                   T* __restrict__ dq, float* __restrict__ delta) {
-  const int lane = threadIdx.x & 31;
-  const int64_t w = int64_t(blockIdx.x) * AT_WARPS + (threadIdx.x >> 5);
-  if (w >= p.tokens * p.heads) return;
-  const int64_t t = w / p.heads;
-  const int h = int(w - t * p.heads), hk = h / (p.heads / p.kv_heads);
-  int64_t a, b;
-  float g[4] = {0, 0, 0, 0}, dl = 0.f;
-  const int64_t off = (t * p.heads + h) * p.head_dim;
-  if (at_sequence(p, t, a, b)) {
-    float q[4], o[4], d[4];
-    at_load(static_cast<const T*>(p.q) + t * p.q_stride + h * p.q_head_stride, lane, p.head_dim, q);
-    at_load(out + off, lane, p.head_dim, o);
-    at_load(dout + off, lane, p.head_dim, d);
-    dl = at_dot(o, d);
-    const float le = lse[int64_t(h) * p.tokens + t];
-    const int64_t j0 = p.left < 0 ? a : max(a, t - p.left), j1 = p.right < 0 ? b : min64(b, t + p.right + 1);
-    for (int64_t j = j0; j < j1; ++j) {
-      float k[4], v[4];
-      at_load(static_cast<const T*>(p.k) + j * p.k_stride + hk * p.k_head_stride, lane, p.head_dim, k);
-      at_load(static_cast<const T*>(p.v) + j * p.v_stride + hk * p.v_head_stride, lane, p.head_dim, v);
-      const float e = le == -INFINITY ? 0.f : expf(at_dot(q, k) * p.scale - le);
-      const float ds = e * (at_dot(d, v) - dl);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) g[i] = fmaf(ds, k[i], g[i]);
-    }
-  }
-  at_store(dq + off, lane, p.head_dim, g, p.scale);
-  if (lane == 0) delta[int64_t(h) * p.tokens + t] = dl;
-}
+// ------------------------------------------------------------------ backward
+// Two launches.  The first (attn_prep_kernel) writes, per (head, token), the row's log-sum-exp in
+// log2 units and delta = do.o, and zeros behind the last sequence.  The second holds two kinds of
+// CTAs with one structure, a resident pair of 128-token tiles X, Y against a ring of tile pairs
+// A, B (D = head_dim):
+//   keys    (DKV): X = K, Y = V of a key tile; A = Q, B = dO over the query tiles of every head of
+//                  the group:  S^T = X A^T, dP^T = Y B^T, dV += P^T B, dK += dS^T A
+//   queries:       X = Q, Y = dO of a query tile and head; A = K, B = V over its key tiles:
+//                  S = X A^T, dP = Y B^T, dQ += dS A
+// S and dP are recomputed by both kinds (7 products instead of 5): that buys dQ, dK and dV summed in
+// TMEM in a fixed order, with no fp32 dQ buffer in memory and no atomics.  P and dS overwrite S and dP
+// in TMEM as 16-bit values and are the A operands of the second products from there.
+//   warps 0-7  elementwise: thread (row = TMEM lane, half of the columns)
+//   warp 8     TMA; in DKV CTAs also the query rows' (lse, delta) into shared memory
+//   warp 9     TMEM allocation, MMA issue
+//
+// fp16 range: dS is rounded to the operand type with a power-of-two scale 2^k that puts the largest
+// |dO||V| + |delta| of the sequence (the prep launch's maxima per tile) at 2^14, and P with 2^8:
+// gradients of any size keep fp16's 11 bits, where unscaled products of small gradients would fall
+// into its subnormals.  bf16 has fp32's range and is not scaled.
+constexpr int AT_BWD_THREADS = 320;
+constexpr int AT_PREP_THREADS = 256;
 
 template <typename T>
-__global__ void __launch_bounds__(32 * AT_WARPS)
-    attn_dkv_kernel(const nf4b_attn p, const float* __restrict__ lse, const T* __restrict__ dout,
-                    const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv) {
-  const int lane = threadIdx.x & 31;
-  const int64_t w = int64_t(blockIdx.x) * AT_WARPS + (threadIdx.x >> 5);
-  if (w >= p.tokens * p.kv_heads) return;
-  const int64_t j = w / p.kv_heads;
-  const int hk = int(w - j * p.kv_heads), grp = p.heads / p.kv_heads;
-  int64_t a, b;
-  float gk[4] = {0, 0, 0, 0}, gv[4] = {0, 0, 0, 0};
-  if (at_sequence(p, j, a, b)) {
-    float k[4], v[4];
-    at_load(static_cast<const T*>(p.k) + j * p.k_stride + hk * p.k_head_stride, lane, p.head_dim, k);
-    at_load(static_cast<const T*>(p.v) + j * p.v_stride + hk * p.v_head_stride, lane, p.head_dim, v);
-    const int64_t i0 = p.right < 0 ? a : max(a, j - p.right), i1 = p.left < 0 ? b : min64(b, j + p.left + 1);
-    for (int h = hk * grp; h < (hk + 1) * grp; ++h) {
-      for (int64_t i = i0; i < i1; ++i) {
-        float q[4], d[4];
-        at_load(static_cast<const T*>(p.q) + i * p.q_stride + h * p.q_head_stride, lane, p.head_dim, q);
-        at_load(dout + (i * p.heads + h) * p.head_dim, lane, p.head_dim, d);
-        const float le = lse[int64_t(h) * p.tokens + i];
-        const float e = le == -INFINITY ? 0.f : expf(at_dot(q, k) * p.scale - le);
-        const float ds = e * (at_dot(d, v) - delta[int64_t(h) * p.tokens + i]);
+constexpr float at_p_shift() { return sizeof(T) == 2 && at_idesc<T>(16, false) == at_idesc<__half>(16, false) ? 8.f : 0.f; }
+
+// The backward's scratch.
+struct AttnWork {
+  float2* row;    // [heads][tokens]: lse log2(e), delta
+  float2* tile;   // [heads][slots]: max |dO_i|, max |delta_i| of a query tile
+  float* vmax;    // [kv_heads][slots]: max |V_j| of a key tile
+};
+
+__device__ __forceinline__ float at_half_warp_sum(float v) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          gv[x] = fmaf(e, d[x], gv[x]);
-          gk[x] = fmaf(ds, q[x], gk[x]);
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// One CTA per (128-token tile, head), half a warp per row; reads O, dO (and V once per group).
+template <typename T>
+__global__ void __launch_bounds__(AT_PREP_THREADS)
+    attn_prep_kernel(const __grid_constant__ AttnParams p, const T* __restrict__ out, const T* __restrict__ dout,
+                     const float* __restrict__ lse, const T* __restrict__ v, int64_t v_stride, int64_t v_head_stride,
+                     AttnWork w, T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dv) {
+  grid_dep_wait();  // programmatic launch: no global access before the wait
+  const int slot = int(blockIdx.x / p.heads), h = blockIdx.x % p.heads;
+  const int grp = p.heads / p.kv_heads, hk = h / grp;
+  const bool first = h % grp == 0;
+  const AttnTile t = at_find(p, slot);
+  if (t.i0 >= t.len) return;
+  const int n = min(AT_TILE, t.len - t.i0);
+  const int sub = threadIdx.x & 15, f = sub * 8;  // this thread's 8 features
+  const bool in = f < p.head_dim;
+  float m_do = 0.f, m_dl = 0.f, m_v = 0.f;
+  for (int r0 = 0; r0 < AT_TILE; r0 += AT_PREP_THREADS / 16) {
+    const int r = r0 + (threadIdx.x >> 4);
+    const bool live = r < n && in;
+    const int64_t row = t.a + t.i0 + r;
+    const int64_t off = (row * p.heads + h) * p.head_dim + f, koff = (row * p.kv_heads + hk) * p.head_dim + f;
+    if (t.tail) {
+      if (live) {
+        *reinterpret_cast<uint4*>(dq + off) = make_uint4(0, 0, 0, 0);
+        if (first) {
+          *reinterpret_cast<uint4*>(dk + koff) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(dv + koff) = make_uint4(0, 0, 0, 0);
+        }
+      }
+      continue;
+    }
+    float dot = 0.f, nd = 0.f, nv = 0.f;
+    if (live) {
+      const uint4 o4 = *reinterpret_cast<const uint4*>(out + off), d4 = *reinterpret_cast<const uint4*>(dout + off);
+      const uint32_t* o = reinterpret_cast<const uint32_t*>(&o4);
+      const uint32_t* d = reinterpret_cast<const uint32_t*>(&d4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 a = at_unpack<T>(o[i]), b = at_unpack<T>(d[i]);
+        dot = fmaf(a.x, b.x, fmaf(a.y, b.y, dot));
+        nd = fmaf(b.x, b.x, fmaf(b.y, b.y, nd));
+      }
+      if (first && at_p_shift<T>() != 0.f) {
+        const uint4 v4 = *reinterpret_cast<const uint4*>(v + row * v_stride + hk * v_head_stride + f);
+        const uint32_t* x = reinterpret_cast<const uint32_t*>(&v4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 a = at_unpack<T>(x[i]);
+          nv = fmaf(a.x, a.x, fmaf(a.y, a.y, nv));
         }
       }
     }
+    dot = at_half_warp_sum(dot);
+    if (r < n && sub == 0) {
+      const float l = lse[int64_t(h) * p.tokens + row];
+      // a row without weight (lse = -inf) must give p = 0
+      w.row[int64_t(h) * p.tokens + row] = make_float2(l == -INFINITY ? INFINITY : l * AT_LOG2E, dot);
+    }
+    if (at_p_shift<T>() != 0.f) {
+      m_do = fmaxf(m_do, at_half_warp_sum(nd));
+      m_dl = fmaxf(m_dl, fabsf(dot));
+      m_v = fmaxf(m_v, at_half_warp_sum(nv));
+    }
   }
-  const int64_t off = (j * p.kv_heads + hk) * p.head_dim;
-  at_store(dk + off, lane, p.head_dim, gk, p.scale);
-  at_store(dv + off, lane, p.head_dim, gv, 1.f);
+  if (t.tail || at_p_shift<T>() == 0.f) return;
+  __shared__ float s_max[3][AT_PREP_THREADS / 16];
+  if (sub == 0) {
+    s_max[0][threadIdx.x >> 4] = m_do;
+    s_max[1][threadIdx.x >> 4] = m_dl;
+    s_max[2][threadIdx.x >> 4] = m_v;
+  }
+  __syncthreads();
+  if (threadIdx.x < 3) {
+    float m = 0.f;
+    for (int i = 0; i < AT_PREP_THREADS / 16; ++i) m = fmaxf(m, s_max[threadIdx.x][i]);
+    const int64_t at = int64_t(h) * p.slots + slot;
+    if (threadIdx.x == 0) w.tile[at].x = sqrtf(m);
+    if (threadIdx.x == 1) w.tile[at].y = m;
+    if (threadIdx.x == 2 && first) w.vmax[int64_t(hk) * p.slots + slot] = sqrtf(m);
+  }
+}
+
+// Whole warp: the exponent k of a (sequence, key/value head)'s dS scale.
+__device__ __forceinline__ int at_ds_exponent(const AttnParams& p, const AttnWork& w, const AttnTile& t, int slot, int hk) {
+  const int lane = threadIdx.x & 31, grp = p.heads / p.kv_heads;
+  const int first = slot - (t.i0 >> 7), tiles = (t.len + AT_TILE - 1) >> 7;
+  float m_do = 0.f, m_dl = 0.f, m_v = 0.f;
+  for (int g = 0; g < grp; ++g)
+    for (int i = lane; i < tiles; i += 32) {
+      const float2 x = w.tile[int64_t(hk * grp + g) * p.slots + first + i];
+      m_do = fmaxf(m_do, x.x);
+      m_dl = fmaxf(m_dl, x.y);
+    }
+  for (int i = lane; i < tiles; i += 32) m_v = fmaxf(m_v, w.vmax[int64_t(hk) * p.slots + first + i]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    m_do = fmaxf(m_do, __shfl_xor_sync(0xffffffffu, m_do, o));
+    m_dl = fmaxf(m_dl, __shfl_xor_sync(0xffffffffu, m_dl, o));
+    m_v = fmaxf(m_v, __shfl_xor_sync(0xffffffffu, m_v, o));
+  }
+  const float m = fmaf(m_do, m_v, m_dl);  // |dS| = p |dP - delta| <= |dO||V| + |delta|
+  if (!(m > 0.f) || !(m < INFINITY)) return 0;
+  const int e = int((__float_as_uint(m) >> 23) & 255u) - 127;
+  return min(max(14 - e, -100), 100);
+}
+__device__ __forceinline__ float at_pow2(int k) { return __uint_as_float(uint32_t(k + 127) << 23); }
+
+template <int DC>
+struct AttnBwdSmem {
+  static constexpr int TILE = DC * AT_BOX;
+  static constexpr int X = 0;
+  static constexpr int Y = TILE;
+  static constexpr int A = 2 * TILE;
+  static constexpr int B = 4 * TILE;
+  static constexpr int AUX = 6 * TILE;             // [2][128] lse, [2][128] -delta (scaled)
+  static constexpr int BAR = AUX + 4 * AT_TILE * 4;
+  // a_full[2], a_empty[2], b_full[2], b_empty[2], aux_full[2], aux_empty[2], xy_full, staged, s_full, p_ready,
+  // dp_full, ds_ready, done
+  static constexpr int NBAR = 19;
+  static constexpr int MISC = BAR + NBAR * 8;
+  static constexpr int ALLOC = MISC + 16 + 1024;  // slack to align the base to 1024 B
+};
+static_assert(AttnBwdSmem<2>::ALLOC <= 232448, "shared memory budget");
+
+// TMEM columns (512): S | P, dP | dS, and the two sums.
+constexpr int AT_TM_S = 0, AT_TM_DP = 128, AT_TM_DV = 256, AT_TM_DX = 384;
+
+// One warp's 32 rows of a sum in TMEM: `cols` columns from `c0` on, times f, to `row` (null: not stored).
+template <typename T>
+__device__ __forceinline__ void at_store_sum(uint32_t taddr, T* row, int c0, int cols, int head_dim, float f) {
+  for (int c = c0; c < c0 + cols && c < head_dim; c += 32) {
+    uint32_t o[32];
+    tmem_ld_32x32b_x32(taddr + c, o);
+    tmem_ld_wait();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint4 v;
+      uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        w[e] = at_pack<T>(__uint_as_float(o[k * 8 + 2 * e]) * f, __uint_as_float(o[k * 8 + 2 * e + 1]) * f);
+      if (row != nullptr && c + k * 8 < head_dim) *reinterpret_cast<uint4*>(row + c + k * 8) = v;
+    }
+  }
+}
+
+struct AttnBwdMaps {
+  CUtensorMap q, k, v, dout;
+};
+
+template <typename T, int DC, bool DKV>
+__device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const AttnParams& p, const AttnWork& w, int slot, int h,
+                                              T* __restrict__ g0, T* __restrict__ g1, uint8_t* smem, uint32_t sbase) {
+  using L = AttnBwdSmem<DC>;
+  uint64_t* a_full = reinterpret_cast<uint64_t*>(smem + L::BAR);
+  uint64_t* a_empty = a_full + 2;
+  uint64_t* b_full = a_empty + 2;
+  uint64_t* b_empty = b_full + 2;
+  uint64_t* aux_full = b_empty + 2;
+  uint64_t* aux_empty = aux_full + 2;
+  uint64_t* xy_full = aux_empty + 2;
+  uint64_t* staged = xy_full + 1;
+  uint64_t* s_full = staged + 1;
+  uint64_t* p_ready = s_full + 1;
+  uint64_t* dp_full = p_ready + 1;
+  uint64_t* ds_ready = dp_full + 1;
+  uint64_t* done = ds_ready + 1;
+  float* aux_lse = reinterpret_cast<float*>(smem + L::AUX);
+  float* aux_dl = aux_lse + 2 * AT_TILE;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int grp = p.heads / p.kv_heads, hk = DKV ? h : h / grp;
+
+  const AttnTile t = at_find(p, slot);
+  if (t.tail || t.i0 >= t.len) return;  // rows behind the last sequence: the prep launch's
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&a_full[i], 1);
+      mbar_init(&a_empty[i], 1);
+      mbar_init(&b_full[i], 1);
+      mbar_init(&b_empty[i], 1);
+      mbar_init(&aux_full[i], 32);
+      mbar_init(&aux_empty[i], 256);
+    }
+    mbar_init(xy_full, 1);
+    mbar_init(staged, 1);
+    mbar_init(s_full, 1);
+    mbar_init(p_ready, 256);
+    mbar_init(dp_full, 1);
+    mbar_init(ds_ready, 256);
+    mbar_init(done, 1);
+    fence_barrier_init();
+    *abort_flag = 0;
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // the ring's tiles (relative to a) and iterations
+  const int x_last = min(t.i0 + AT_TILE, t.len) - 1;
+  const int back = DKV ? p.right : p.left, ahead = DKV ? p.left : p.right;  // the window seen from X's side
+  const int y_lo = back < 0 ? 0 : max(0, t.i0 - back);
+  const int y_hi = ahead < 0 ? t.len - 1 : min(t.len - 1, x_last + ahead);
+  const int yt0 = y_lo >> 7, nt = (y_hi >> 7) - yt0 + 1;
+  const int n = DKV ? nt * grp : nt;
+  const int k_exp = at_p_shift<T>() != 0.f ? at_ds_exponent(p, w, t, slot, hk) : 0;
+  const float sc = at_pow2(k_exp - int(at_p_shift<T>()));
+
+  if (warp == 8) {
+    // ---------------------------------------------------------------- TMA
+    bool ok = true;
+    int issued = 0;
+    if (lane == 0) {
+      mbar_arrive_expect_tx(xy_full, 2 * L::TILE);
+      for (int c = 0; c < DC; ++c) {
+        tma_load_3d(sbase + L::X + c * AT_BOX, DKV ? &maps.k : &maps.q, xy_full, c * 64, h, t.a + t.i0);
+        tma_load_3d(sbase + L::Y + c * AT_BOX, DKV ? &maps.v : &maps.dout, xy_full, c * 64, h, t.a + t.i0);
+      }
+    }
+    uint32_t st_phase = 0;
+    for (int it = 0; it < n; ++it, ++issued) {
+      const int s = it & 1;
+      const uint32_t ph = ((it >> 1) & 1) ^ 1;
+      const int hy = DKV ? hk * grp + it / nt : hk;
+      const int y0 = (yt0 + (DKV ? it % nt : it)) * AT_TILE;
+      // rows of other sequences must add nothing to a sum over the ring tile's tokens: Q and dO in
+      // DKV CTAs, K in the others (V only meets rows that are masked)
+      const bool ragged = y0 + AT_TILE > t.len;
+      ok = at_wait(&a_empty[s], ph, abort_flag, 11) && at_wait(&b_empty[s], ph, abort_flag, 12);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      if (lane == 0) {
+        uint64_t* bar_a = ragged ? staged : &a_full[s];
+        uint64_t* bar_b = ragged && DKV ? staged : &b_full[s];
+        if (bar_a == bar_b) {
+          mbar_arrive_expect_tx(bar_a, 2 * L::TILE);
+        } else {
+          mbar_arrive_expect_tx(bar_a, L::TILE);
+          mbar_arrive_expect_tx(bar_b, L::TILE);
+        }
+        for (int c = 0; c < DC; ++c)
+          tma_load_3d(sbase + L::A + s * L::TILE + c * AT_BOX, DKV ? &maps.q : &maps.k, bar_a, c * 64, hy, t.a + y0);
+        for (int c = 0; c < DC; ++c)
+          tma_load_3d(sbase + L::B + s * L::TILE + c * AT_BOX, DKV ? &maps.dout : &maps.v, bar_b, c * 64, hy, t.a + y0);
+      }
+      if (DKV) {
+        ok = __all_sync(0xffffffffu, at_wait(&aux_empty[s], ph, abort_flag, 13));
+        if (ok) {
+          const float2* src = w.row + int64_t(hy) * p.tokens + t.a;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = e * 32 + lane;
+            const float2 x = y0 + r < t.len ? src[y0 + r] : make_float2(INFINITY, 0.f);  // p = 0 behind the end
+            aux_lse[s * AT_TILE + r] = x.x - at_p_shift<T>();
+            aux_dl[s * AT_TILE + r] = -x.y * sc;
+          }
+        }
+        mbar_arrive(&aux_full[s]);
+      }
+      if (ragged) {
+        ok = __all_sync(0xffffffffu, at_wait(staged, st_phase, abort_flag, 14)) && ok;
+        if (!ok) at_drain(staged, st_phase);
+        st_phase ^= 1;
+        at_zero_rows<DC>(smem + L::A + s * L::TILE, t.len - y0);
+        if (DKV) at_zero_rows<DC>(smem + L::B + s * L::TILE, t.len - y0);
+        if (lane == 0) {
+          mbar_arrive(&a_full[s]);
+          if (DKV) mbar_arrive(&b_full[s]);
+        }
+      }
+      if (!ok) {
+        ++issued;
+        break;
+      }
+    }
+    if (*abort_flag && lane == 0) {
+      at_drain(xy_full, 0);
+      for (int it = max(0, issued - 2); it < issued; ++it) {
+        at_drain(&a_full[it & 1], (it >> 1) & 1);
+        at_drain(&b_full[it & 1], (it >> 1) & 1);
+      }
+    }
+  } else if (warp == 9) {
+    // ---------------------------------------------------------------- MMA
+    if (lane == 0) {
+      const int kd = (p.head_dim + 15) / 16;
+      const uint32_t id_s = at_idesc<T>(AT_TILE, false);
+      const uint32_t id_g = at_idesc<T>(kd * 16, true);
+      const uint64_t dx = smem_desc_sw128(sbase + L::X, 16, 1024), dy = smem_desc_sw128(sbase + L::Y, 16, 1024);
+      const uint64_t da = smem_desc_sw128(sbase + L::A, 16, 1024), db = smem_desc_sw128(sbase + L::B, 16, 1024);
+      const uint64_t ta = smem_desc_sw128(sbase + L::A, AT_BOX, 1024), tb = smem_desc_sw128(sbase + L::B, AT_BOX, 1024);
+      // d (128 x 128) = x a^T over head_dim
+      auto scores = [&](uint32_t d, uint64_t x, uint64_t a) {
+        for (int k = 0; k < kd; ++k) {
+          const uint64_t off = uint64_t((k >> 2) * (AT_BOX >> 4) + (k & 3) * 2);
+          umma_f16(d, x + off, a + off, id_s, k > 0);
+        }
+      };
+      // d (128 x head_dim) += p b over the ring tile's 128 tokens; each half of the columns of p lies
+      // at the start of its own half of the scores it overwrote
+      auto sum = [&](uint32_t d, uint32_t pm, uint64_t b, bool acc) {
+#pragma unroll
+        for (int k = 0; k < AT_TILE / 16; ++k)
+          umma_f16_ts(d, pm + (k >> 2) * 64 + (k & 3) * 8, b + uint64_t(k * (2048 >> 4)), id_g, acc || k > 0);
+      };
+      constexpr uint64_t STEP = uint64_t(L::TILE >> 4);
+      bool ok = at_wait(xy_full, 0, abort_flag, 15) && at_wait(&a_full[0], 0, abort_flag, 16);
+      if (ok) {
+        tc_fence_after();
+        scores(tmem + AT_TM_S, dx, da);
+        umma_commit(s_full);
+        ok = at_wait(&b_full[0], 0, abort_flag, 17);
+      }
+      if (ok) {
+        tc_fence_after();
+        scores(tmem + AT_TM_DP, dy, db);
+        umma_commit(dp_full);
+        if (!DKV) umma_commit(&b_empty[0]);
+      }
+      for (int it = 0; ok && it < n; ++it) {
+        const int s = it & 1, s1 = s ^ 1;
+        const uint32_t ph = it & 1, ph1 = ((it + 1) >> 1) & 1;
+        const bool more = it + 1 < n;
+        ok = at_wait(p_ready, ph, abort_flag, 18);
+        if (!ok) break;
+        tc_fence_after();
+        if (DKV) {
+          sum(tmem + AT_TM_DV, tmem + AT_TM_S, tb + s * STEP, it > 0);
+          umma_commit(&b_empty[s]);
+        }
+        if (more) {
+          ok = at_wait(&a_full[s1], ph1, abort_flag, 19);
+          if (!ok) break;
+          tc_fence_after();
+          scores(tmem + AT_TM_S, dx, da + s1 * STEP);  // after the product that reads P: MMAs run in order
+          umma_commit(s_full);
+        }
+        ok = at_wait(ds_ready, ph, abort_flag, 20);
+        if (!ok) break;
+        tc_fence_after();
+        sum(tmem + AT_TM_DX, tmem + AT_TM_DP, ta + s * STEP, it > 0);
+        umma_commit(&a_empty[s]);
+        if (more) {
+          ok = at_wait(&b_full[s1], ph1, abort_flag, 21);
+          if (!ok) break;
+          tc_fence_after();
+          scores(tmem + AT_TM_DP, dy, db + s1 * STEP);
+          umma_commit(dp_full);
+          if (!DKV) umma_commit(&b_empty[s1]);
+        }
+      }
+      umma_commit(done);
+      at_drain(done, 0);  // nothing in flight when TMEM and shared memory go
+    }
+  } else {
+    // ---------------------------------------------------------------- elementwise
+    const int half = warp >> 2;  // columns [64 half, 64 half + 64)
+    const int r = (warp & 3) * 32 + lane;
+    const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + AT_TM_S + lane_off + half * 64, t_dp = tmem + AT_TM_DP + lane_off + half * 64;
+    const int x = t.i0 + r;  // this thread's row, relative to a
+    const float sl2 = p.scale * AT_LOG2E;
+    const int see_lo = back < 0 ? 0 : x - back;
+    const int see_hi = ahead < 0 ? t.len - 1 : min(t.len - 1, x + ahead);
+    float row_lse = 0.f, row_dl = 0.f;
+    if (!DKV) {
+      const float2 v = x < t.len ? w.row[int64_t(h) * p.tokens + t.a + x] : make_float2(INFINITY, 0.f);
+      row_lse = -(v.x - at_p_shift<T>());
+      row_dl = -v.y * sc;
+    }
+    bool ok = true;
+    for (int it = 0; it < n; ++it) {
+      const int s = it & 1;
+      const int y0 = (yt0 + (DKV ? it % nt : it)) * AT_TILE + half * 64;
+      ok = at_wait(s_full, it & 1, abort_flag, 22);
+      if (DKV) ok = ok && at_wait(&aux_full[s], (it >> 1) & 1, abort_flag, 23);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      const bool cut = y0 + 64 > t.len || (ahead >= 0 && y0 + 63 > t.i0 + ahead) ||
+                       (back >= 0 && y0 < t.i0 + AT_TILE - 1 - back);
+      uint32_t sv[64];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(t_s + c * 32, *reinterpret_cast<uint32_t(*)[32]>(sv + c * 32));
+      tmem_ld_wait();
+      if (!DKV) {
+        tc_fence_before();
+        mbar_arrive(p_ready);  // the scores are in registers: the next tile's may overwrite them
+      }
+      float pv[64];
+      const float4* la = reinterpret_cast<const float4*>(aux_lse + s * AT_TILE + half * 64);
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        float4 l4 = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (DKV) l4 = la[c];
+        const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          pv[c * 4 + e] = at_exp2(fmaf(__uint_as_float(sv[c * 4 + e]), sl2, DKV ? -lv[e] : row_lse));
+      }
+      if (cut) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if (y0 + c < see_lo || y0 + c > see_hi) pv[c] = 0.f;
+      }
+      if (DKV) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) pk[k] = at_pack<T>(pv[2 * k], pv[2 * k + 1]);  // the MMA's operand type
+        tmem_st_32x32b_x32(t_s, pk);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(p_ready);
+      }
+      ok = at_wait(dp_full, it & 1, abort_flag, 24);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      uint32_t dv[64];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(t_dp + c * 32, *reinterpret_cast<uint32_t(*)[32]>(dv + c * 32));
+      tmem_ld_wait();
+      const float4* ld = reinterpret_cast<const float4*>(aux_dl + s * AT_TILE + half * 64);
+      uint32_t pk[32];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        float4 d4 = make_float4(row_dl, row_dl, row_dl, row_dl);
+        if (DKV) d4 = ld[c];
+        const float dl[4] = {d4.x, d4.y, d4.z, d4.w};
+        float ds[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          ds[e] = pv[c * 4 + e] * fmaf(__uint_as_float(dv[c * 4 + e]), sc, dl[e]);
+          // a hidden pair adds nothing, whatever its dP is
+          if (cut && (y0 + c * 4 + e < see_lo || y0 + c * 4 + e > see_hi)) ds[e] = 0.f;
+        }
+        pk[2 * c] = at_pack<T>(ds[0], ds[1]);
+        pk[2 * c + 1] = at_pack<T>(ds[2], ds[3]);
+      }
+      tmem_st_32x32b_x32(t_dp, pk);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(ds_ready);
+      if (DKV) mbar_arrive(&aux_empty[s]);
+    }
+    if (__all_sync(0xffffffffu, ok)) ok = at_wait(done, 0, abort_flag, 25);
+    if (__all_sync(0xffffffffu, ok)) {
+      tc_fence_after();
+      const int64_t off = (int64_t(t.a + x) * (DKV ? p.kv_heads : p.heads) + h) * p.head_dim;
+      const bool live = x < t.len;
+      const float fx = p.scale * at_pow2(-k_exp);
+      if (DKV) {
+        if (half == 0)
+          at_store_sum<T>(tmem + AT_TM_DV + lane_off, live ? g1 + off : nullptr, 0, p.head_dim, p.head_dim,
+                          at_pow2(-int(at_p_shift<T>())));
+        else
+          at_store_sum<T>(tmem + AT_TM_DX + lane_off, live ? g0 + off : nullptr, 0, p.head_dim, p.head_dim, fx);
+      } else {
+        at_store_sum<T>(tmem + AT_TM_DX + lane_off, live ? g0 + off : nullptr, half * DC * 32, DC * 32, p.head_dim, fx);
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+template <typename T, int DC>
+__global__ void __launch_bounds__(AT_BWD_THREADS, 1)
+    attn_bwd_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_constant__ AttnParams p, const AttnWork w,
+                    T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dv) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  grid_dep_wait();  // programmatic launch: no global access before the wait
+  // the CTAs of key tiles first (a group's heads each: the longer ones), a causal sequence's first
+  // tiles, which the most queries see, before its last; the query tiles the other way round
+  const unsigned n_dkv = unsigned(p.slots) * unsigned(p.kv_heads);
+  if (blockIdx.x < n_dkv) {
+    attn_bwd_role<T, DC, true>(maps, p, w, blockIdx.x / p.kv_heads, blockIdx.x % p.kv_heads, dk, dv, smem, smem_u32(smem));
+  } else {
+    const unsigned b = blockIdx.x - n_dkv;
+    attn_bwd_role<T, DC, false>(maps, p, w, p.slots - 1 - int(b / p.heads), b % p.heads, dq, nullptr, smem,
+                                smem_u32(smem));
+  }
 }
 
 static bool attn_strides_ok(int64_t stride, int64_t head_stride, const nf4b_attn& a, int heads) {
@@ -418,7 +826,7 @@ static int attn_checks(const nf4b_attn* in, nf4b_attn* a) {
   NF4B_RETURN_IF(a->head_dim % 8 != 0 || a->head_dim > AT_MAX_DIM, NF4B_ERR_UNSUPPORTED);
   NF4B_RETURN_IF(a->tokens > 0x3FFFFFFF || a->rows > 0x3FFFFFFF || a->heads > 65535, NF4B_ERR_UNSUPPORTED);
   // CTAs of a launch
-  NF4B_RETURN_IF(at_slots(a->tokens, a->rows) * a->heads > 0x7FFFFFFF, NF4B_ERR_UNSUPPORTED);
+  NF4B_RETURN_IF(at_slots(a->tokens, a->rows) * (a->heads + a->kv_heads) > 0x7FFFFFFF, NF4B_ERR_UNSUPPORTED);
   if (a->tokens == 0) return NF4B_OK;
   NF4B_RETURN_IF(!a->q || !a->k || !a->v || !a->cu, NF4B_ERR_INVALID_ARG);
   NF4B_RETURN_IF(!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->cu, 4), NF4B_ERR_ALIGNMENT);
@@ -506,23 +914,45 @@ extern "C" int nf4b_attn_error_flag(int* value, int reset) {
   return NF4B_OK;
 }
 
+static int64_t attn_work(int64_t tokens, int64_t slots, int64_t heads, int64_t kv_heads, void* base, AttnWork* w) {
+  const int64_t rows = heads * tokens * 8, tiles = heads * slots * 8, vmax = kv_heads * slots * 4;
+  if (w != nullptr) {
+    char* b = static_cast<char*>(base);
+    w->row = reinterpret_cast<float2*>(b);
+    w->tile = reinterpret_cast<float2*>(b + rows);
+    w->vmax = reinterpret_cast<float*>(b + rows + tiles);
+  }
+  return (rows + tiles + vmax + 15) / 16 * 16;
+}
+
 extern "C" int64_t nf4b_attn_bwd_work_bytes(int64_t tokens, int32_t rows, int32_t heads, int32_t kv_heads) {
   if (tokens < 0 || rows < 0 || heads <= 0 || kv_heads <= 0 || tokens > 0x3FFFFFFF || rows > 0x3FFFFFFF ||
       heads > 65535 || heads % kv_heads != 0)
     return -1;
-  return (tokens * heads * 4 + 15) / 16 * 16;
+  return attn_work(tokens, at_slots(tokens, rows), heads, kv_heads, nullptr, nullptr);
 }
 
-template <typename T>
+template <typename T, int DC>
 static int attn_bwd_launch(const nf4b_attn& a, const void* out, const float* lse, const void* dout, void* dq, void* dk,
-                           void* dv, float* delta, cudaStream_t s) {
-  const unsigned gq = unsigned((a.tokens * a.heads + AT_WARPS - 1) / AT_WARPS);
-  const unsigned gk = unsigned((a.tokens * a.kv_heads + AT_WARPS - 1) / AT_WARPS);
-  attn_dq_kernel<T><<<gq, 32 * AT_WARPS, 0, s>>>(a, static_cast<const T*>(out), lse, static_cast<const T*>(dout),
-                                                 static_cast<T*>(dq), delta);
-  attn_dkv_kernel<T><<<gk, 32 * AT_WARPS, 0, s>>>(a, lse, static_cast<const T*>(dout), delta, static_cast<T*>(dk),
-                                                  static_cast<T*>(dv));
-  return launch_status("attn backward launch");
+                           void* dv, void* work, cudaStream_t s) {
+  AttnBwdMaps m;
+  int st = attn_tmap(&m.q, a, a.q, a.heads, a.q_stride, a.q_head_stride);
+  if (st == NF4B_OK) st = attn_tmap(&m.k, a, a.k, a.kv_heads, a.k_stride, a.k_head_stride);
+  if (st == NF4B_OK) st = attn_tmap(&m.v, a, a.v, a.kv_heads, a.v_stride, a.v_head_stride);
+  if (st == NF4B_OK) st = attn_tmap(&m.dout, a, dout, a.heads, int64_t(a.heads) * a.head_dim, a.head_dim);
+  static bool done[64] = {false};
+  if (st == NF4B_OK) st = attn_smem(attn_bwd_kernel<T, DC>, AttnBwdSmem<DC>::ALLOC, done);
+  if (st != NF4B_OK) return st;
+  const AttnParams p = attn_params(a);
+  AttnWork w;
+  attn_work(a.tokens, p.slots, a.heads, a.kv_heads, work, &w);
+  T *tq = static_cast<T*>(dq), *tk = static_cast<T*>(dk), *tv = static_cast<T*>(dv);
+  NF4B_CUDA_TRY(launch_pdl(attn_prep_kernel<T>, dim3(unsigned(p.slots) * unsigned(a.heads)), dim3(AT_PREP_THREADS),
+                           size_t(0), s, p, static_cast<const T*>(out), static_cast<const T*>(dout), lse,
+                           static_cast<const T*>(a.v), a.v_stride, a.v_head_stride, w, tq, tk, tv));
+  NF4B_CUDA_TRY(launch_pdl(attn_bwd_kernel<T, DC>, dim3(unsigned(p.slots) * unsigned(a.heads + a.kv_heads)),
+                           dim3(AT_BWD_THREADS), size_t(AttnBwdSmem<DC>::ALLOC), s, m, p, w, tq, tk, tv));
+  return launch_status("attn_bwd_kernel launch");
 }
 
 extern "C" int nf4b_attn_bwd(const nf4b_attn* args, const void* out, const float* lse, const void* dout, void* dq,
@@ -538,11 +968,13 @@ extern "C" int nf4b_attn_bwd(const nf4b_attn* args, const void* out, const float
   const int64_t need = nf4b_attn_bwd_work_bytes(a.tokens, a.rows, a.heads, a.kv_heads);
   NF4B_RETURN_IF(need < 0, NF4B_ERR_UNSUPPORTED);
   NF4B_RETURN_IF(work_bytes < need, NF4B_ERR_INVALID_ARG);
-  NF4B_RETURN_IF(a.tokens * a.heads / AT_WARPS >= 0x7FFFFFFF, NF4B_ERR_UNSUPPORTED);
   st = check_device();
   if (st != NF4B_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  float* delta = static_cast<float*>(work);
-  return a.dtype == NF4B_F16 ? attn_bwd_launch<__half>(a, out, lse, dout, dq, dk, dv, delta, s)
-                             : attn_bwd_launch<__nv_bfloat16>(a, out, lse, dout, dq, dk, dv, delta, s);
+  const bool wide = a.head_dim > 64;
+  if (a.dtype == NF4B_F16)
+    return wide ? attn_bwd_launch<__half, 2>(a, out, lse, dout, dq, dk, dv, work, s)
+                : attn_bwd_launch<__half, 1>(a, out, lse, dout, dq, dk, dv, work, s);
+  return wide ? attn_bwd_launch<__nv_bfloat16, 2>(a, out, lse, dout, dq, dk, dv, work, s)
+              : attn_bwd_launch<__nv_bfloat16, 1>(a, out, lse, dout, dq, dk, dv, work, s);
 }
