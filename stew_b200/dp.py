@@ -12,14 +12,13 @@ G-rank step equals a 1-rank step over the concatenated batches.
 from __future__ import annotations
 
 import math
-
-import ctypes
-from itertools import chain
+from array import array
 
 import torch
 import torch.distributed as dist
 
 from . import _lib
+from .nf4 import _launch
 
 
 def _world(group) -> int:
@@ -29,6 +28,8 @@ def _world(group) -> int:
 
 
 _GRAD_DTYPE = {torch.float32: _lib.NF4B_F32, torch.float16: _lib.NF4B_F16, torch.bfloat16: _lib.NF4B_BF16}
+_PTR, _NUMEL, _INDEX = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
+_CONTIGUOUS, _DTYPE = torch.Tensor.is_contiguous, torch.Tensor.dtype.__get__
 
 
 def clip_grads(grads, max_norm: float, divisor: torch.Tensor | None = None, out=None) -> torch.Tensor:
@@ -54,36 +55,38 @@ def clip_grads(grads, max_norm: float, divisor: torch.Tensor | None = None, out=
     dev = grads[0].device
     if dev.type != "cuda":
         raise _lib.NF4Unsupported(_lib.NF4B_ERR_UNSUPPORTED, f"clip_grads: gradients on {dev} (CUDA only)")
-    table = []
-    for g, o in zip(grads, dst):
-        dt = _GRAD_DTYPE.get(g.dtype)
-        if dt is None:
-            raise _lib.NF4Unsupported(_lib.NF4B_ERR_UNSUPPORTED, f"clip_grads: {g.dtype} gradient")
-        n = g.numel()
-        if g.device != dev or not g.is_contiguous():
-            raise ValueError("clip_grads: gradients must be contiguous and on one device")
-        if o is not g and (o.dtype != g.dtype or o.numel() != n or o.device != dev or not o.is_contiguous()):
-            raise ValueError("clip_grads: an output must be contiguous, of its gradient's type, size and device")
-        table.append((g.data_ptr(), o.data_ptr(), n, dt))
-    used = [t[1] for t in table if t[2]]
-    if len(set(used)) != len(used):
-        raise ValueError("clip_grads: one tensor is the output of two gradients")
+    # one C-level pass per property: a call over a hundred tensors is bound by this
+    src, sizes, types = list(map(_PTR, grads)), list(map(_NUMEL, grads)), list(map(_DTYPE, grads))
+    kinds = set(types)
+    if not kinds <= _GRAD_DTYPE.keys():
+        raise _lib.NF4Unsupported(_lib.NF4B_ERR_UNSUPPORTED, f"clip_grads: {kinds - _GRAD_DTYPE.keys()} gradients")
+    if set(map(_INDEX, grads)) != {dev.index} or not all(map(_CONTIGUOUS, grads)):
+        raise ValueError("clip_grads: gradients must be contiguous and on one device")
+    to = src
     if out is not None:
-        read = {t[0] for t in table if t[2]}
-        if any(t[1] != t[0] and t[1] in read for t in table if t[2]):
+        to = list(map(_PTR, dst))
+        if (set(map(_INDEX, dst)) != {dev.index} or not all(map(_CONTIGUOUS, dst))
+                or list(map(_DTYPE, dst)) != types or list(map(_NUMEL, dst)) != sizes):
+            raise ValueError("clip_grads: an output must be contiguous, of its gradient's type, size and device")
+        if to != src and not set(to).isdisjoint(src) and any(
+                t != s and t in src for s, t, n in zip(src, to, sizes) if n):
             raise ValueError("clip_grads: an output is another gradient of the list")
+    if len(set(to)) != len(to) and len({t for t, n in zip(to, sizes) if n}) != sum(map(bool, sizes)):
+        raise ValueError("clip_grads: one tensor is the output of two gradients")
     if divisor is not None and (divisor.dtype != torch.float32 or divisor.numel() != 1 or divisor.device != dev):
         raise ValueError("clip_grads: divisor must be one fp32 value on the gradients' device")
-    L = _lib.lib()
-    wb = int(L.nf4b_clip_grads_work_bytes(len(table)))
     # nf4b_grad is four 64-bit words: src, dst, numel, and dtype beside a reserved half
-    arr = (ctypes.c_int64 * (4 * len(table)))(*chain.from_iterable(table))
-    with torch.cuda.device(dev):
-        norm = torch.empty((), dtype=torch.float32, device=dev)
-        work = torch.empty(wb, dtype=torch.uint8, device=dev)
-        _lib.check(L.nf4b_clip_grads(arr, len(table), max_norm, None if divisor is None else divisor.data_ptr(),
-                                     norm.data_ptr(), work.data_ptr(), wb, torch.cuda.current_stream(dev).cuda_stream),
-                   "nf4b_clip_grads")
+    n = len(src)
+    table = array("Q", bytes(32 * n))
+    table[0::4], table[1::4], table[2::4] = array("Q", src), array("Q", to), array("Q", sizes)
+    code = _GRAD_DTYPE[types[0]]
+    table[3::4] = array("Q", [code]) * n if len(kinds) == 1 else array("Q", [_GRAD_DTYPE[t] for t in types])
+    L = _lib.lib()
+    wb = L.nf4b_clip_grads_work_bytes(n)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    work = torch.empty(wb, dtype=torch.uint8, device=dev)
+    _launch(L.nf4b_clip_grads, "nf4b_clip_grads", dev, table.buffer_info()[0], n, max_norm,
+            None if divisor is None else divisor.data_ptr(), norm.data_ptr(), work.data_ptr(), wb)
     return norm
 
 

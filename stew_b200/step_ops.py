@@ -9,12 +9,13 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .nf4 import _stream
+from .nf4 import _launch, _stream
 
 
 def _c(t: torch.Tensor) -> torch.Tensor:
@@ -159,78 +160,73 @@ ATTN_MAX_HEAD_DIM = 128
 _ATTN_DTYPE = {torch.float16: _lib.NF4B_F16, torch.bfloat16: _lib.NF4B_BF16}
 
 
-def _attn_layout(t: torch.Tensor) -> torch.Tensor:
-    """t [tokens, heads, head_dim] as the kernels read it: contiguous features, strides that are
-    multiples of 8 elements, a 16-byte aligned base (slices of one projection output stay as they
-    are; anything else, a broadcast view too, is copied)."""
-    n, h, d = t.shape
-    if (t.stride(2) == 1 and (n == 1 or (t.stride(0) >= d and t.stride(0) % 8 == 0))
-            and (h == 1 or (t.stride(1) >= d and t.stride(1) % 8 == 0)) and t.data_ptr() % 16 == 0):
-        return t
-    return _aligned_c(t)
-
-
 def _aligned_c(t: torch.Tensor) -> torch.Tensor:
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _attn_c(q, k, v, cu, left, right, scale) -> _lib.AttnC:
-    n, hq, d = q.shape
-    hk = k.shape[1]
-    a = _lib.AttnC()
-    a.q, a.k, a.v, a.cu = q.data_ptr(), k.data_ptr(), v.data_ptr(), cu.data_ptr()
-    a.tokens, a.rows, a.heads, a.kv_heads, a.head_dim = n, cu.numel() - 1, hq, hk, d
+def _attn_layout(t: torch.Tensor) -> tuple:
+    """(t, token stride, head stride) of t [tokens, heads, head_dim] as the kernels read it:
+    contiguous features, strides that are multiples of 8 elements, a 16-byte aligned base (slices
+    of one projection output stay as they are; anything else, a broadcast view too, is copied)."""
+    n, h, d = t.shape
+    st, sh, sd = t.stride()
     # a dimension of one element may carry any stride
-    a.q_stride, a.q_head_stride = (q.stride(0) if n > 1 else hq * d), (q.stride(1) if hq > 1 else d)
-    a.k_stride, a.k_head_stride = (k.stride(0) if n > 1 else hk * d), (k.stride(1) if hk > 1 else d)
-    a.v_stride, a.v_head_stride = (v.stride(0) if n > 1 else hk * d), (v.stride(1) if hk > 1 else d)
-    a.dtype, a.left, a.right, a.scale = _ATTN_DTYPE[q.dtype], left, right, scale
-    return a
+    st, sh = (st if n > 1 else h * d), (sh if h > 1 else d)
+    if sd == 1 and st >= d and sh >= d and not (st | sh) & 7 and not t.data_ptr() & 15:
+        return t, st, sh
+    return _aligned_c(t), h * d, d
+
+
+# nf4b_attn as one packed record (a quarter of the time of filling a ctypes structure)
+_ATTN_RECORD = struct.Struct("=4Q7q7if")
+assert _ATTN_RECORD.size == ctypes.sizeof(_lib.AttnC)
+
+
+def _attn_record(q, qs, k, ks, v, vs, cu, left, right, scale) -> bytes:
+    n, hq, d = q.shape
+    return _ATTN_RECORD.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu.data_ptr(), n, *qs, *ks, *vs,
+                             cu.numel() - 1, hq, k.shape[1], d, _ATTN_DTYPE[q.dtype], left, right, scale)
 
 
 def _attn_forward(q, k, v, cu, left, right, scale):
-    q, k, v = _attn_layout(q), _attn_layout(k), _attn_layout(v)
-    n, hq, d = q.shape
-    dev = q.device
-    out = torch.empty(n, hq, d, dtype=q.dtype, device=dev)
-    lse = torch.empty(hq, n, dtype=torch.float32, device=dev)
+    """(out, lse, q, k, v as read, the call's nf4b_attn record)."""
+    q, *qs = _attn_layout(q)
+    k, *ks = _attn_layout(k)
+    v, *vs = _attn_layout(v)
+    n, hq, _ = q.shape
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((hq, n), dtype=torch.float32, device=q.device)
+    rec = _attn_record(q, qs, k, ks, v, vs, cu, left, right, scale)
     if n:
-        with torch.cuda.device(dev):
-            a = _attn_c(q, k, v, cu, left, right, scale)
-            _lib.check(_lib.lib().nf4b_attn_fwd(ctypes.byref(a), out.data_ptr(), lse.data_ptr(), _stream(dev)),
-                       "nf4b_attn_fwd")
-    return q, k, v, out, lse
+        _launch(_lib.lib().nf4b_attn_fwd, "nf4b_attn_fwd", q.device, rec, out.data_ptr(), lse.data_ptr())
+    return out, lse, q, k, v, rec
 
 
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu, left, right, scale):
-        q, k, v, out, lse = _attn_forward(q, k, v, cu, left, right, scale)
+        out, lse, q, k, v, ctx.rec = _attn_forward(q, k, v, cu, left, right, scale)
         ctx.save_for_backward(q, k, v, cu, out, lse)
-        ctx.args = (left, right, scale)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, cu, out, lse = ctx.saved_tensors
-        n, hq, d = q.shape
-        hk = k.shape[1]
-        dev = q.device
-        dout = _aligned_c(dout.to(q.dtype))
-        dq = torch.empty(n, hq, d, dtype=q.dtype, device=dev)
-        dk = torch.empty(n, hk, d, dtype=q.dtype, device=dev)
-        dv = torch.empty(n, hk, d, dtype=q.dtype, device=dev)
+        dev, dt = q.device, q.dtype
+        n, hq, _ = q.shape
+        dout = _aligned_c(dout if dout.dtype == dt else dout.to(dt))
+        dq = torch.empty(q.shape, dtype=dt, device=dev)
+        dk = torch.empty(k.shape, dtype=dt, device=dev)
+        dv = torch.empty(v.shape, dtype=dt, device=dev)
         if n:
             L = _lib.lib()
-            with torch.cuda.device(dev):
-                a = _attn_c(q, k, v, cu, *ctx.args)
-                wb = int(L.nf4b_attn_bwd_work_bytes(n, a.rows, hq, hk))
-                work = torch.empty(max(wb, 16), dtype=torch.uint8, device=dev)
-                _lib.check(L.nf4b_attn_bwd(ctypes.byref(a), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
-                                           dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), work.data_ptr(), wb,
-                                           _stream(dev)), "nf4b_attn_bwd")
+            wb = L.nf4b_attn_bwd_work_bytes(n, cu.numel() - 1, hq, k.shape[1])
+            work = torch.empty(wb, dtype=torch.uint8, device=dev)
+            # the record's addresses are those of the saved tensors, which the graph keeps alive
+            _launch(L.nf4b_attn_bwd, "nf4b_attn_bwd", dev, ctx.rec, out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
+                    dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), work.data_ptr(), wb)
         return dq, dk, dv, None, None, None, None
 
 
@@ -254,11 +250,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torc
     contiguous features are read in place when they are multiples of 8 elements, else copied.
     The backward recomputes the probabilities from the saved log-sum-exp; forward and backward
     give the same bits on every run.  Second derivatives are refused."""
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 3:
-            raise ValueError(f"packed_attention: {name} must be [tokens, heads, head_dim], got {tuple(t.shape)}")
-        if t.dtype != q.dtype or t.device != q.device:
-            raise ValueError("packed_attention: q, k and v must share one type and device")
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError("packed_attention: q, k and v must be [tokens, heads, head_dim]")
+    if not (q.dtype == k.dtype == v.dtype and q.device == k.device == v.device):
+        raise ValueError("packed_attention: q, k and v must share one type and device")
     n, hq, d = q.shape
     if k.shape != v.shape or k.shape[0] != n or k.shape[2] != d:
         raise ValueError(f"packed_attention: k {tuple(k.shape)} and v {tuple(v.shape)} do not fit q {tuple(q.shape)}")
@@ -280,7 +275,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torc
         raise ValueError(f"packed_attention: scale must be positive and finite, got {scale}")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _PackedAttention.apply(q, k, v, cu, left, right, scale)
-    return _attn_forward(q, k, v, cu, left, right, scale)[3]
+    return _attn_forward(q, k, v, cu, left, right, scale)[0]
 
 
 # The backward's softmax - onehot is written as fp16 times this power of two (exact to divide
