@@ -7,6 +7,7 @@
 // Every product runs on tcgen05 over 128-token tiles that TMA brings in; a ragged tile's rows of other
 // sequences are zeroed in shared memory where a product sums over them, and masked elsewhere.
 // Sums and softmax statistics are fp32 (TMEM, registers), in a fixed order.
+#include <cstdlib>
 #include <mutex>
 
 #include "attn_common.cuh"
@@ -442,6 +443,13 @@ struct AttnBwdSmem {
 };
 static_assert(AttnBwdSmem<2>::ALLOC <= 232448, "shared memory budget");
 
+// Row pitch (floats) of a DKV CTA's sums in shared memory, dK beside dV: 16 bytes more than the
+// features, so the 16-byte stores of a warp's 32 rows fall into different banks.
+template <int DC>
+constexpr int AT_JOIN_PITCH = 2 * DC * 64 + 4;
+static_assert(AT_TILE * AT_JOIN_PITCH<2> * 4 <= AttnBwdSmem<2>::AUX && AT_TILE * AT_JOIN_PITCH<1> * 4 <= AttnBwdSmem<1>::AUX,
+              "the sums fit where the tiles were");
+
 // TMEM columns (512): S | P, dP | dS, and the two sums.
 constexpr int AT_TM_S = 0, AT_TM_DP = 128, AT_TM_DV = 256, AT_TM_DX = 384;
 
@@ -464,13 +472,20 @@ __device__ __forceinline__ void at_store_sum(uint32_t taddr, T* row, int c0, int
   }
 }
 
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
+  return v;
+}
+
 struct AttnBwdMaps {
   CUtensorMap q, k, v, dout;
 };
 
 template <typename T, int DC, bool DKV>
 __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const AttnParams& p, const AttnWork& w, int slot, int h,
-                                              T* __restrict__ g0, T* __restrict__ g1, uint8_t* smem, uint32_t sbase) {
+                                              int split, int rank, T* __restrict__ g0, T* __restrict__ g1, uint8_t* smem,
+                                              uint32_t sbase) {
   using L = AttnBwdSmem<DC>;
   uint64_t* a_full = reinterpret_cast<uint64_t*>(smem + L::BAR);
   uint64_t* a_empty = a_full + 2;
@@ -529,9 +544,16 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
   const int y_lo = back < 0 ? 0 : max(0, t.i0 - back);
   const int y_hi = ahead < 0 ? t.len - 1 : min(t.len - 1, x_last + ahead);
   const int yt0 = y_lo >> 7, nt = (y_hi >> 7) - yt0 + 1;
-  const int n = DKV ? nt * grp : nt;
-  const int k_exp = at_p_shift<T>() != 0.f ? at_ds_exponent(p, w, t, slot, hk) : 0;
-  const float sc = at_pow2(k_exp - int(at_p_shift<T>()));
+  // a DKV CTA's share of the group's heads
+  const int n = DKV ? nt * (grp / split) : nt;
+  const int h0 = DKV ? hk * grp + rank * (grp / split) : 0;
+  int k_exp = 0;
+  float sc = at_pow2(-int(at_p_shift<T>()));
+  auto ds_scale = [&] {
+    if (at_p_shift<T>() == 0.f) return;
+    k_exp = at_ds_exponent(p, w, t, slot, hk);
+    sc = at_pow2(k_exp - int(at_p_shift<T>()));
+  };
 
   if (warp == 8) {
     // ---------------------------------------------------------------- TMA
@@ -548,7 +570,7 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
     for (int it = 0; it < n; ++it, ++issued) {
       const int s = it & 1;
       const uint32_t ph = ((it >> 1) & 1) ^ 1;
-      const int hy = DKV ? hk * grp + it / nt : hk;
+      const int hy = DKV ? h0 + it / nt : hk;
       const int y0 = (yt0 + (DKV ? it % nt : it)) * AT_TILE;
       // rows of other sequences must add nothing to a sum over the ring tile's tokens: Q and dO in
       // DKV CTAs, K in the others (V only meets rows that are masked)
@@ -570,6 +592,7 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
           tma_load_3d(sbase + L::B + s * L::TILE + c * AT_BOX, DKV ? &maps.dout : &maps.v, bar_b, c * 64, hy, t.a + y0);
       }
       if (DKV) {
+        if (it == 0) ds_scale();  // while the first tiles are on their way
         ok = __all_sync(0xffffffffu, at_wait(&aux_empty[s], ph, abort_flag, 13));
         if (ok) {
           const float2* src = w.row + int64_t(hy) * p.tokens + t.a;
@@ -689,6 +712,7 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
     const int see_lo = back < 0 ? 0 : x - back;
     const int see_hi = ahead < 0 ? t.len - 1 : min(t.len - 1, x + ahead);
     float row_lse = 0.f, row_dl = 0.f;
+    ds_scale();
     if (!DKV) {
       const float2 v = x < t.len ? w.row[int64_t(h) * p.tokens + t.a + x] : make_float2(INFINITY, 0.f);
       row_lse = -(v.x - at_p_shift<T>());
@@ -773,7 +797,23 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
       const int64_t off = (int64_t(t.a + x) * (DKV ? p.kv_heads : p.heads) + h) * p.head_dim;
       const bool live = x < t.len;
       const float fx = p.scale * at_pow2(-k_exp);
-      if (DKV) {
+      if (DKV && split > 1) {
+        // fp32 to this CTA's shared memory (its tiles are done with): [128 rows][dK | dV]
+        const uint32_t from = tmem + (half == 0 ? AT_TM_DX : AT_TM_DV) + lane_off;
+        const float f = half == 0 ? fx : at_pow2(-int(at_p_shift<T>()));
+        float* row = reinterpret_cast<float*>(smem) + r * AT_JOIN_PITCH<DC> + half * DC * 64;
+#pragma unroll 1
+        for (int c = 0; c < DC * 64; c += 32) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(from + c, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < 32; k += 4)
+            *reinterpret_cast<float4*>(row + c + k) =
+                make_float4(__uint_as_float(o[k]) * f, __uint_as_float(o[k + 1]) * f, __uint_as_float(o[k + 2]) * f,
+                            __uint_as_float(o[k + 3]) * f);
+        }
+      } else if (DKV) {
         if (half == 0)
           at_store_sum<T>(tmem + AT_TM_DV + lane_off, live ? g1 + off : nullptr, 0, p.head_dim, p.head_dim,
                           at_pow2(-int(at_p_shift<T>())));
@@ -787,23 +827,57 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
   }
   __syncthreads();
   if (warp == 9) tmem_dealloc(tmem, 512);
+  if (DKV && split > 1) {
+    // the cluster's CTAs add up their heads' sums, rank by rank, each a share of the 8-feature pieces
+    cluster_sync_all();
+    if (warp < 8) {
+      const int per = 2 * DC * 8, live = min(AT_TILE, t.len - t.i0);
+      for (int i = rank * 256 + threadIdx.x; i < live * per; i += split * 256) {
+        const int row = i / per, c = (i % per) * 8;  // column of [dK | dV]
+        const int f = c & (DC * 64 - 1);
+        if (f >= p.head_dim) continue;
+        const uint32_t at = sbase + uint32_t(row * AT_JOIN_PITCH<DC> + c) * 4;
+        float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int q = 0; q < split; ++q) {
+          const uint32_t peer = mapa_shared(at, q);
+          const float4 a = ld_cluster_f4(peer), b = ld_cluster_f4(peer + 16);
+          sum[0] += a.x, sum[1] += a.y, sum[2] += a.z, sum[3] += a.w;
+          sum[4] += b.x, sum[5] += b.y, sum[6] += b.z, sum[7] += b.w;
+        }
+        T* to = (c < DC * 64 ? g0 : g1) + (int64_t(t.a + t.i0 + row) * p.kv_heads + h) * p.head_dim + f;
+        *reinterpret_cast<uint4*>(to) = make_uint4(at_pack<T>(sum[0], sum[1]), at_pack<T>(sum[2], sum[3]),
+                                                   at_pack<T>(sum[4], sum[5]), at_pack<T>(sum[6], sum[7]));
+      }
+    }
+    cluster_sync_all();  // no CTA leaves while its sums are read
+  }
 }
 
 template <typename T, int DC>
 __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
     attn_bwd_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_constant__ AttnParams p, const AttnWork w,
-                    T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dv) {
+                    int split, T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dv) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  if (threadIdx.x == 256) {
+    prefetch_tma_desc(&maps.q);
+    prefetch_tma_desc(&maps.k);
+    prefetch_tma_desc(&maps.v);
+    prefetch_tma_desc(&maps.dout);
+  }
   grid_dep_wait();  // programmatic launch: no global access before the wait
-  // the CTAs of key tiles first (a group's heads each: the longer ones), a causal sequence's first
-  // tiles, which the most queries see, before its last; the query tiles the other way round
-  const unsigned n_dkv = unsigned(p.slots) * unsigned(p.kv_heads);
+  // the CTAs of key tiles first, a causal sequence's first tiles, which the most queries see,
+  // before its last; the query tiles the other way round.  `split` CTAs (a cluster) share a key
+  // tile's heads; the grid is a multiple of it.
+  const unsigned n_dkv = unsigned(p.slots) * unsigned(p.kv_heads) * unsigned(split);
   if (blockIdx.x < n_dkv) {
-    attn_bwd_role<T, DC, true>(maps, p, w, blockIdx.x / p.kv_heads, blockIdx.x % p.kv_heads, dk, dv, smem, smem_u32(smem));
+    const unsigned b = blockIdx.x / split;
+    attn_bwd_role<T, DC, true>(maps, p, w, b / p.kv_heads, b % p.kv_heads, split, blockIdx.x % split, dk, dv, smem,
+                               smem_u32(smem));
   } else {
     const unsigned b = blockIdx.x - n_dkv;
-    attn_bwd_role<T, DC, false>(maps, p, w, p.slots - 1 - int(b / p.heads), b % p.heads, dq, nullptr, smem,
+    if (b >= unsigned(p.slots) * unsigned(p.heads)) return;
+    attn_bwd_role<T, DC, false>(maps, p, w, p.slots - 1 - int(b / p.heads), b % p.heads, 1, 0, dq, nullptr, smem,
                                 smem_u32(smem));
   }
 }
@@ -826,7 +900,7 @@ static int attn_checks(const nf4b_attn* in, nf4b_attn* a) {
   NF4B_RETURN_IF(a->head_dim % 8 != 0 || a->head_dim > AT_MAX_DIM, NF4B_ERR_UNSUPPORTED);
   NF4B_RETURN_IF(a->tokens > 0x3FFFFFFF || a->rows > 0x3FFFFFFF || a->heads > 65535, NF4B_ERR_UNSUPPORTED);
   // CTAs of a launch
-  NF4B_RETURN_IF(at_slots(a->tokens, a->rows) * (a->heads + a->kv_heads) > 0x7FFFFFFF, NF4B_ERR_UNSUPPORTED);
+  NF4B_RETURN_IF(at_slots(a->tokens, a->rows) * 2 * a->heads + 8 > 0x7FFFFFFF, NF4B_ERR_UNSUPPORTED);
   if (a->tokens == 0) return NF4B_OK;
   NF4B_RETURN_IF(!a->q || !a->k || !a->v || !a->cu, NF4B_ERR_INVALID_ARG);
   NF4B_RETURN_IF(!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->cu, 4), NF4B_ERR_ALIGNMENT);
@@ -932,6 +1006,35 @@ extern "C" int64_t nf4b_attn_bwd_work_bytes(int64_t tokens, int32_t rows, int32_
   return attn_work(tokens, at_slots(tokens, rows), heads, kv_heads, nullptr, nullptr);
 }
 
+// CTAs that share a key tile's heads: the divisor of the group (at most 8, a cluster) with the
+// shortest estimated time on 148 SMs, from an average sequence: the longer of all CTAs' work
+// shared out and the longest key-tile CTA.  In microseconds, as measured: about 4 of set-up and
+// store for a CTA, 1 more for the join, 1.2 a key-tile step, 0.9 a query-tile step.
+static int attn_split(const nf4b_attn& a) {
+  const int grp = a.heads / a.kv_heads;
+  const double len = double(a.tokens) / (a.rows > 0 ? a.rows : 1);
+  const double seen_max = (a.left < 0 ? len : a.left) + (a.right < 0 ? len : a.right) + 1;
+  const double most = (seen_max < len ? seen_max : len) / AT_TILE + 1;                          // tiles a key tile meets
+  const double mean = (a.left < 0) != (a.right < 0) && most * AT_TILE > len ? (most + 1) / 2 : most;
+  const double tiles = double(a.tokens) / AT_TILE + 0.5 * a.rows;
+  int best = 1;
+  double best_us = 0;
+  for (int c = 1; c <= 8 && c <= grp; ++c) {
+    if (grp % c != 0) continue;
+    const double keys = tiles * a.kv_heads * c * (4.0 + (c > 1 ? 1.0 : 0.0) + 1.2 * mean * (grp / c));
+    const double queries = tiles * a.heads * (4.0 + 0.9 * mean);
+    const double all = (keys + queries) / 148, longest = 5.0 + 1.2 * most * (grp / c);
+    const double us = all > longest ? all : longest;
+    if (c == 1 || us < best_us) {
+      best = c;
+      best_us = us;
+    }
+  }
+  const char* v = std::getenv("STEW_ATTN_SPLIT");
+  if (v != nullptr && v[0] >= '1' && v[0] <= '8' && grp % (v[0] - '0') == 0) best = v[0] - '0';
+  return best;
+}
+
 template <typename T, int DC>
 static int attn_bwd_launch(const nf4b_attn& a, const void* out, const float* lse, const void* dout, void* dq, void* dk,
                            void* dv, void* work, cudaStream_t s) {
@@ -950,8 +1053,22 @@ static int attn_bwd_launch(const nf4b_attn& a, const void* out, const float* lse
   NF4B_CUDA_TRY(launch_pdl(attn_prep_kernel<T>, dim3(unsigned(p.slots) * unsigned(a.heads)), dim3(AT_PREP_THREADS),
                            size_t(0), s, p, static_cast<const T*>(out), static_cast<const T*>(dout), lse,
                            static_cast<const T*>(a.v), a.v_stride, a.v_head_stride, w, tq, tk, tv));
-  NF4B_CUDA_TRY(launch_pdl(attn_bwd_kernel<T, DC>, dim3(unsigned(p.slots) * unsigned(a.heads + a.kv_heads)),
-                           dim3(AT_BWD_THREADS), size_t(AttnBwdSmem<DC>::ALLOC), s, m, p, w, tq, tk, tv));
+  const int split = attn_split(a);
+  const int64_t ctas = int64_t(p.slots) * (int64_t(a.kv_heads) * split + a.heads);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned((ctas + split - 1) / split * split));
+  cfg.blockDim = dim3(AT_BWD_THREADS);
+  cfg.dynamicSmemBytes = AttnBwdSmem<DC>::ALLOC;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(split);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled(s) ? 2 : 1;
+  NF4B_CUDA_TRY(cudaLaunchKernelEx(&cfg, attn_bwd_kernel<T, DC>, m, p, w, split, tq, tk, tv));
   return launch_status("attn_bwd_kernel launch");
 }
 
