@@ -33,8 +33,8 @@ struct AttnFwdSmem {
   static constexpr int Q = 0;
   static constexpr int KV = TILE;
   static constexpr int BAR = KV + RING * TILE;
-  // full[RING], empty[RING], q_full, s_full, p_ready, o_full, staged
-  static constexpr int NBAR = 2 * RING + 5;
+  // full[RING], empty[RING], q_full, s_full, p_ready[2], o_full, staged
+  static constexpr int NBAR = 2 * RING + 6;
   static constexpr int MISC = BAR + NBAR * 8;
   static constexpr int ALLOC = MISC + 16 + 1024;  // slack to align the base to 1024 B
 };
@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
   uint64_t* q_full = empty + L::RING;
   uint64_t* s_full = q_full + 1;
   uint64_t* p_ready = s_full + 1;
-  uint64_t* o_full = p_ready + 1;
+  uint64_t* o_full = p_ready + 2;
   uint64_t* staged = o_full + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC + 4);
@@ -84,7 +84,8 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
     }
     mbar_init(q_full, 1);
     mbar_init(s_full, 1);
-    mbar_init(p_ready, 128);
+    mbar_init(&p_ready[0], 128);
+    mbar_init(&p_ready[1], 128);
     mbar_init(o_full, 1);
     mbar_init(staged, 1);
     fence_barrier_init();
@@ -172,13 +173,18 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
       scores(0);
       for (int i = 0; ok && i < nt; ++i) {
         const int x = 2 * i + 1, s = x % L::RING;
-        ok = at_wait(&full[s], (x / L::RING) & 1, abort_flag, 5) && at_wait(p_ready, i & 1, abort_flag, 6);
-        if (!ok) break;
-        tc_fence_after();
+        ok = at_wait(&full[s], (x / L::RING) & 1, abort_flag, 5);
         const uint64_t dv = dv0 + uint64_t(s * (L::TILE >> 4));
 #pragma unroll
-        for (int k = 0; k < AT_TILE / 16; ++k)
-          umma_f16_ts(t_o, t_s + k * 8, dv + uint64_t(k * (2048 >> 4)), id_o, i > 0 || k > 0);
+        for (int half = 0; half < 2; ++half) {
+          ok = ok && at_wait(&p_ready[half], i & 1, abort_flag, 6);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = half * 4; k < half * 4 + 4; ++k)
+            umma_f16_ts(t_o, t_s + k * 8, dv + uint64_t(k * (2048 >> 4)), id_o, i > 0 || k > 0);
+        }
+        if (!ok) break;
         umma_commit(&empty[s]);
         // the next scores overwrite P: MMAs of one thread run in order
         if (i + 1 < nt) scores(x + 1);
@@ -213,7 +219,8 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
       }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(s[c >> 5][c & 31]));
+      for (int c = 0; c < 128; c += 2)
+        mx[(c >> 1) & 3] = fmaxf(mx[(c >> 1) & 3], fmaxf(__uint_as_float(s[c >> 5][c & 31]), __uint_as_float(s[c >> 5][(c & 31) + 1])));
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       // also where nothing was visible before (m = -inf: the factor is 0, and so are O and l)
       const bool grow = (top - m) * sl2 > AT_LAZY;
@@ -232,24 +239,26 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
       }
       if (it == 0 || grow) m = top;
       const float neg = m == -INFINITY ? 0.f : -m * sl2;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t sl2x2 = f2_pack(sl2, sl2), negx2 = f2_pack(neg, neg);
+      uint64_t sum[2] = {0, 0};
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < 2; ++c) {  // half of the keys at a time: their MMAs start on the first half
         uint32_t pk[32];
 #pragma unroll
         for (int k = 0; k < 32; ++k) {
           const int e = c * 64 + 2 * k;
-          const float a = at_exp2(fmaf(__uint_as_float(s[e >> 5][e & 31]), sl2, neg));
-          const float b = at_exp2(fmaf(__uint_as_float(s[e >> 5][(e & 31) + 1]), sl2, neg));
-          sum[k & 3] += a + b;
+          const float2 x = f2_unpack(f2_fma(f2_pack_u(s[e >> 5][e & 31], s[e >> 5][(e & 31) + 1]), sl2x2, negx2));
+          const float a = at_exp2(x.x), b = at_exp2(x.y);
+          sum[k & 1] = f2_add(sum[k & 1], f2_pack(a, b));
           pk[k] = at_pack<T>(a, b);  // the MMA's operand type; l keeps the 32-bit values
         }
         tmem_st_32x32b_x32(t_s + lane_off + c * 32, pk);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&p_ready[c]);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(p_ready);
+      const float2 l2 = f2_unpack(f2_add(sum[0], sum[1]));
+      l += l2.x + l2.y;
     }
     if (__all_sync(0xffffffffu, ok)) ok = at_wait(o_full, 0, abort_flag, 8);
     if (__all_sync(0xffffffffu, ok)) {
@@ -433,7 +442,7 @@ struct AttnBwdSmem {
   static constexpr int Y = TILE;
   static constexpr int A = 2 * TILE;
   static constexpr int B = 4 * TILE;
-  static constexpr int AUX = 6 * TILE;             // [2][128] lse, [2][128] -delta (scaled)
+  static constexpr int AUX = 6 * TILE;             // [2][128] -lse, [2][128] -delta (scaled)
   static constexpr int BAR = AUX + 4 * AT_TILE * 4;
   // a_full[2], a_empty[2], b_full[2], b_empty[2], aux_full[2], aux_empty[2], xy_full, staged, s_full, p_ready,
   // dp_full, ds_ready, done
@@ -600,7 +609,7 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
           for (int e = 0; e < 4; ++e) {
             const int r = e * 32 + lane;
             const float2 x = y0 + r < t.len ? src[y0 + r] : make_float2(INFINITY, 0.f);  // p = 0 behind the end
-            aux_lse[s * AT_TILE + r] = x.x - at_p_shift<T>();
+            aux_lse[s * AT_TILE + r] = at_p_shift<T>() - x.x;
             aux_dl[s * AT_TILE + r] = -x.y * sc;
           }
         }
@@ -711,12 +720,12 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
     const float sl2 = p.scale * AT_LOG2E;
     const int see_lo = back < 0 ? 0 : x - back;
     const int see_hi = ahead < 0 ? t.len - 1 : min(t.len - 1, x + ahead);
-    float row_lse = 0.f, row_dl = 0.f;
+    uint64_t row_lse = 0, row_dl = 0;  // twice each
     ds_scale();
     if (!DKV) {
       const float2 v = x < t.len ? w.row[int64_t(h) * p.tokens + t.a + x] : make_float2(INFINITY, 0.f);
-      row_lse = -(v.x - at_p_shift<T>());
-      row_dl = -v.y * sc;
+      row_lse = f2_pack(at_p_shift<T>() - v.x, at_p_shift<T>() - v.x);
+      row_dl = f2_pack(-v.y * sc, -v.y * sc);
     }
     bool ok = true;
     for (int it = 0; it < n; ++it) {
@@ -736,26 +745,33 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
         tc_fence_before();
         mbar_arrive(p_ready);  // the scores are in registers: the next tile's may overwrite them
       }
-      float pv[64];
-      const float4* la = reinterpret_cast<const float4*>(aux_lse + s * AT_TILE + half * 64);
+      uint64_t pv[32];
+      const uint64_t sl2x2 = f2_pack(sl2, sl2);
+      const ulonglong2* la = reinterpret_cast<const ulonglong2*>(aux_lse + s * AT_TILE + half * 64);
 #pragma unroll
       for (int c = 0; c < 16; ++c) {
-        float4 l4 = make_float4(0.f, 0.f, 0.f, 0.f);
+        ulonglong2 l4 = make_ulonglong2(row_lse, row_lse);
         if (DKV) l4 = la[c];
-        const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          pv[c * 4 + e] = at_exp2(fmaf(__uint_as_float(sv[c * 4 + e]), sl2, DKV ? -lv[e] : row_lse));
+        const float2 x = f2_unpack(f2_fma(f2_pack_u(sv[4 * c], sv[4 * c + 1]), sl2x2, l4.x));
+        const float2 y = f2_unpack(f2_fma(f2_pack_u(sv[4 * c + 2], sv[4 * c + 3]), sl2x2, l4.y));
+        pv[2 * c] = f2_pack(at_exp2(x.x), at_exp2(x.y));
+        pv[2 * c + 1] = f2_pack(at_exp2(y.x), at_exp2(y.y));
       }
       if (cut) {
 #pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (y0 + c < see_lo || y0 + c > see_hi) pv[c] = 0.f;
+        for (int c = 0; c < 64; c += 2) {
+          const float2 v = f2_unpack(pv[c >> 1]);
+          pv[c >> 1] = f2_pack(y0 + c < see_lo || y0 + c > see_hi ? 0.f : v.x,
+                               y0 + c + 1 < see_lo || y0 + c + 1 > see_hi ? 0.f : v.y);
+        }
       }
       if (DKV) {
         uint32_t pk[32];
 #pragma unroll
-        for (int k = 0; k < 32; ++k) pk[k] = at_pack<T>(pv[2 * k], pv[2 * k + 1]);  // the MMA's operand type
+        for (int k = 0; k < 32; ++k) {
+          const float2 v = f2_unpack(pv[k]);
+          pk[k] = at_pack<T>(v.x, v.y);  // the MMA's operand type
+        }
         tmem_st_32x32b_x32(t_s, pk);
         tmem_st_wait();
         tc_fence_before();
@@ -768,22 +784,28 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
 #pragma unroll
       for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(t_dp + c * 32, *reinterpret_cast<uint32_t(*)[32]>(dv + c * 32));
       tmem_ld_wait();
-      const float4* ld = reinterpret_cast<const float4*>(aux_dl + s * AT_TILE + half * 64);
-      uint32_t pk[32];
+      const uint64_t scx2 = f2_pack(sc, sc);
+      const ulonglong2* ld = reinterpret_cast<const ulonglong2*>(aux_dl + s * AT_TILE + half * 64);
 #pragma unroll
       for (int c = 0; c < 16; ++c) {
-        float4 d4 = make_float4(row_dl, row_dl, row_dl, row_dl);
+        ulonglong2 d4 = make_ulonglong2(row_dl, row_dl);
         if (DKV) d4 = ld[c];
-        const float dl[4] = {d4.x, d4.y, d4.z, d4.w};
-        float ds[4];
+        pv[2 * c] = f2_mul(pv[2 * c], f2_fma(f2_pack_u(dv[4 * c], dv[4 * c + 1]), scx2, d4.x));
+        pv[2 * c + 1] = f2_mul(pv[2 * c + 1], f2_fma(f2_pack_u(dv[4 * c + 2], dv[4 * c + 3]), scx2, d4.y));
+      }
+      if (cut) {  // a hidden pair adds nothing, whatever its dP is
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          ds[e] = pv[c * 4 + e] * fmaf(__uint_as_float(dv[c * 4 + e]), sc, dl[e]);
-          // a hidden pair adds nothing, whatever its dP is
-          if (cut && (y0 + c * 4 + e < see_lo || y0 + c * 4 + e > see_hi)) ds[e] = 0.f;
+        for (int c = 0; c < 64; c += 2) {
+          const float2 v = f2_unpack(pv[c >> 1]);
+          pv[c >> 1] = f2_pack(y0 + c < see_lo || y0 + c > see_hi ? 0.f : v.x,
+                               y0 + c + 1 < see_lo || y0 + c + 1 > see_hi ? 0.f : v.y);
         }
-        pk[2 * c] = at_pack<T>(ds[0], ds[1]);
-        pk[2 * c + 1] = at_pack<T>(ds[2], ds[3]);
+      }
+      uint32_t pk[32];
+#pragma unroll
+      for (int k = 0; k < 32; ++k) {
+        const float2 v = f2_unpack(pv[k]);
+        pk[k] = at_pack<T>(v.x, v.y);
       }
       tmem_st_32x32b_x32(t_dp, pk);
       tmem_st_wait();
