@@ -15,26 +15,30 @@
 namespace nf4b {
 
 // ------------------------------------------------------------------- forward
-// One CTA per (128-token query tile, head); two CTAs on an SM, so one's softmax runs beside the
-// other's MMAs.  The scores S = Q K^T and the output O live in TMEM (128 + 64 DC columns), the
-// probabilities overwrite the scores as 16-bit values and are the A operand of P V straight from
-// TMEM; Q, K and V are TMA tiles in shared memory (V's is read as an MN-major operand, so nothing
-// is transposed).
+// One CTA per (128-token query tile, head), over key tiles of 64 tokens; two CTAs on an SM, so one's
+// softmax runs beside the other's MMAs.  TMEM (256 columns): two buffers of scores S = Q K^T, 64
+// columns each, and the output O.  The scores of tile i + 1 are computed while the softmax of tile i
+// runs; its probabilities overwrite its own scores as 16-bit values and are the A operand of P V
+// straight from TMEM.  Q, K and V are TMA tiles in shared memory (V's is read as an MN-major operand,
+// so nothing is transposed).
 //   warps 0-3  softmax: one thread per query row
-//   warp 4     TMA: Q, then K and V tiles through a ring of AT_RING slots
+//   warp 4     TMA: Q, then K and V tiles through a ring of slots
 //   warp 5     TMEM allocation, MMA issue
 // One pass over the keys with a running maximum m and sum l (Milakov and Gimelshein's online
 // softmax); O is rescaled only when the maximum has grown by more than 2^8, else P may exceed 1
 // (by at most 2^8, far inside fp16's range) and l with it -- the quotient is the same.
+constexpr int AT_KEYS = 64;                  // keys of a tile
+constexpr int AT_KBOX = AT_KEYS * 128;       // bytes of its 64-feature TMA box
 template <int DC>
 struct AttnFwdSmem {
-  static constexpr int TILE = DC * AT_BOX;
-  static constexpr int RING = DC == 1 ? 4 : 2;
+  static constexpr int QTILE = DC * AT_BOX;
+  static constexpr int TILE = DC * AT_KBOX;
+  static constexpr int RING = 4;
   static constexpr int Q = 0;
-  static constexpr int KV = TILE;
+  static constexpr int KV = QTILE;
   static constexpr int BAR = KV + RING * TILE;
-  // full[RING], empty[RING], q_full, s_full, p_ready[2], o_full, staged
-  static constexpr int NBAR = 2 * RING + 6;
+  // full[RING], empty[RING], q_full, s_full[2], p_ready[2], o_done, staged
+  static constexpr int NBAR = 2 * RING + 7;
   static constexpr int MISC = BAR + NBAR * 8;
   static constexpr int ALLOC = MISC + 16 + 1024;  // slack to align the base to 1024 B
 };
@@ -53,14 +57,19 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR);
   uint64_t* empty = full + L::RING;
   uint64_t* q_full = empty + L::RING;
-  uint64_t* s_full = q_full + 1;
-  uint64_t* p_ready = s_full + 1;
-  uint64_t* o_full = p_ready + 2;
-  uint64_t* staged = o_full + 1;
+  uint64_t* s_full = q_full + 1;    // [2]
+  uint64_t* p_ready = s_full + 2;   // [2]
+  uint64_t* o_done = p_ready + 2;   // a phase per P V
+  uint64_t* staged = o_done + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  if (threadIdx.x == 128) {
+    prefetch_tma_desc(&tm_q);
+    prefetch_tma_desc(&tm_k);
+    prefetch_tma_desc(&tm_v);
+  }
   grid_dep_wait();  // programmatic launch: no global access before the wait
   // the last slots first: a causal sequence's last tiles see the most keys
   const int slot = p.slots - 1 - int(blockIdx.x / p.heads);
@@ -83,10 +92,11 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
       mbar_init(&empty[i], 1);
     }
     mbar_init(q_full, 1);
-    mbar_init(s_full, 1);
-    mbar_init(&p_ready[0], 128);
-    mbar_init(&p_ready[1], 128);
-    mbar_init(o_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_ready[i], 128);
+    }
+    mbar_init(o_done, 1);
     mbar_init(staged, 1);
     fence_barrier_init();
     *abort_flag = 0;
@@ -95,50 +105,45 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
     tmem_alloc(tmem_slot, 256);
     tmem_relinquish();
   }
-  if (warp == 4 && lane == 0) {
-    prefetch_tma_desc(&tm_q);
-    prefetch_tma_desc(&tm_k);
-    prefetch_tma_desc(&tm_v);
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t t_s = tmem, t_o = tmem + AT_TILE;
+  const uint32_t t_o = tmem + 2 * AT_KEYS;
 
-  // the tile's keys [j_lo, j_hi] (relative to a), in tiles of 128 from a multiple of 128 on
+  // the tile's keys [j_lo, j_hi] (relative to a), in tiles of 64 from a multiple of 64 on
   const int i_last = min(t.i0 + AT_TILE, t.len) - 1;
   const int j_lo = p.left < 0 ? 0 : max(0, t.i0 - p.left);
   const int j_hi = p.right < 0 ? t.len - 1 : min(t.len - 1, i_last + p.right);
-  const int jt0 = j_lo >> 7, nt = (j_hi >> 7) - jt0 + 1;
+  const int jt0 = j_lo / AT_KEYS, nt = j_hi / AT_KEYS - jt0 + 1;
 
   if (warp == 4) {
     // ---------------------------------------------------------------- TMA
     int issued = 0;
     bool ok = true;
     if (lane == 0) {
-      mbar_arrive_expect_tx(q_full, L::TILE);
+      mbar_arrive_expect_tx(q_full, L::QTILE);
       for (int c = 0; c < DC; ++c) tma_load_3d(sbase + L::Q + c * AT_BOX, &tm_q, q_full, c * 64, h, t.a + t.i0);
     }
     uint32_t st_phase = 0;
     for (int x = 0; ok && x < 2 * nt; ++x, ++issued) {
       const int s = x % L::RING;
       const bool is_v = x & 1;
-      const int j0 = (jt0 + (x >> 1)) * AT_TILE;
+      const int j0 = (jt0 + (x >> 1)) * AT_KEYS;
       ok = at_wait(&empty[s], ((x / L::RING) & 1) ^ 1, abort_flag, 1);
       if (!__all_sync(0xffffffffu, ok)) break;
-      const bool ragged = is_v && j0 + AT_TILE > t.len;
+      const bool ragged = is_v && j0 + AT_KEYS > t.len;
       if (lane == 0) {
         uint64_t* bar = ragged ? staged : &full[s];
         mbar_arrive_expect_tx(bar, L::TILE);
         for (int c = 0; c < DC; ++c)
-          tma_load_3d(sbase + L::KV + s * L::TILE + c * AT_BOX, is_v ? &tm_v : &tm_k, bar, c * 64, hk, t.a + j0);
+          tma_load_3d(sbase + L::KV + s * L::TILE + c * AT_KBOX, is_v ? &tm_v : &tm_k, bar, c * 64, hk, t.a + j0);
       }
       if (ragged) {
         ok = __all_sync(0xffffffffu, at_wait(staged, st_phase, abort_flag, 2));
         if (!ok) at_drain(staged, st_phase);
         st_phase ^= 1;
-        at_zero_rows<DC>(smem + L::KV + s * L::TILE, t.len - j0);
+        at_zero_rows<DC, AT_KEYS>(smem + L::KV + s * L::TILE, t.len - j0);
         if (lane == 0) mbar_arrive(&full[s]);
       }
     }
@@ -151,75 +156,79 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
     // ---------------------------------------------------------------- MMA
     if (lane == 0) {
       const int kd = (p.head_dim + 15) / 16;               // K steps of the scores
-      const uint32_t id_s = at_idesc<T>(AT_TILE, false);
+      const uint32_t id_s = at_idesc<T>(AT_KEYS, false);
       const uint32_t id_o = at_idesc<T>(kd * 16, true);    // N = head_dim rounded up to 16
       const uint64_t dq = smem_desc_sw128(sbase + L::Q, 16, 1024);
       const uint64_t dk0 = smem_desc_sw128(sbase + L::KV, 16, 1024);
-      const uint64_t dv0 = smem_desc_sw128(sbase + L::KV, AT_BOX, 1024);
+      const uint64_t dv0 = smem_desc_sw128(sbase + L::KV, AT_KBOX, 1024);
       bool ok = at_wait(q_full, 0, abort_flag, 3);
-      auto scores = [&](int x) {  // x: ring position of the K tile
-        const int s = x % L::RING;
+      auto scores = [&](int i) {
+        const int x = 2 * i, s = x % L::RING;
         ok = ok && at_wait(&full[s], (x / L::RING) & 1, abort_flag, 4);
         if (!ok) return;
         tc_fence_after();
         const uint64_t dk = dk0 + uint64_t(s * (L::TILE >> 4));
-        for (int k = 0; k < kd; ++k) {
-          const uint64_t off = uint64_t((k >> 2) * (AT_BOX >> 4) + (k & 3) * 2);
-          umma_f16(t_s, dq + off, dk + off, id_s, k > 0);
-        }
+        for (int k = 0; k < kd; ++k)
+          umma_f16(tmem + (i & 1) * AT_KEYS, dq + uint64_t((k >> 2) * (AT_BOX >> 4) + (k & 3) * 2),
+                   dk + uint64_t((k >> 2) * (AT_KBOX >> 4) + (k & 3) * 2), id_s, k > 0);
         umma_commit(&empty[s]);
-        umma_commit(s_full);
+        umma_commit(&s_full[i & 1]);
       };
       scores(0);
+      if (nt > 1) scores(1);
+      int issued = 0;
       for (int i = 0; ok && i < nt; ++i) {
         const int x = 2 * i + 1, s = x % L::RING;
-        ok = at_wait(&full[s], (x / L::RING) & 1, abort_flag, 5);
+        ok = at_wait(&full[s], (x / L::RING) & 1, abort_flag, 5) && at_wait(&p_ready[i & 1], (i >> 1) & 1, abort_flag, 6);
+        if (!ok) break;
+        tc_fence_after();
         const uint64_t dv = dv0 + uint64_t(s * (L::TILE >> 4));
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          ok = ok && at_wait(&p_ready[half], i & 1, abort_flag, 6);
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int k = half * 4; k < half * 4 + 4; ++k)
-            umma_f16_ts(t_o, t_s + k * 8, dv + uint64_t(k * (2048 >> 4)), id_o, i > 0 || k > 0);
-        }
-        if (!ok) break;
+        for (int k = 0; k < AT_KEYS / 16; ++k)
+          umma_f16_ts(t_o, tmem + (i & 1) * AT_KEYS + k * 8, dv + uint64_t(k * (2048 >> 4)), id_o, i > 0 || k > 0);
         umma_commit(&empty[s]);
-        // the next scores overwrite P: MMAs of one thread run in order
-        if (i + 1 < nt) scores(x + 1);
+        umma_commit(o_done);
+        ++issued;
+        // the scores of tile i + 2 overwrite P of tile i: MMAs of one thread run in order
+        if (i + 2 < nt) scores(i + 2);
       }
-      umma_commit(o_full);
-      at_drain(o_full, 0);  // nothing in flight when TMEM and shared memory go
+      // nothing in flight when TMEM and shared memory go
+      if (!ok) {
+        umma_commit(o_done);
+        ++issued;
+      }
+      at_drain(o_done, (issued - 1) & 1);
     }
   } else {
     // ---------------------------------------------------------------- softmax
     const uint32_t lane_off = uint32_t(warp * 32) << 16;
     const int i = t.i0 + threadIdx.x;  // this thread's query row, relative to a
     const float sl2 = p.scale * AT_LOG2E;
+    const uint64_t sl2x2 = f2_pack(sl2, sl2);
     const int see_lo = p.left < 0 ? 0 : i - p.left;
     const int see_hi = p.right < 0 ? t.len - 1 : min(t.len - 1, i + p.right);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int it = 0; it < nt; ++it) {
-      const int j0 = (jt0 + it) * AT_TILE;
-      ok = at_wait(s_full, it & 1, abort_flag, 7);
+      const int j0 = (jt0 + it) * AT_KEYS;
+      const uint32_t t_s = tmem + lane_off + (it & 1) * AT_KEYS;
+      ok = at_wait(&s_full[it & 1], (it >> 1) & 1, abort_flag, 7);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
-      uint32_t s[4][32];
+      uint32_t s[2][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(t_s + lane_off + c * 32, s[c]);
+      for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(t_s + c * 32, s[c]);
       tmem_ld_wait();
       // tiles that the window or the sequence's end cuts (the same for the whole CTA)
-      if (j0 + AT_TILE > t.len || (p.right >= 0 && j0 + AT_TILE - 1 > t.i0 + p.right) ||
+      if (j0 + AT_KEYS > t.len || (p.right >= 0 && j0 + AT_KEYS - 1 > t.i0 + p.right) ||
           (p.left >= 0 && j0 < t.i0 + AT_TILE - 1 - p.left)) {
 #pragma unroll
-        for (int c = 0; c < 128; ++c)
+        for (int c = 0; c < AT_KEYS; ++c)
           if (j0 + c < see_lo || j0 + c > see_hi) s[c >> 5][c & 31] = 0xff800000u;  // -inf
       }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 128; c += 2)
+      for (int c = 0; c < AT_KEYS; c += 2)
         mx[(c >> 1) & 3] = fmaxf(mx[(c >> 1) & 3], fmaxf(__uint_as_float(s[c >> 5][c & 31]), __uint_as_float(s[c >> 5][(c & 31) + 1])));
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       // also where nothing was visible before (m = -inf: the factor is 0, and so are O and l)
@@ -227,6 +236,9 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
       if (it > 0 && __any_sync(0xffffffffu, grow)) {
         const float f = grow ? at_exp2((m - top) * sl2) : 1.f;
         l *= f;
+        ok = at_wait(o_done, (it - 1) & 1, abort_flag, 9);  // the products so far
+        if (!__all_sync(0xffffffffu, ok)) break;
+        tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < p.head_dim; c += 32) {
           uint32_t o[32];
@@ -239,28 +251,25 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
       }
       if (it == 0 || grow) m = top;
       const float neg = m == -INFINITY ? 0.f : -m * sl2;
-      const uint64_t sl2x2 = f2_pack(sl2, sl2), negx2 = f2_pack(neg, neg);
+      const uint64_t negx2 = f2_pack(neg, neg);
       uint64_t sum[2] = {0, 0};
+      uint32_t pk[32];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {  // half of the keys at a time: their MMAs start on the first half
-        uint32_t pk[32];
-#pragma unroll
-        for (int k = 0; k < 32; ++k) {
-          const int e = c * 64 + 2 * k;
-          const float2 x = f2_unpack(f2_fma(f2_pack_u(s[e >> 5][e & 31], s[e >> 5][(e & 31) + 1]), sl2x2, negx2));
-          const float a = at_exp2(x.x), b = at_exp2(x.y);
-          sum[k & 1] = f2_add(sum[k & 1], f2_pack(a, b));
-          pk[k] = at_pack<T>(a, b);  // the MMA's operand type; l keeps the 32-bit values
-        }
-        tmem_st_32x32b_x32(t_s + lane_off + c * 32, pk);
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(&p_ready[c]);
+      for (int k = 0; k < 32; ++k) {
+        const int e = 2 * k;
+        const float2 x = f2_unpack(f2_fma(f2_pack_u(s[e >> 5][e & 31], s[e >> 5][(e & 31) + 1]), sl2x2, negx2));
+        const float a = at_exp2(x.x), b = at_exp2(x.y);
+        sum[k & 1] = f2_add(sum[k & 1], f2_pack(a, b));
+        pk[k] = at_pack<T>(a, b);  // the MMA's operand type; l keeps the 32-bit values
       }
+      tmem_st_32x32b_x32(t_s, pk);
       const float2 l2 = f2_unpack(f2_add(sum[0], sum[1]));
       l += l2.x + l2.y;
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&p_ready[it & 1]);
     }
-    if (__all_sync(0xffffffffu, ok)) ok = at_wait(o_full, 0, abort_flag, 8);
+    if (__all_sync(0xffffffffu, ok)) ok = at_wait(o_done, (nt - 1) & 1, abort_flag, 8);
     if (__all_sync(0xffffffffu, ok)) {
       tc_fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -619,8 +628,8 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
         ok = __all_sync(0xffffffffu, at_wait(staged, st_phase, abort_flag, 14)) && ok;
         if (!ok) at_drain(staged, st_phase);
         st_phase ^= 1;
-        at_zero_rows<DC>(smem + L::A + s * L::TILE, t.len - y0);
-        if (DKV) at_zero_rows<DC>(smem + L::B + s * L::TILE, t.len - y0);
+        at_zero_rows<DC, AT_TILE>(smem + L::A + s * L::TILE, t.len - y0);
+        if (DKV) at_zero_rows<DC, AT_TILE>(smem + L::B + s * L::TILE, t.len - y0);
         if (lane == 0) {
           mbar_arrive(&a_full[s]);
           if (DKV) mbar_arrive(&b_full[s]);
@@ -939,12 +948,13 @@ static int attn_checks(const nf4b_attn* in, nf4b_attn* a) {
 
 using namespace nf4b;
 
-// [tokens][heads][head_dim] as 64-feature boxes of 128 tokens of one head, 128-byte swizzle, zeros
+// [tokens][heads][head_dim] as 64-feature boxes of `rows` tokens of one head, 128-byte swizzle, zeros
 // outside the tensor.
-static int attn_tmap(CUtensorMap* m, const nf4b_attn& a, const void* base, int heads, int64_t stride, int64_t head_stride) {
+static int attn_tmap(CUtensorMap* m, const nf4b_attn& a, const void* base, int heads, int64_t stride, int64_t head_stride,
+                     int rows) {
   const uint64_t dims[3] = {uint64_t(a.head_dim), uint64_t(heads), uint64_t(a.tokens)};
   const uint64_t strides[2] = {uint64_t(head_stride) * 2, uint64_t(stride) * 2};
-  const uint32_t box[3] = {64, 1, AT_TILE};
+  const uint32_t box[3] = {64, 1, uint32_t(rows)};
   return make_tmap_tiled(m, a.dtype == NF4B_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
                          base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
@@ -972,9 +982,9 @@ static int attn_smem(K kernel, int bytes, bool (&done)[64]) {
 template <typename T, int DC>
 static int attn_fwd_launch(const nf4b_attn& a, void* out, float* lse, cudaStream_t s) {
   CUtensorMap q, k, v;
-  int st = attn_tmap(&q, a, a.q, a.heads, a.q_stride, a.q_head_stride);
-  if (st == NF4B_OK) st = attn_tmap(&k, a, a.k, a.kv_heads, a.k_stride, a.k_head_stride);
-  if (st == NF4B_OK) st = attn_tmap(&v, a, a.v, a.kv_heads, a.v_stride, a.v_head_stride);
+  int st = attn_tmap(&q, a, a.q, a.heads, a.q_stride, a.q_head_stride, AT_TILE);
+  if (st == NF4B_OK) st = attn_tmap(&k, a, a.k, a.kv_heads, a.k_stride, a.k_head_stride, AT_KEYS);
+  if (st == NF4B_OK) st = attn_tmap(&v, a, a.v, a.kv_heads, a.v_stride, a.v_head_stride, AT_KEYS);
   static bool done[64] = {false};
   if (st == NF4B_OK) st = attn_smem(attn_fwd_kernel<T, DC>, AttnFwdSmem<DC>::ALLOC, done);
   if (st != NF4B_OK) return st;
@@ -1061,10 +1071,10 @@ template <typename T, int DC>
 static int attn_bwd_launch(const nf4b_attn& a, const void* out, const float* lse, const void* dout, void* dq, void* dk,
                            void* dv, void* work, cudaStream_t s) {
   AttnBwdMaps m;
-  int st = attn_tmap(&m.q, a, a.q, a.heads, a.q_stride, a.q_head_stride);
-  if (st == NF4B_OK) st = attn_tmap(&m.k, a, a.k, a.kv_heads, a.k_stride, a.k_head_stride);
-  if (st == NF4B_OK) st = attn_tmap(&m.v, a, a.v, a.kv_heads, a.v_stride, a.v_head_stride);
-  if (st == NF4B_OK) st = attn_tmap(&m.dout, a, dout, a.heads, int64_t(a.heads) * a.head_dim, a.head_dim);
+  int st = attn_tmap(&m.q, a, a.q, a.heads, a.q_stride, a.q_head_stride, AT_TILE);
+  if (st == NF4B_OK) st = attn_tmap(&m.k, a, a.k, a.kv_heads, a.k_stride, a.k_head_stride, AT_TILE);
+  if (st == NF4B_OK) st = attn_tmap(&m.v, a, a.v, a.kv_heads, a.v_stride, a.v_head_stride, AT_TILE);
+  if (st == NF4B_OK) st = attn_tmap(&m.dout, a, dout, a.heads, int64_t(a.heads) * a.head_dim, a.head_dim, AT_TILE);
   static bool done[64] = {false};
   if (st == NF4B_OK) st = attn_smem(attn_bwd_kernel<T, DC>, AttnBwdSmem<DC>::ALLOC, done);
   if (st != NF4B_OK) return st;

@@ -162,16 +162,16 @@ __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap
       : "memory");
 }
 
-// Whole warp: zeros in rows [first, 128) of a [128 tokens][DC x 64 features] tile, so that the rows of
+// Whole warp: zeros in rows [first, ROWS) of a [ROWS tokens][DC x 64 features] tile, so that the rows of
 // other sequences behind a ragged tile add nothing to a product over tokens (0 x their NaN would).
 // The 128-byte swizzle permutes inside a row only.  The writes are made visible to the MMA.
-template <int DC>
+template <int DC, int ROWS>
 __device__ __forceinline__ void at_zero_rows(uint8_t* tile, int first) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int c = 0; c < DC; ++c)
-    for (int at = first * 128 + lane * 16; at < AT_BOX; at += 512)
-      *reinterpret_cast<uint4*>(tile + c * AT_BOX + at) = make_uint4(0, 0, 0, 0);
+    for (int at = first * 128 + lane * 16; at < ROWS * 128; at += 512)
+      *reinterpret_cast<uint4*>(tile + c * ROWS * 128 + at) = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
   __syncwarp();
 }
