@@ -4,8 +4,8 @@
 //   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i
 // over the pairs (i, j) of one sequence inside the window i - left <= j <= i + right.
 //
-// Every product runs on tcgen05 over 128-token tiles that TMA brings in; a ragged tile's rows of other
-// sequences are zeroed in shared memory where a product sums over them, and masked elsewhere.
+// Every product runs on tcgen05 over tiles of 128 or 64 tokens that TMA brings in; a ragged tile's rows of
+// other sequences are zeroed in shared memory where a product sums over them, and masked elsewhere.
 // Sums and softmax statistics are fp32 (TMEM, registers), in a fixed order.
 #include <cstdlib>
 #include <mutex>
@@ -37,8 +37,8 @@ struct AttnFwdSmem {
   static constexpr int Q = 0;
   static constexpr int KV = QTILE;
   static constexpr int BAR = KV + RING * TILE;
-  // full[RING], empty[RING], q_full, s_full[2], p_ready[2], o_done, staged
-  static constexpr int NBAR = 2 * RING + 7;
+  // full[RING], empty[RING], q_full, s_full[2], p_ready[2], o_done
+  static constexpr int NBAR = 2 * RING + 6;
   static constexpr int MISC = BAR + NBAR * 8;
   static constexpr int ALLOC = MISC + 16 + 1024;  // slack to align the base to 1024 B
 };
@@ -60,7 +60,6 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
   uint64_t* s_full = q_full + 1;    // [2]
   uint64_t* p_ready = s_full + 2;   // [2]
   uint64_t* o_done = p_ready + 2;   // a phase per P V
-  uint64_t* staged = o_done + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -97,7 +96,6 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
       mbar_init(&p_ready[i], 128);
     }
     mbar_init(o_done, 1);
-    mbar_init(staged, 1);
     fence_barrier_init();
     *abort_flag = 0;
   }
@@ -120,31 +118,19 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
   if (warp == 4) {
     // ---------------------------------------------------------------- TMA
     int issued = 0;
-    bool ok = true;
     if (lane == 0) {
       mbar_arrive_expect_tx(q_full, L::QTILE);
       for (int c = 0; c < DC; ++c) tma_load_3d(sbase + L::Q + c * AT_BOX, &tm_q, q_full, c * 64, h, t.a + t.i0);
     }
-    uint32_t st_phase = 0;
-    for (int x = 0; ok && x < 2 * nt; ++x, ++issued) {
+    for (int x = 0; x < 2 * nt; ++x, ++issued) {
       const int s = x % L::RING;
       const bool is_v = x & 1;
-      const int j0 = (jt0 + (x >> 1)) * AT_KEYS;
-      ok = at_wait(&empty[s], ((x / L::RING) & 1) ^ 1, abort_flag, 1);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      const bool ragged = is_v && j0 + AT_KEYS > t.len;
+      if (!__all_sync(0xffffffffu, at_wait(&empty[s], ((x / L::RING) & 1) ^ 1, abort_flag, 1))) break;
       if (lane == 0) {
-        uint64_t* bar = ragged ? staged : &full[s];
-        mbar_arrive_expect_tx(bar, L::TILE);
+        mbar_arrive_expect_tx(&full[s], L::TILE);
         for (int c = 0; c < DC; ++c)
-          tma_load_3d(sbase + L::KV + s * L::TILE + c * AT_KBOX, is_v ? &tm_v : &tm_k, bar, c * 64, hk, t.a + j0);
-      }
-      if (ragged) {
-        ok = __all_sync(0xffffffffu, at_wait(staged, st_phase, abort_flag, 2));
-        if (!ok) at_drain(staged, st_phase);
-        st_phase ^= 1;
-        at_zero_rows<DC, AT_KEYS>(smem + L::KV + s * L::TILE, t.len - j0);
-        if (lane == 0) mbar_arrive(&full[s]);
+          tma_load_3d(sbase + L::KV + s * L::TILE + c * AT_KBOX, is_v ? &tm_v : &tm_k, &full[s], c * 64, hk,
+                      t.a + (jt0 + (x >> 1)) * AT_KEYS);
       }
     }
     // an abandoned CTA's loads must have landed before its shared memory goes
@@ -265,6 +251,12 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
       tmem_st_32x32b_x32(t_s, pk);
       const float2 l2 = f2_unpack(f2_add(sum[0], sum[1]));
       l += l2.x + l2.y;
+      if (j0 + AT_KEYS > t.len) {  // the ragged last tile: V's rows behind the sequence's end
+        const int x = 2 * it + 1;
+        ok = at_wait(&full[x % L::RING], (x / L::RING) & 1, abort_flag, 2);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        at_zero_rows<DC, AT_KEYS, 128>(smem + L::KV + (x % L::RING) * L::TILE, t.len - j0, threadIdx.x);
+      }
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&p_ready[it & 1]);
@@ -274,22 +266,10 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
       tc_fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const int64_t row = t.a + i;
-      T* o_row = out + (row * p.heads + h) * p.head_dim;
-#pragma unroll
-      for (int c = 0; c < DC * 2; ++c) {
-        uint32_t o[32];
-        tmem_ld_32x32b_x32(t_o + lane_off + c * 32, o);
-        tmem_ld_wait();
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          uint4 v;
-          uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[e] = at_pack<T>(__uint_as_float(o[k * 8 + 2 * e]) * inv, __uint_as_float(o[k * 8 + 2 * e + 1]) * inv);
-          if (i < t.len && c * 32 + k * 8 < p.head_dim) *reinterpret_cast<uint4*>(o_row + c * 32 + k * 8) = v;
-        }
-      }
+      // every MMA is done: the Q, K and V tiles' memory is free
+      at_store_rows<T, DC * 64>(t_o + lane_off, smem + warp * 32 * (DC * 128 + 16),
+                       out + (int64_t(t.a + t.i0 + warp * 32) * p.heads + h) * p.head_dim, int64_t(p.heads) * p.head_dim,
+                       t.len - t.i0 - warp * 32, p.head_dim, inv);
       if (i < t.len) lse[int64_t(h) * p.tokens + row] = l == 0.f ? -INFINITY : m * p.scale + logf(l);
     }
     tc_fence_before();
@@ -424,12 +404,12 @@ __device__ __forceinline__ int at_ds_exponent(const AttnParams& p, const AttnWor
   const int lane = threadIdx.x & 31, grp = p.heads / p.kv_heads;
   const int first = slot - (t.i0 >> 7), tiles = (t.len + AT_TILE - 1) >> 7;
   float m_do = 0.f, m_dl = 0.f, m_v = 0.f;
-  for (int g = 0; g < grp; ++g)
-    for (int i = lane; i < tiles; i += 32) {
-      const float2 x = w.tile[int64_t(hk * grp + g) * p.slots + first + i];
-      m_do = fmaxf(m_do, x.x);
-      m_dl = fmaxf(m_dl, x.y);
-    }
+  for (int i = lane; i < grp * tiles; i += 32) {
+    const int g = i / tiles;
+    const float2 x = w.tile[int64_t(hk * grp + g) * p.slots + first + i - g * tiles];
+    m_do = fmaxf(m_do, x.x);
+    m_dl = fmaxf(m_dl, x.y);
+  }
   for (int i = lane; i < tiles; i += 32) m_v = fmaxf(m_v, w.vmax[int64_t(hk) * p.slots + first + i]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -453,9 +433,9 @@ struct AttnBwdSmem {
   static constexpr int B = 4 * TILE;
   static constexpr int AUX = 6 * TILE;             // [2][128] -lse, [2][128] -delta (scaled)
   static constexpr int BAR = AUX + 4 * AT_TILE * 4;
-  // a_full[2], a_empty[2], b_full[2], b_empty[2], aux_full[2], aux_empty[2], xy_full, staged, s_full, p_ready,
-  // dp_full, ds_ready, done
-  static constexpr int NBAR = 19;
+  // a_full[2], a_empty[2], b_full[2], b_empty[2], aux_full[2], aux_empty[2], xy_full, s_full, p_ready, dp_full,
+  // ds_ready, done
+  static constexpr int NBAR = 18;
   static constexpr int MISC = BAR + NBAR * 8;
   static constexpr int ALLOC = MISC + 16 + 1024;  // slack to align the base to 1024 B
 };
@@ -470,25 +450,6 @@ static_assert(AT_TILE * AT_JOIN_PITCH<2> * 4 <= AttnBwdSmem<2>::AUX && AT_TILE *
 
 // TMEM columns (512): S | P, dP | dS, and the two sums.
 constexpr int AT_TM_S = 0, AT_TM_DP = 128, AT_TM_DV = 256, AT_TM_DX = 384;
-
-// One warp's 32 rows of a sum in TMEM: `cols` columns from `c0` on, times f, to `row` (null: not stored).
-template <typename T>
-__device__ __forceinline__ void at_store_sum(uint32_t taddr, T* row, int c0, int cols, int head_dim, float f) {
-  for (int c = c0; c < c0 + cols && c < head_dim; c += 32) {
-    uint32_t o[32];
-    tmem_ld_32x32b_x32(taddr + c, o);
-    tmem_ld_wait();
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      uint4 v;
-      uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        w[e] = at_pack<T>(__uint_as_float(o[k * 8 + 2 * e]) * f, __uint_as_float(o[k * 8 + 2 * e + 1]) * f);
-      if (row != nullptr && c + k * 8 < head_dim) *reinterpret_cast<uint4*>(row + c + k * 8) = v;
-    }
-  }
-}
 
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t cluster_addr) {
   float4 v;
@@ -512,8 +473,7 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
   uint64_t* aux_full = b_empty + 2;
   uint64_t* aux_empty = aux_full + 2;
   uint64_t* xy_full = aux_empty + 2;
-  uint64_t* staged = xy_full + 1;
-  uint64_t* s_full = staged + 1;
+  uint64_t* s_full = xy_full + 1;
   uint64_t* p_ready = s_full + 1;
   uint64_t* dp_full = p_ready + 1;
   uint64_t* ds_ready = dp_full + 1;
@@ -538,7 +498,6 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
       mbar_init(&aux_empty[i], 256);
     }
     mbar_init(xy_full, 1);
-    mbar_init(staged, 1);
     mbar_init(s_full, 1);
     mbar_init(p_ready, 256);
     mbar_init(dp_full, 1);
@@ -584,60 +543,37 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
         tma_load_3d(sbase + L::Y + c * AT_BOX, DKV ? &maps.v : &maps.dout, xy_full, c * 64, h, t.a + t.i0);
       }
     }
-    uint32_t st_phase = 0;
-    for (int it = 0; it < n; ++it, ++issued) {
+    for (int it = 0; ok && it < n; ++it) {
       const int s = it & 1;
       const uint32_t ph = ((it >> 1) & 1) ^ 1;
       const int hy = DKV ? h0 + it / nt : hk;
       const int y0 = (yt0 + (DKV ? it % nt : it)) * AT_TILE;
-      // rows of other sequences must add nothing to a sum over the ring tile's tokens: Q and dO in
-      // DKV CTAs, K in the others (V only meets rows that are masked)
-      const bool ragged = y0 + AT_TILE > t.len;
-      ok = at_wait(&a_empty[s], ph, abort_flag, 11) && at_wait(&b_empty[s], ph, abort_flag, 12);
-      if (!__all_sync(0xffffffffu, ok)) break;
+      ok = __all_sync(0xffffffffu, at_wait(&a_empty[s], ph, abort_flag, 11) && at_wait(&b_empty[s], ph, abort_flag, 12));
+      if (!ok) break;
       if (lane == 0) {
-        uint64_t* bar_a = ragged ? staged : &a_full[s];
-        uint64_t* bar_b = ragged && DKV ? staged : &b_full[s];
-        if (bar_a == bar_b) {
-          mbar_arrive_expect_tx(bar_a, 2 * L::TILE);
-        } else {
-          mbar_arrive_expect_tx(bar_a, L::TILE);
-          mbar_arrive_expect_tx(bar_b, L::TILE);
-        }
+        mbar_arrive_expect_tx(&a_full[s], L::TILE);
         for (int c = 0; c < DC; ++c)
-          tma_load_3d(sbase + L::A + s * L::TILE + c * AT_BOX, DKV ? &maps.q : &maps.k, bar_a, c * 64, hy, t.a + y0);
+          tma_load_3d(sbase + L::A + s * L::TILE + c * AT_BOX, DKV ? &maps.q : &maps.k, &a_full[s], c * 64, hy, t.a + y0);
+        mbar_arrive_expect_tx(&b_full[s], L::TILE);
         for (int c = 0; c < DC; ++c)
-          tma_load_3d(sbase + L::B + s * L::TILE + c * AT_BOX, DKV ? &maps.dout : &maps.v, bar_b, c * 64, hy, t.a + y0);
+          tma_load_3d(sbase + L::B + s * L::TILE + c * AT_BOX, DKV ? &maps.dout : &maps.v, &b_full[s], c * 64, hy, t.a + y0);
       }
+      ++issued;
       if (DKV) {
+        const float2* src = w.row + int64_t(hy) * p.tokens + t.a;
+        float2 x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)  // p = 0 behind the end
+          x[e] = y0 + e * 32 + lane < t.len ? src[y0 + e * 32 + lane] : make_float2(INFINITY, 0.f);
         if (it == 0) ds_scale();  // while the first tiles are on their way
         ok = __all_sync(0xffffffffu, at_wait(&aux_empty[s], ph, abort_flag, 13));
-        if (ok) {
-          const float2* src = w.row + int64_t(hy) * p.tokens + t.a;
+        if (!ok) break;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = e * 32 + lane;
-            const float2 x = y0 + r < t.len ? src[y0 + r] : make_float2(INFINITY, 0.f);  // p = 0 behind the end
-            aux_lse[s * AT_TILE + r] = at_p_shift<T>() - x.x;
-            aux_dl[s * AT_TILE + r] = -x.y * sc;
-          }
+        for (int e = 0; e < 4; ++e) {
+          aux_lse[s * AT_TILE + e * 32 + lane] = at_p_shift<T>() - x[e].x;
+          aux_dl[s * AT_TILE + e * 32 + lane] = -x[e].y * sc;
         }
         mbar_arrive(&aux_full[s]);
-      }
-      if (ragged) {
-        ok = __all_sync(0xffffffffu, at_wait(staged, st_phase, abort_flag, 14)) && ok;
-        if (!ok) at_drain(staged, st_phase);
-        st_phase ^= 1;
-        at_zero_rows<DC, AT_TILE>(smem + L::A + s * L::TILE, t.len - y0);
-        if (DKV) at_zero_rows<DC, AT_TILE>(smem + L::B + s * L::TILE, t.len - y0);
-        if (lane == 0) {
-          mbar_arrive(&a_full[s]);
-          if (DKV) mbar_arrive(&b_full[s]);
-        }
-      }
-      if (!ok) {
-        ++issued;
-        break;
       }
     }
     if (*abort_flag && lane == 0) {
@@ -746,6 +682,18 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
       tc_fence_after();
       const bool cut = y0 + 64 > t.len || (ahead >= 0 && y0 + 63 > t.i0 + ahead) ||
                        (back >= 0 && y0 < t.i0 + AT_TILE - 1 - back);
+      // rows of other sequences behind a ragged ring tile must add nothing to a sum over its tokens: Q's and dO's
+      // in DKV CTAs, K's in the others (V only meets scores that are masked).  The scores that read the tiles
+      // are done by then.
+      const int end = t.len - (y0 - half * 64);
+      if (end < AT_TILE) {
+        if (DKV) {
+          ok = at_wait(dp_full, it & 1, abort_flag, 14);
+          if (!__all_sync(0xffffffffu, ok)) break;
+          at_zero_rows<DC, AT_TILE, 256>(smem + L::B + s * L::TILE, end, threadIdx.x);
+        }
+        at_zero_rows<DC, AT_TILE, 256>(smem + L::A + s * L::TILE, end, threadIdx.x);
+      }
       uint32_t sv[64];
 #pragma unroll
       for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(t_s + c * 32, *reinterpret_cast<uint32_t(*)[32]>(sv + c * 32));
@@ -825,8 +773,6 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
     if (__all_sync(0xffffffffu, ok)) ok = at_wait(done, 0, abort_flag, 25);
     if (__all_sync(0xffffffffu, ok)) {
       tc_fence_after();
-      const int64_t off = (int64_t(t.a + x) * (DKV ? p.kv_heads : p.heads) + h) * p.head_dim;
-      const bool live = x < t.len;
       const float fx = p.scale * at_pow2(-k_exp);
       if (DKV && split > 1) {
         // fp32 to this CTA's shared memory (its tiles are done with): [128 rows][dK | dV]
@@ -844,14 +790,19 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
                 make_float4(__uint_as_float(o[k]) * f, __uint_as_float(o[k + 1]) * f, __uint_as_float(o[k + 2]) * f,
                             __uint_as_float(o[k + 3]) * f);
         }
-      } else if (DKV) {
-        if (half == 0)
-          at_store_sum<T>(tmem + AT_TM_DV + lane_off, live ? g1 + off : nullptr, 0, p.head_dim, p.head_dim,
-                          at_pow2(-int(at_p_shift<T>())));
-        else
-          at_store_sum<T>(tmem + AT_TM_DX + lane_off, live ? g0 + off : nullptr, 0, p.head_dim, p.head_dim, fx);
       } else {
-        at_store_sum<T>(tmem + AT_TM_DX + lane_off, live ? g0 + off : nullptr, half * DC * 32, DC * 32, p.head_dim, fx);
+        // the tiles' memory is free: every MMA is done
+        const int heads = DKV ? p.kv_heads : p.heads, w0 = (warp & 3) * 32;
+        const int64_t first = (int64_t(t.a + t.i0 + w0) * heads + h) * p.head_dim, pitch = int64_t(heads) * p.head_dim;
+        uint8_t* buf = smem + warp * 32 * (DC * 128 + 16);
+        if (DKV) {
+          at_store_rows<T, DC * 64>(tmem + (half == 0 ? AT_TM_DX : AT_TM_DV) + lane_off, buf, (half == 0 ? g0 : g1) + first, pitch,
+                           t.len - t.i0 - w0, p.head_dim, half == 0 ? fx : at_pow2(-int(at_p_shift<T>())));
+        } else {
+          const int c0 = half * DC * 32, cols = min(p.head_dim - c0, DC * 32);
+          if (cols > 0)
+            at_store_rows<T, DC * 32>(tmem + AT_TM_DX + lane_off + c0, buf, g0 + first + c0, pitch, t.len - t.i0 - w0, cols, fx);
+        }
       }
     }
     tc_fence_before();
@@ -868,13 +819,21 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
         const int f = c & (DC * 64 - 1);
         if (f >= p.head_dim) continue;
         const uint32_t at = sbase + uint32_t(row * AT_JOIN_PITCH<DC> + c) * 4;
+        float4 v[8][2];  // all peers' loads in flight
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (q < split) {
+            const uint32_t peer = mapa_shared(at, q);
+            v[q][0] = ld_cluster_f4(peer);
+            v[q][1] = ld_cluster_f4(peer + 16);
+          }
         float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        for (int q = 0; q < split; ++q) {
-          const uint32_t peer = mapa_shared(at, q);
-          const float4 a = ld_cluster_f4(peer), b = ld_cluster_f4(peer + 16);
-          sum[0] += a.x, sum[1] += a.y, sum[2] += a.z, sum[3] += a.w;
-          sum[4] += b.x, sum[5] += b.y, sum[6] += b.z, sum[7] += b.w;
-        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (q < split) {
+            sum[0] += v[q][0].x, sum[1] += v[q][0].y, sum[2] += v[q][0].z, sum[3] += v[q][0].w;
+            sum[4] += v[q][1].x, sum[5] += v[q][1].y, sum[6] += v[q][1].z, sum[7] += v[q][1].w;
+          }
         T* to = (c < DC * 64 ? g0 : g1) + (int64_t(t.a + t.i0 + row) * p.kv_heads + h) * p.head_dim + f;
         *reinterpret_cast<uint4*>(to) = make_uint4(at_pack<T>(sum[0], sum[1]), at_pack<T>(sum[2], sum[3]),
                                                    at_pack<T>(sum[4], sum[5]), at_pack<T>(sum[6], sum[7]));

@@ -162,18 +162,49 @@ __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap
       : "memory");
 }
 
-// Whole warp: zeros in rows [first, ROWS) of a [ROWS tokens][DC x 64 features] tile, so that the rows of
-// other sequences behind a ragged tile add nothing to a product over tokens (0 x their NaN would).
-// The 128-byte swizzle permutes inside a row only.  The writes are made visible to the MMA.
-template <int DC, int ROWS>
-__device__ __forceinline__ void at_zero_rows(uint8_t* tile, int first) {
-  const int lane = threadIdx.x & 31;
+// N threads (this one `id`): zeros in rows [first, ROWS) of a [ROWS tokens][DC x 64 features] tile that
+// has arrived, so that the rows of other sequences behind a ragged tile add nothing to a product over
+// tokens (0 x their NaN would).  The 128-byte swizzle permutes inside a row only.  The writes are made
+// visible to the MMAs of the thread that this one arrives at next.
+template <int DC, int ROWS, int N>
+__device__ __forceinline__ void at_zero_rows(uint8_t* tile, int first, int id) {
 #pragma unroll
   for (int c = 0; c < DC; ++c)
-    for (int at = first * 128 + lane * 16; at < ROWS * 128; at += 512)
+    for (int at = first * 128 + id * 16; at < ROWS * 128; at += N * 16)
       *reinterpret_cast<uint4*>(tile + c * ROWS * 128 + at) = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
+}
+
+// Whole warp: `cols` fp32 columns (a multiple of 8, at most MAX) from TMEM column `taddr` on of the warp's 32 rows, row r
+// times its thread's f, rounded to T and written to out + r * stride for r < rows.  The rows pass through
+// `buf` (32 x (2 MAX + 16) bytes of shared memory, the 16 against bank conflicts), so that a warp writes
+// whole rows instead of 16 bytes of each of 32.
+template <typename T, int MAX>
+__device__ __forceinline__ void at_store_rows(uint32_t taddr, uint8_t* buf, T* out, int64_t stride, int rows, int cols, float f) {
+  const int lane = threadIdx.x & 31;
+  constexpr int PITCH = 2 * MAX + 16;
+#pragma unroll
+  for (int c = 0; c < MAX; c += 32) {
+    uint32_t o[32];
+    tmem_ld_32x32b_x32(taddr + c, o);
+    tmem_ld_wait();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint4 v;
+      uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        w[e] = at_pack<T>(__uint_as_float(o[k * 8 + 2 * e]) * f, __uint_as_float(o[k * 8 + 2 * e + 1]) * f);
+      *reinterpret_cast<uint4*>(buf + lane * PITCH + (c + k * 8) * 2) = v;
+    }
+  }
   __syncwarp();
+  constexpr int VEC = MAX / 8;  // 16-byte pieces of a row; a power of two
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) {
+    const int i = k * 32 + lane, r = i / VEC, c = (i % VEC) * 8;
+    if (r < rows && c < cols) *reinterpret_cast<uint4*>(out + r * stride + c) = *reinterpret_cast<const uint4*>(buf + r * PITCH + c * 2);
+  }
 }
 
 // Bounded waits: after about two seconds the CTA's abort flag is raised, g_attn_error records where,
