@@ -15,38 +15,42 @@
 namespace nf4b {
 
 // ------------------------------------------------------------------- forward
-// One CTA per (128-token query tile, head), over key tiles of 64 tokens; two CTAs on an SM, so one's
-// softmax runs beside the other's MMAs.  TMEM (256 columns): two buffers of scores S = Q K^T, 64
-// columns each, and the output O.  The scores of tile i + 1 are computed while the softmax of tile i
-// runs; its probabilities overwrite its own scores as 16-bit values and are the A operand of P V
-// straight from TMEM.  Q, K and V are TMA tiles in shared memory (V's is read as an MN-major operand,
-// so nothing is transposed).
-//   warps 0-3  softmax: one thread per query row
-//   warp 4     TMA: Q, then K and V tiles through a ring of slots
-//   warp 5     TMEM allocation, MMA issue
+// One CTA per SM works on two 128-token query tiles A and B side by side (two heads of a group, or two
+// neighbouring tiles of a head) over key tiles of 64 tokens, so one tile's softmax runs beside the other's
+// MMAs and every K and V tile that TMA brings in serves both.  TMEM (512 columns): per query tile two
+// buffers of scores S = Q K^T, 64 columns each, and the output O.  The scores of key tile i + 1 are computed
+// while the softmax of tile i runs; its probabilities overwrite its own scores as 16-bit values and are the A
+// operand of P V straight from TMEM.  V's tile is read as an MN-major operand, so nothing is transposed.
+//   warps 0-7  softmax: one thread per query row, warps 0-3 for A, 4-7 for B
+//   warp 8     TMA: Q, then K and V tiles through a ring of slots
+//   warp 9     TMEM allocation, MMA issue
 // One pass over the keys with a running maximum m and sum l (Milakov and Gimelshein's online
 // softmax); O is rescaled only when the maximum has grown by more than 2^8, else P may exceed 1
 // (by at most 2^8, far inside fp16's range) and l with it -- the quotient is the same.
 constexpr int AT_KEYS = 64;                  // keys of a tile
 constexpr int AT_KBOX = AT_KEYS * 128;       // bytes of its 64-feature TMA box
+// What a CTA's two query tiles are: one only (few tiles: an SM each), two heads of a group, or two
+// neighbouring tiles of a head (heads that share no keys).
+enum { AT_SINGLE = 0, AT_HEADS = 1, AT_TILES = 2 };
 template <int DC>
 struct AttnFwdSmem {
   static constexpr int QTILE = DC * AT_BOX;
   static constexpr int TILE = DC * AT_KBOX;
-  static constexpr int RING = 4;
+  static constexpr int RING = 10;
   static constexpr int Q = 0;
-  static constexpr int KV = QTILE;
+  static constexpr int KV = 2 * QTILE;
   static constexpr int BAR = KV + RING * TILE;
-  // full[RING], empty[RING], q_full, s_full[2], p_ready[2], o_done
-  static constexpr int NBAR = 2 * RING + 6;
+  // full[RING], empty[RING], q_full, s_full[2][2], p_ready[2][2], o_done[2], o_full[2]
+  static constexpr int NBAR = 2 * RING + 13;
   static constexpr int MISC = BAR + NBAR * 8;
   static constexpr int ALLOC = MISC + 16 + 1024;  // slack to align the base to 1024 B
 };
-constexpr int AT_FWD_THREADS = 192;
+static_assert(AttnFwdSmem<2>::ALLOC <= 232448, "shared memory budget");
+constexpr int AT_FWD_THREADS = 320;
 constexpr float AT_LAZY = 8.f;  // log2 growth of the maximum that O tolerates unscaled
 
 template <typename T, int DC>
-__global__ void __launch_bounds__(AT_FWD_THREADS, 2)
+__global__ void __launch_bounds__(AT_FWD_THREADS, 1)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttnParams p, T* __restrict__ out,
                     float* __restrict__ lse) {
@@ -57,31 +61,38 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR);
   uint64_t* empty = full + L::RING;
   uint64_t* q_full = empty + L::RING;
-  uint64_t* s_full = q_full + 1;    // [2]
-  uint64_t* p_ready = s_full + 2;   // [2]
-  uint64_t* o_done = p_ready + 2;   // a phase per P V
+  uint64_t* s_full = q_full + 1;    // [query tile][buffer]
+  uint64_t* p_ready = s_full + 4;   // [query tile][buffer]
+  uint64_t* o_done = p_ready + 4;   // [query tile], a phase per P V (at most one behind where it is waited for)
+  uint64_t* o_full = o_done + 2;    // [query tile], after the last
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC + 4);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 128) {
+  if (threadIdx.x == 256) {
     prefetch_tma_desc(&tm_q);
     prefetch_tma_desc(&tm_k);
     prefetch_tma_desc(&tm_v);
   }
   grid_dep_wait();  // programmatic launch: no global access before the wait
   // the last slots first: a causal sequence's last tiles see the most keys
-  const int slot = p.slots - 1 - int(blockIdx.x / p.heads);
-  const int h = blockIdx.x % p.heads, hk = h / (p.heads / p.kv_heads);
+  const int grp = p.heads / p.kv_heads, pairs = (grp + 1) >> 1;
+  const int per_slot = p.pair == AT_HEADS ? p.kv_heads * pairs : p.heads;
+  const int slot = p.slots - 1 - int(blockIdx.x / per_slot), unit = blockIdx.x % per_slot;
+  const int h0 = p.pair == AT_HEADS ? unit / pairs * grp + unit % pairs * 2 : unit;  // tile A's head
+  const int hk = h0 / grp, step_h = p.pair == AT_HEADS, step_i = p.pair == AT_TILES ? AT_TILE : 0;
   const AttnTile t = at_find(p, slot);
   if (t.i0 >= t.len) return;
+  const int both = p.pair == AT_HEADS ? (h0 + 1) / grp == hk : p.pair == AT_TILES && t.i0 + AT_TILE < t.len;
   if (t.tail) {
-    const int n = min(AT_TILE, t.len - t.i0), vec = p.head_dim / 8;
-    for (int i = threadIdx.x; i < n * vec; i += AT_FWD_THREADS) {
-      const int64_t row = t.a + t.i0 + i / vec;
-      *reinterpret_cast<uint4*>(out + (row * p.heads + h) * p.head_dim + (i % vec) * 8) = make_uint4(0, 0, 0, 0);
+    const int n = min(1 << p.shift, t.len - t.i0), vec = p.head_dim / 8;
+    for (int h = h0; h <= h0 + (both & step_h); ++h) {
+      for (int i = threadIdx.x; i < n * vec; i += AT_FWD_THREADS) {
+        const int64_t row = t.a + t.i0 + i / vec;
+        *reinterpret_cast<uint4*>(out + (row * p.heads + h) * p.head_dim + (i % vec) * 8) = make_uint4(0, 0, 0, 0);
+      }
+      for (int i = threadIdx.x; i < n; i += AT_FWD_THREADS) lse[int64_t(h) * p.tokens + t.a + t.i0 + i] = -INFINITY;
     }
-    if (threadIdx.x < n) lse[int64_t(h) * p.tokens + t.a + t.i0 + threadIdx.x] = -INFINITY;
     return;
   }
 
@@ -91,104 +102,120 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
       mbar_init(&empty[i], 1);
     }
     mbar_init(q_full, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_ready[i], 128);
     }
-    mbar_init(o_done, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&o_done[i], 1);
+      mbar_init(&o_full[i], 1);
+    }
     fence_barrier_init();
     *abort_flag = 0;
   }
-  if (warp == 5) {
-    tmem_alloc(tmem_slot, 256);
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  const uint32_t t_o = tmem + 2 * AT_KEYS;
+  // per query tile g: scores at [128 g, 128 g + 128), O at 256 + 128 g
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
-  // the tile's keys [j_lo, j_hi] (relative to a), in tiles of 64 from a multiple of 64 on
-  const int i_last = min(t.i0 + AT_TILE, t.len) - 1;
+  // both tiles' keys [j_lo, j_hi] (relative to a), in tiles of 64 from a multiple of 64 on
+  const int i_last = min(t.i0 + (both ? step_i : 0) + AT_TILE, t.len) - 1;
   const int j_lo = p.left < 0 ? 0 : max(0, t.i0 - p.left);
   const int j_hi = p.right < 0 ? t.len - 1 : min(t.len - 1, i_last + p.right);
   const int jt0 = j_lo / AT_KEYS, nt = j_hi / AT_KEYS - jt0 + 1;
 
-  if (warp == 4) {
+  if (warp == 8) {
     // ---------------------------------------------------------------- TMA
     int issued = 0;
     if (lane == 0) {
-      mbar_arrive_expect_tx(q_full, L::QTILE);
-      for (int c = 0; c < DC; ++c) tma_load_3d(sbase + L::Q + c * AT_BOX, &tm_q, q_full, c * 64, h, t.a + t.i0);
-    }
-    for (int x = 0; x < 2 * nt; ++x, ++issued) {
-      const int s = x % L::RING;
-      const bool is_v = x & 1;
-      if (!__all_sync(0xffffffffu, at_wait(&empty[s], ((x / L::RING) & 1) ^ 1, abort_flag, 1))) break;
-      if (lane == 0) {
+      mbar_arrive_expect_tx(q_full, (1 + both) * L::QTILE);
+      for (int g = 0; g <= both; ++g)
+        for (int c = 0; c < DC; ++c)
+          tma_load_3d(sbase + L::Q + g * L::QTILE + c * AT_BOX, &tm_q, q_full, c * 64, h0 + g * step_h,
+                      t.a + t.i0 + g * step_i);
+      for (int x = 0; x < 2 * nt; ++x, ++issued) {
+        const int s = x % L::RING;
+        if (!at_wait(&empty[s], ((x / L::RING) & 1) ^ 1, abort_flag, 1)) break;
         mbar_arrive_expect_tx(&full[s], L::TILE);
         for (int c = 0; c < DC; ++c)
-          tma_load_3d(sbase + L::KV + s * L::TILE + c * AT_KBOX, is_v ? &tm_v : &tm_k, &full[s], c * 64, hk,
+          tma_load_3d(sbase + L::KV + s * L::TILE + c * AT_KBOX, x & 1 ? &tm_v : &tm_k, &full[s], c * 64, hk,
                       t.a + (jt0 + (x >> 1)) * AT_KEYS);
       }
+      // an abandoned CTA's loads must have landed before its shared memory goes
+      if (*abort_flag) {
+        at_drain(q_full, 0);
+        for (int x = max(0, issued - L::RING); x < issued; ++x) at_drain(&full[x % L::RING], (x / L::RING) & 1);
+      }
     }
-    // an abandoned CTA's loads must have landed before its shared memory goes
-    if (*abort_flag && lane == 0) {
-      at_drain(q_full, 0);
-      for (int x = max(0, issued - L::RING); x < issued; ++x) at_drain(&full[x % L::RING], (x / L::RING) & 1);
-    }
-  } else if (warp == 5) {
+  } else if (warp == 9) {
     // ---------------------------------------------------------------- MMA
-    if (lane == 0) {
-      const int kd = (p.head_dim + 15) / 16;               // K steps of the scores
-      const uint32_t id_s = at_idesc<T>(AT_KEYS, false);
-      const uint32_t id_o = at_idesc<T>(kd * 16, true);    // N = head_dim rounded up to 16
-      const uint64_t dq = smem_desc_sw128(sbase + L::Q, 16, 1024);
-      const uint64_t dk0 = smem_desc_sw128(sbase + L::KV, 16, 1024);
-      const uint64_t dv0 = smem_desc_sw128(sbase + L::KV, AT_KBOX, 1024);
-      bool ok = at_wait(q_full, 0, abort_flag, 3);
-      auto scores = [&](int i) {
-        const int x = 2 * i, s = x % L::RING;
-        ok = ok && at_wait(&full[s], (x / L::RING) & 1, abort_flag, 4);
-        if (!ok) return;
+    const uint32_t lead = elect_one();
+    const int kd = (p.head_dim + 15) / 16;               // K steps of the scores
+    const uint32_t id_s = at_idesc<T>(AT_KEYS, false);
+    const uint32_t id_o = at_idesc<T>(kd * 16, true);    // N = head_dim rounded up to 16
+    const uint64_t dq0 = smem_desc_sw128(sbase + L::Q, 16, 1024);
+    const uint64_t dk0 = smem_desc_sw128(sbase + L::KV, 16, 1024);
+    const uint64_t dv0 = smem_desc_sw128(sbase + L::KV, AT_KBOX, 1024);
+    bool ok = __all_sync(0xffffffffu, at_wait(q_full, 0, abort_flag, 3));
+    auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
+      ok = __all_sync(0xffffffffu, ok && at_wait(bar, parity, abort_flag, where));
+      return ok;
+    };
+    auto arrived = [&](int x) { return wait(&full[x % L::RING], (x / L::RING) & 1, 4); };
+    auto scores = [&](int i, int g) {
+      const uint64_t dk = dk0 + uint64_t((2 * i) % L::RING * (L::TILE >> 4)), dq = dq0 + uint64_t(g * (L::QTILE >> 4));
+#pragma unroll
+      for (int k = 0; k < DC * 4; ++k)
+        if (k < kd)
+          at_mma_ss(lead, tmem + g * AT_TILE + (i & 1) * AT_KEYS, dq + uint64_t((k >> 2) * (AT_BOX >> 4) + (k & 3) * 2),
+                    dk + uint64_t((k >> 2) * (AT_KBOX >> 4) + (k & 3) * 2), id_s, k > 0);
+      at_commit(lead, &s_full[2 * g + (i & 1)]);
+      if (g == both) at_commit(lead, &empty[(2 * i) % L::RING]);
+    };
+    for (int i = 0; i < 2 && i < nt; ++i) {
+      if (!arrived(2 * i)) break;
+      tc_fence_after();
+      for (int g = 0; g <= both; ++g) scores(i, g);
+    }
+    int last = -1;  // query tiles whose last product is issued
+    for (int i = 0; ok && i < nt; ++i) {
+      const int sv = (2 * i + 1) % L::RING;
+      if (!arrived(2 * i + 1) || (i + 2 < nt && !arrived(2 * i + 4))) break;
+      const uint64_t dv = dv0 + uint64_t(sv * (L::TILE >> 4));
+      for (int g = 0; g <= both; ++g) {
+        if (!wait(&p_ready[2 * g + (i & 1)], (i >> 1) & 1, 6)) break;
         tc_fence_after();
-        const uint64_t dk = dk0 + uint64_t(s * (L::TILE >> 4));
-        for (int k = 0; k < kd; ++k)
-          umma_f16(tmem + (i & 1) * AT_KEYS, dq + uint64_t((k >> 2) * (AT_BOX >> 4) + (k & 3) * 2),
-                   dk + uint64_t((k >> 2) * (AT_KBOX >> 4) + (k & 3) * 2), id_s, k > 0);
-        umma_commit(&empty[s]);
-        umma_commit(&s_full[i & 1]);
-      };
-      scores(0);
-      if (nt > 1) scores(1);
-      int issued = 0;
-      for (int i = 0; ok && i < nt; ++i) {
-        const int x = 2 * i + 1, s = x % L::RING;
-        ok = at_wait(&full[s], (x / L::RING) & 1, abort_flag, 5) && at_wait(&p_ready[i & 1], (i >> 1) & 1, abort_flag, 6);
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t dv = dv0 + uint64_t(s * (L::TILE >> 4));
 #pragma unroll
         for (int k = 0; k < AT_KEYS / 16; ++k)
-          umma_f16_ts(t_o, tmem + (i & 1) * AT_KEYS + k * 8, dv + uint64_t(k * (2048 >> 4)), id_o, i > 0 || k > 0);
-        umma_commit(&empty[s]);
-        umma_commit(o_done);
-        ++issued;
+          at_mma_ts(lead, tmem + (2 + g) * AT_TILE, tmem + g * AT_TILE + (i & 1) * AT_KEYS + k * 8,
+                    dv + uint64_t(k * (2048 >> 4)), id_o, i > 0 || k > 0);
+        at_commit(lead, &o_done[g]);
+        if (i + 1 == nt) {
+          at_commit(lead, &o_full[g]);
+          last = g;
+        }
+        if (g == both) at_commit(lead, &empty[sv]);
         // the scores of tile i + 2 overwrite P of tile i: MMAs of one thread run in order
-        if (i + 2 < nt) scores(i + 2);
+        if (i + 2 < nt) scores(i + 2, g);
       }
-      // nothing in flight when TMEM and shared memory go
-      if (!ok) {
-        umma_commit(o_done);
-        ++issued;
-      }
-      at_drain(o_done, (issued - 1) & 1);
     }
-  } else {
+    // nothing in flight when TMEM and shared memory go
+    for (int g = 0; g <= both; ++g) {
+      if (g > last) at_commit(lead, &o_full[g]);
+      at_drain(&o_full[g], 0);
+    }
+  } else if (warp < 4 + 4 * both) {
     // ---------------------------------------------------------------- softmax
-    const uint32_t lane_off = uint32_t(warp * 32) << 16;
-    const int i = t.i0 + threadIdx.x;  // this thread's query row, relative to a
+    const int g = warp >> 2, w0 = (warp & 3) * 32;
+    const uint32_t lane_off = uint32_t(w0) << 16;
+    const uint32_t t_s = tmem + lane_off + g * AT_TILE, t_o = tmem + lane_off + (2 + g) * AT_TILE;
+    const int h = h0 + g * step_h, i0 = t.i0 + g * step_i;
+    const int i = i0 + w0 + lane;  // this thread's query row, relative to a
     const float sl2 = p.scale * AT_LOG2E;
     const uint64_t sl2x2 = f2_pack(sl2, sl2);
     const int see_lo = p.left < 0 ? 0 : i - p.left;
@@ -196,18 +223,17 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int it = 0; it < nt; ++it) {
-      const int j0 = (jt0 + it) * AT_KEYS;
-      const uint32_t t_s = tmem + lane_off + (it & 1) * AT_KEYS;
-      ok = at_wait(&s_full[it & 1], (it >> 1) & 1, abort_flag, 7);
+      const int j0 = (jt0 + it) * AT_KEYS, b = it & 1;
+      ok = at_wait(&s_full[2 * g + b], (it >> 1) & 1, abort_flag, 7);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       uint32_t s[2][32];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(t_s + c * 32, s[c]);
+      for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(t_s + b * AT_KEYS + c * 32, s[c]);
       tmem_ld_wait();
-      // tiles that the window or the sequence's end cuts (the same for the whole CTA)
-      if (j0 + AT_KEYS > t.len || (p.right >= 0 && j0 + AT_KEYS - 1 > t.i0 + p.right) ||
-          (p.left >= 0 && j0 < t.i0 + AT_TILE - 1 - p.left)) {
+      // tiles that the window or the sequence's end cuts (the same for the whole query tile)
+      if (j0 + AT_KEYS > t.len || (p.right >= 0 && j0 + AT_KEYS - 1 > i0 + p.right) ||
+          (p.left >= 0 && j0 < i0 + AT_TILE - 1 - p.left)) {
 #pragma unroll
         for (int c = 0; c < AT_KEYS; ++c)
           if (j0 + c < see_lo || j0 + c > see_hi) s[c >> 5][c & 31] = 0xff800000u;  // -inf
@@ -222,17 +248,17 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
       if (it > 0 && __any_sync(0xffffffffu, grow)) {
         const float f = grow ? at_exp2((m - top) * sl2) : 1.f;
         l *= f;
-        ok = at_wait(o_done, (it - 1) & 1, abort_flag, 9);  // the products so far
+        ok = at_wait(&o_done[g], (it - 1) & 1, abort_flag, 9);  // the products so far
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < p.head_dim; c += 32) {
           uint32_t o[32];
-          tmem_ld_32x32b_x32(t_o + lane_off + c, o);
+          tmem_ld_32x32b_x32(t_o + c, o);
           tmem_ld_wait();
 #pragma unroll
           for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-          tmem_st_32x32b_x32(t_o + lane_off + c, o);
+          tmem_st_32x32b_x32(t_o + c, o);
         }
       }
       if (it == 0 || grow) m = top;
@@ -244,38 +270,37 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
       for (int k = 0; k < 32; ++k) {
         const int e = 2 * k;
         const float2 x = f2_unpack(f2_fma(f2_pack_u(s[e >> 5][e & 31], s[e >> 5][(e & 31) + 1]), sl2x2, negx2));
-        const float a = at_exp2(x.x), b = at_exp2(x.y);
-        sum[k & 1] = f2_add(sum[k & 1], f2_pack(a, b));
-        pk[k] = at_pack<T>(a, b);  // the MMA's operand type; l keeps the 32-bit values
+        const float u = at_exp2(x.x), v = at_exp2(x.y);
+        sum[k & 1] = f2_add(sum[k & 1], f2_pack(u, v));
+        pk[k] = at_pack<T>(u, v);  // the MMA's operand type; l keeps the 32-bit values
       }
-      tmem_st_32x32b_x32(t_s, pk);
+      tmem_st_32x32b_x32(t_s + b * AT_KEYS, pk);
       const float2 l2 = f2_unpack(f2_add(sum[0], sum[1]));
       l += l2.x + l2.y;
-      if (j0 + AT_KEYS > t.len) {  // the ragged last tile: V's rows behind the sequence's end
+      if (j0 + AT_KEYS > t.len) {  // the ragged last tile: V's rows behind the sequence's end (zeros from either)
         const int x = 2 * it + 1;
         ok = at_wait(&full[x % L::RING], (x / L::RING) & 1, abort_flag, 2);
         if (!__all_sync(0xffffffffu, ok)) break;
-        at_zero_rows<DC, AT_KEYS, 128>(smem + L::KV + (x % L::RING) * L::TILE, t.len - j0, threadIdx.x);
+        at_zero_rows<DC, AT_KEYS, 128>(smem + L::KV + (x % L::RING) * L::TILE, t.len - j0, threadIdx.x & 127);
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&p_ready[it & 1]);
+      mbar_arrive(&p_ready[2 * g + b]);
     }
-    if (__all_sync(0xffffffffu, ok)) ok = at_wait(o_done, (nt - 1) & 1, abort_flag, 8);
+    if (__all_sync(0xffffffffu, ok)) ok = at_wait(&o_full[g], 0, abort_flag, 8);
     if (__all_sync(0xffffffffu, ok)) {
       tc_fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      const int64_t row = t.a + i;
-      // every MMA is done: the Q, K and V tiles' memory is free
-      at_store_rows<T, DC * 64>(t_o + lane_off, smem + warp * 32 * (DC * 128 + 16),
-                       out + (int64_t(t.a + t.i0 + warp * 32) * p.heads + h) * p.head_dim, int64_t(p.heads) * p.head_dim,
-                       t.len - t.i0 - warp * 32, p.head_dim, inv);
-      if (i < t.len) lse[int64_t(h) * p.tokens + row] = l == 0.f ? -INFINITY : m * p.scale + logf(l);
+      const int64_t row = t.a + i0 + w0;
+      // this tile's MMAs are done: its Q tile's memory is free
+      at_store_rows<T, DC * 64>(t_o, smem + L::Q + g * L::QTILE + w0 * DC * 128, out + (row * p.heads + h) * p.head_dim,
+                                int64_t(p.heads) * p.head_dim, t.len - i0 - w0, p.head_dim, inv);
+      if (i < t.len) lse[int64_t(h) * p.tokens + row + lane] = l == 0.f ? -INFINITY : m * p.scale + logf(l);
     }
     tc_fence_before();
   }
   __syncthreads();
-  if (warp == 5) tmem_dealloc(tmem, 256);
+  if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
 // ------------------------------------------------------------------ backward
@@ -482,7 +507,7 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
   float* aux_dl = aux_lse + 2 * AT_TILE;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC + 4);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int grp = p.heads / p.kv_heads, hk = DKV ? h : h / grp;
 
   const AttnTile t = at_find(p, slot);
@@ -513,7 +538,7 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   // the ring's tiles (relative to a) and iterations
   const int x_last = min(t.i0 + AT_TILE, t.len) - 1;
@@ -585,76 +610,70 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
     }
   } else if (warp == 9) {
     // ---------------------------------------------------------------- MMA
-    if (lane == 0) {
-      const int kd = (p.head_dim + 15) / 16;
-      const uint32_t id_s = at_idesc<T>(AT_TILE, false);
-      const uint32_t id_g = at_idesc<T>(kd * 16, true);
-      const uint64_t dx = smem_desc_sw128(sbase + L::X, 16, 1024), dy = smem_desc_sw128(sbase + L::Y, 16, 1024);
-      const uint64_t da = smem_desc_sw128(sbase + L::A, 16, 1024), db = smem_desc_sw128(sbase + L::B, 16, 1024);
-      const uint64_t ta = smem_desc_sw128(sbase + L::A, AT_BOX, 1024), tb = smem_desc_sw128(sbase + L::B, AT_BOX, 1024);
-      // d (128 x 128) = x a^T over head_dim
-      auto scores = [&](uint32_t d, uint64_t x, uint64_t a) {
-        for (int k = 0; k < kd; ++k) {
-          const uint64_t off = uint64_t((k >> 2) * (AT_BOX >> 4) + (k & 3) * 2);
-          umma_f16(d, x + off, a + off, id_s, k > 0);
-        }
-      };
-      // d (128 x head_dim) += p b over the ring tile's 128 tokens; each half of the columns of p lies
-      // at the start of its own half of the scores it overwrote
-      auto sum = [&](uint32_t d, uint32_t pm, uint64_t b, bool acc) {
+    const uint32_t lead = elect_one();
+    const int kd = (p.head_dim + 15) / 16;
+    const uint32_t id_s = at_idesc<T>(AT_TILE, false);
+    const uint32_t id_g = at_idesc<T>(kd * 16, true);
+    const uint64_t dx = smem_desc_sw128(sbase + L::X, 16, 1024), dy = smem_desc_sw128(sbase + L::Y, 16, 1024);
+    const uint64_t da = smem_desc_sw128(sbase + L::A, 16, 1024), db = smem_desc_sw128(sbase + L::B, 16, 1024);
+    const uint64_t ta = smem_desc_sw128(sbase + L::A, AT_BOX, 1024), tb = smem_desc_sw128(sbase + L::B, AT_BOX, 1024);
+    // d (128 x 128) = x a^T over head_dim
+    auto scores = [&](uint32_t d, uint64_t x, uint64_t a) {
 #pragma unroll
-        for (int k = 0; k < AT_TILE / 16; ++k)
-          umma_f16_ts(d, pm + (k >> 2) * 64 + (k & 3) * 8, b + uint64_t(k * (2048 >> 4)), id_g, acc || k > 0);
-      };
-      constexpr uint64_t STEP = uint64_t(L::TILE >> 4);
-      bool ok = at_wait(xy_full, 0, abort_flag, 15) && at_wait(&a_full[0], 0, abort_flag, 16);
-      if (ok) {
-        tc_fence_after();
-        scores(tmem + AT_TM_S, dx, da);
-        umma_commit(s_full);
-        ok = at_wait(&b_full[0], 0, abort_flag, 17);
+      for (int k = 0; k < DC * 4; ++k) {
+        const uint64_t off = uint64_t((k >> 2) * (AT_BOX >> 4) + (k & 3) * 2);
+        if (k < kd) at_mma_ss(lead, d, x + off, a + off, id_s, k > 0);
       }
-      if (ok) {
-        tc_fence_after();
+    };
+    // d (128 x head_dim) += p b over the ring tile's 128 tokens; each half of the columns of p lies
+    // at the start of its own half of the scores it overwrote
+    auto sum = [&](uint32_t d, uint32_t pm, uint64_t b, bool acc) {
+#pragma unroll
+      for (int k = 0; k < AT_TILE / 16; ++k)
+        at_mma_ts(lead, d, pm + (k >> 2) * 64 + (k & 3) * 8, b + uint64_t(k * (2048 >> 4)), id_g, acc || k > 0);
+    };
+    constexpr uint64_t STEP = uint64_t(L::TILE >> 4);
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
+      ok = __all_sync(0xffffffffu, ok && at_wait(bar, parity, abort_flag, where));
+      if (ok) tc_fence_after();
+      return ok;
+    };
+    if (wait(xy_full, 0, 15) && wait(&a_full[0], 0, 16)) {
+      scores(tmem + AT_TM_S, dx, da);
+      at_commit(lead, s_full);
+      if (wait(&b_full[0], 0, 17)) {
         scores(tmem + AT_TM_DP, dy, db);
-        umma_commit(dp_full);
-        if (!DKV) umma_commit(&b_empty[0]);
+        at_commit(lead, dp_full);
+        if (!DKV) at_commit(lead, &b_empty[0]);
       }
-      for (int it = 0; ok && it < n; ++it) {
-        const int s = it & 1, s1 = s ^ 1;
-        const uint32_t ph = it & 1, ph1 = ((it + 1) >> 1) & 1;
-        const bool more = it + 1 < n;
-        ok = at_wait(p_ready, ph, abort_flag, 18);
-        if (!ok) break;
-        tc_fence_after();
-        if (DKV) {
-          sum(tmem + AT_TM_DV, tmem + AT_TM_S, tb + s * STEP, it > 0);
-          umma_commit(&b_empty[s]);
-        }
-        if (more) {
-          ok = at_wait(&a_full[s1], ph1, abort_flag, 19);
-          if (!ok) break;
-          tc_fence_after();
-          scores(tmem + AT_TM_S, dx, da + s1 * STEP);  // after the product that reads P: MMAs run in order
-          umma_commit(s_full);
-        }
-        ok = at_wait(ds_ready, ph, abort_flag, 20);
-        if (!ok) break;
-        tc_fence_after();
-        sum(tmem + AT_TM_DX, tmem + AT_TM_DP, ta + s * STEP, it > 0);
-        umma_commit(&a_empty[s]);
-        if (more) {
-          ok = at_wait(&b_full[s1], ph1, abort_flag, 21);
-          if (!ok) break;
-          tc_fence_after();
-          scores(tmem + AT_TM_DP, dy, db + s1 * STEP);
-          umma_commit(dp_full);
-          if (!DKV) umma_commit(&b_empty[s1]);
-        }
-      }
-      umma_commit(done);
-      at_drain(done, 0);  // nothing in flight when TMEM and shared memory go
     }
+    for (int it = 0; ok && it < n; ++it) {
+      const int s = it & 1, s1 = s ^ 1;
+      const uint32_t ph = it & 1, ph1 = ((it + 1) >> 1) & 1;
+      const bool more = it + 1 < n;
+      if (!wait(p_ready, ph, 18)) break;
+      if (DKV) {
+        sum(tmem + AT_TM_DV, tmem + AT_TM_S, tb + s * STEP, it > 0);
+        at_commit(lead, &b_empty[s]);
+      }
+      if (more) {
+        if (!wait(&a_full[s1], ph1, 19)) break;
+        scores(tmem + AT_TM_S, dx, da + s1 * STEP);  // after the product that reads P: MMAs run in order
+        at_commit(lead, s_full);
+      }
+      if (!wait(ds_ready, ph, 20)) break;
+      sum(tmem + AT_TM_DX, tmem + AT_TM_DP, ta + s * STEP, it > 0);
+      at_commit(lead, &a_empty[s]);
+      if (more) {
+        if (!wait(&b_full[s1], ph1, 21)) break;
+        scores(tmem + AT_TM_DP, dy, db + s1 * STEP);
+        at_commit(lead, dp_full);
+        if (!DKV) at_commit(lead, &b_empty[s1]);
+      }
+    }
+    at_commit(lead, done);
+    at_drain(done, 0);  // nothing in flight when TMEM and shared memory go
   } else {
     // ---------------------------------------------------------------- elementwise
     const int half = warp >> 2;  // columns [64 half, 64 half + 64)
@@ -794,7 +813,7 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
         // the tiles' memory is free: every MMA is done
         const int heads = DKV ? p.kv_heads : p.heads, w0 = (warp & 3) * 32;
         const int64_t first = (int64_t(t.a + t.i0 + w0) * heads + h) * p.head_dim, pitch = int64_t(heads) * p.head_dim;
-        uint8_t* buf = smem + warp * 32 * (DC * 128 + 16);
+        uint8_t* buf = smem + warp * 32 * DC * 128;
         if (DKV) {
           at_store_rows<T, DC * 64>(tmem + (half == 0 ? AT_TM_DX : AT_TM_DV) + lane_off, buf, (half == 0 ? g0 : g1) + first, pitch,
                            t.len - t.i0 - w0, p.head_dim, half == 0 ? fx : at_pow2(-int(at_p_shift<T>())));
@@ -890,7 +909,7 @@ static int attn_checks(const nf4b_attn* in, nf4b_attn* a) {
   NF4B_RETURN_IF(a->head_dim % 8 != 0 || a->head_dim > AT_MAX_DIM, NF4B_ERR_UNSUPPORTED);
   NF4B_RETURN_IF(a->tokens > 0x3FFFFFFF || a->rows > 0x3FFFFFFF || a->heads > 65535, NF4B_ERR_UNSUPPORTED);
   // CTAs of a launch
-  NF4B_RETURN_IF(at_slots(a->tokens, a->rows) * 2 * a->heads + 8 > 0x7FFFFFFF, NF4B_ERR_UNSUPPORTED);
+  NF4B_RETURN_IF(at_slots(a->tokens, a->rows, 7) * 2 * a->heads + 8 > 0x7FFFFFFF, NF4B_ERR_UNSUPPORTED);
   if (a->tokens == 0) return NF4B_OK;
   NF4B_RETURN_IF(!a->q || !a->k || !a->v || !a->cu, NF4B_ERR_INVALID_ARG);
   NF4B_RETURN_IF(!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->cu, 4), NF4B_ERR_ALIGNMENT);
@@ -918,9 +937,9 @@ static int attn_tmap(CUtensorMap* m, const nf4b_attn& a, const void* base, int h
                          base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-static AttnParams attn_params(const nf4b_attn& a) {
-  return AttnParams{a.cu,       int32_t(a.tokens), a.rows,  a.heads, a.kv_heads,
-                    a.head_dim, a.left,            a.right, int32_t(at_slots(a.tokens, a.rows)), a.scale};
+static AttnParams attn_params(const nf4b_attn& a, int shift, int pair) {
+  return AttnParams{a.cu,    int32_t(a.tokens), a.rows, a.heads, a.kv_heads, a.head_dim, a.left,
+                    a.right, int32_t(at_slots(a.tokens, a.rows, shift)), shift, pair, a.scale};
 }
 
 // Dynamic shared memory of a kernel, set once per device.
@@ -947,8 +966,13 @@ static int attn_fwd_launch(const nf4b_attn& a, void* out, float* lse, cudaStream
   static bool done[64] = {false};
   if (st == NF4B_OK) st = attn_smem(attn_fwd_kernel<T, DC>, AttnFwdSmem<DC>::ALLOC, done);
   if (st != NF4B_OK) return st;
-  const AttnParams p = attn_params(a);
-  NF4B_CUDA_TRY(launch_pdl(attn_fwd_kernel<T, DC>, dim3(unsigned(p.slots) * unsigned(a.heads)), dim3(AT_FWD_THREADS),
+  // pairs of query tiles once there are more tiles than SMs; with fewer an SM each is quicker
+  const int grp = a.heads / a.kv_heads;
+  const bool many = (double(a.tokens) / AT_TILE + 0.5 * a.rows) * a.heads > 148;
+  const int pair = !many ? AT_SINGLE : grp > 1 ? AT_HEADS : AT_TILES;
+  const AttnParams p = attn_params(a, pair == AT_TILES ? 8 : 7, pair);
+  const unsigned per_slot = unsigned(pair == AT_HEADS ? a.kv_heads * ((grp + 1) / 2) : a.heads);
+  NF4B_CUDA_TRY(launch_pdl(attn_fwd_kernel<T, DC>, dim3(unsigned(p.slots) * per_slot), dim3(AT_FWD_THREADS),
                            size_t(AttnFwdSmem<DC>::ALLOC), s, q, k, v, p, static_cast<T*>(out), lse));
   return launch_status("attn_fwd_kernel launch");
 }
@@ -994,7 +1018,7 @@ extern "C" int64_t nf4b_attn_bwd_work_bytes(int64_t tokens, int32_t rows, int32_
   if (tokens < 0 || rows < 0 || heads <= 0 || kv_heads <= 0 || tokens > 0x3FFFFFFF || rows > 0x3FFFFFFF ||
       heads > 65535 || heads % kv_heads != 0)
     return -1;
-  return attn_work(tokens, at_slots(tokens, rows), heads, kv_heads, nullptr, nullptr);
+  return attn_work(tokens, at_slots(tokens, rows, 7), heads, kv_heads, nullptr, nullptr);
 }
 
 // CTAs that share a key tile's heads: the divisor of the group (at most 8, a cluster) with the
@@ -1037,7 +1061,7 @@ static int attn_bwd_launch(const nf4b_attn& a, const void* out, const float* lse
   static bool done[64] = {false};
   if (st == NF4B_OK) st = attn_smem(attn_bwd_kernel<T, DC>, AttnBwdSmem<DC>::ALLOC, done);
   if (st != NF4B_OK) return st;
-  const AttnParams p = attn_params(a);
+  const AttnParams p = attn_params(a, 7, AT_SINGLE);
   AttnWork w;
   attn_work(a.tokens, p.slots, a.heads, a.kv_heads, work, &w);
   T *tq = static_cast<T*>(dq), *tk = static_cast<T*>(dk), *tv = static_cast<T*>(dv);

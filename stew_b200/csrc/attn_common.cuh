@@ -21,15 +21,16 @@ struct AttnParams {
   int32_t tokens, rows, heads, kv_heads, head_dim;
   int32_t left, right;
   int32_t slots;       // tile slots of the packed rows, at_slots()
+  int32_t shift;       // log2 of a slot's tokens
+  int32_t pair;        // forward: what a CTA's two query tiles are, AT_SINGLE ...
   float scale;
 };
 
-// Tiles never cross a sequence.  Sequence s owns the tile slots from floor(start_s / 128) + s on:
-// that many slots hold its tiles for any lengths (floor(b/128) - floor(a/128) + 1 >= ceil((b-a)/128)),
-// so the launch needs only the token and row counts, and a CTA finds its sequence by searching a
-// strictly ascending function of s.  Slots from that of s = rows on cover the rows behind the last
-// sequence.
-inline int64_t at_slots(int64_t tokens, int64_t rows) { return tokens / AT_TILE + rows + 1; }
+// Tiles never cross a sequence.  Sequence s owns the slots of N = 2^shift tokens from floor(start_s / N) + s
+// on: that many hold its tiles for any lengths (floor(b/N) - floor(a/N) + 1 >= ceil((b-a)/N)), so the
+// launch needs only the token and row counts, and a CTA finds its sequence by searching a strictly
+// ascending function of s.  Slots from that of s = rows on cover the rows behind the last sequence.
+inline int64_t at_slots(int64_t tokens, int64_t rows, int shift) { return (tokens >> shift) + rows + 1; }
 
 struct AttnTile {
   int a, len;   // the sequence's first token and length
@@ -41,7 +42,7 @@ struct AttnTile {
 __device__ __forceinline__ int at_start(const AttnParams& p, int s) {
   return s == 0 ? 0 : min(max(__ldg(p.cu + s), 0), p.tokens);
 }
-__device__ __forceinline__ int at_first_slot(const AttnParams& p, int s) { return (at_start(p, s) >> 7) + s; }
+__device__ __forceinline__ int at_first_slot(const AttnParams& p, int s) { return (at_start(p, s) >> p.shift) + s; }
 
 // Whole warp; 32 probes a step (one step for up to 31 sequences).
 __device__ __forceinline__ AttnTile at_find(const AttnParams& p, int slot) {
@@ -58,7 +59,7 @@ __device__ __forceinline__ AttnTile at_find(const AttnParams& p, int slot) {
   t.tail = lo == p.rows;
   t.a = at_start(p, lo);
   t.len = (t.tail ? p.tokens : max(at_start(p, lo + 1), t.a)) - t.a;
-  t.i0 = (slot - ((t.a >> 7) + lo)) << 7;
+  t.i0 = (slot - ((t.a >> p.shift) + lo)) << p.shift;
   return t;
 }
 
@@ -128,15 +129,47 @@ constexpr uint32_t at_idesc<__nv_bfloat16>(int n, bool b_mn_major) {
   return idesc_f16(AT_TILE, n, false, b_mn_major) | (1u << 7) | (1u << 10);
 }
 
+// The MMA warp runs its loop as a whole, so that descriptors stay in uniform registers, and one lane's
+// predicate issues: inside a one-lane branch each MMA took 80-100 clocks to issue, longer than to run.
+// D[tmem] (+)= A[smem] . B[smem]^T.
+__device__ __forceinline__ void at_mma_ss(uint32_t lead, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lead)
+      : "memory");
+}
 // D[tmem] (+)= A[tmem] . B[smem]^T: A holds two 16-bit values of a row per 32-bit column.
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                            uint32_t accumulate) {
+__device__ __forceinline__ void at_mma_ts(uint32_t lead, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void at_commit(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(lead)
+      : "memory");
+}
+// One lane of a whole warp.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t lead;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(lead));
+  return lead;
 }
 
 // 32 lanes x 32 columns of 32-bit values into TMEM (the layout of tmem_ld_32x32b_x32).
@@ -175,14 +208,15 @@ __device__ __forceinline__ void at_zero_rows(uint8_t* tile, int first, int id) {
   fence_proxy_async_smem();
 }
 
-// Whole warp: `cols` fp32 columns (a multiple of 8, at most MAX) from TMEM column `taddr` on of the warp's 32 rows, row r
-// times its thread's f, rounded to T and written to out + r * stride for r < rows.  The rows pass through
-// `buf` (32 x (2 MAX + 16) bytes of shared memory, the 16 against bank conflicts), so that a warp writes
-// whole rows instead of 16 bytes of each of 32.
+// Whole warp: `cols` fp32 columns (a multiple of 8, at most MAX) from TMEM column `taddr` on of the warp's 32
+// rows, row r times its thread's f, rounded to T and written to out + r * stride for r < rows.  The rows pass
+// through `buf` (32 x 2 MAX bytes of shared memory, the 16-byte pieces of a row permuted by its number against
+// bank conflicts), so that a warp writes whole rows instead of 16 bytes of each of 32.
 template <typename T, int MAX>
 __device__ __forceinline__ void at_store_rows(uint32_t taddr, uint8_t* buf, T* out, int64_t stride, int rows, int cols, float f) {
   const int lane = threadIdx.x & 31;
-  constexpr int PITCH = 2 * MAX + 16;
+  constexpr int VEC = MAX / 8;  // 16-byte pieces of a row: 4, 8 or 16
+  auto place = [&](int r, int c) { return buf + r * (2 * MAX) + (c ^ (VEC >= 8 ? r & 7 : (r >> 1) & 3)) * 16; };
 #pragma unroll
   for (int c = 0; c < MAX; c += 32) {
     uint32_t o[32];
@@ -195,15 +229,14 @@ __device__ __forceinline__ void at_store_rows(uint32_t taddr, uint8_t* buf, T* o
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         w[e] = at_pack<T>(__uint_as_float(o[k * 8 + 2 * e]) * f, __uint_as_float(o[k * 8 + 2 * e + 1]) * f);
-      *reinterpret_cast<uint4*>(buf + lane * PITCH + (c + k * 8) * 2) = v;
+      *reinterpret_cast<uint4*>(place(lane, c / 8 + k)) = v;
     }
   }
   __syncwarp();
-  constexpr int VEC = MAX / 8;  // 16-byte pieces of a row; a power of two
 #pragma unroll
   for (int k = 0; k < VEC; ++k) {
-    const int i = k * 32 + lane, r = i / VEC, c = (i % VEC) * 8;
-    if (r < rows && c < cols) *reinterpret_cast<uint4*>(out + r * stride + c) = *reinterpret_cast<const uint4*>(buf + r * PITCH + c * 2);
+    const int i = k * 32 + lane, r = i / VEC, c = i % VEC;
+    if (r < rows && c * 8 < cols) *reinterpret_cast<uint4*>(out + r * stride + c * 8) = *reinterpret_cast<const uint4*>(place(r, c));
   }
 }
 
