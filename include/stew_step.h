@@ -101,9 +101,9 @@ int nf4b_attn_fwd(const nf4b_attn* a, void* out, float* lse, void* stream);
  * k's and v's summed over the query heads that share them.  The probabilities are recomputed
  * from lse; every sum is taken in a fixed order (the same bits on every run).  dout, dq
  * [tokens, heads, head_dim] and dk, dv [tokens, kv_heads, head_dim] are contiguous, of q's type;
- * tokens at and behind cu[rows] get zeros.  work: nf4b_attn_bwd_work_bytes() bytes of device
- * scratch, 16-byte aligned, of any content; -1 for sizes outside the envelope.  */
-int64_t nf4b_attn_bwd_work_bytes(int64_t tokens, int32_t rows, int32_t heads, int32_t kv_heads);
+ * tokens at and behind cu[rows] get zeros.  work: nf4b_attn_bwd_work_bytes(a) bytes of device
+ * scratch, 16-byte aligned, of any content; -1 for a call that would be refused.  */
+int64_t nf4b_attn_bwd_work_bytes(const nf4b_attn* a);
 int nf4b_attn_bwd(const nf4b_attn* a, const void* out, const float* lse, const void* dout, void* dq,
                   void* dk, void* dv, void* work, int64_t work_bytes, void* stream);
 

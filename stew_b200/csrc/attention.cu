@@ -9,6 +9,7 @@
 // Sums and softmax statistics are fp32 (TMEM, registers), in a fixed order.
 #include <cstdlib>
 #include <mutex>
+#include <type_traits>
 
 #include "attn_common.cuh"
 
@@ -305,18 +306,18 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1)
 
 // ------------------------------------------------------------------ backward
 // Two launches.  The first (attn_prep_kernel) writes, per (head, token), the row's log-sum-exp in
-// log2 units and delta = do.o, and zeros behind the last sequence.  The second holds two kinds of
-// CTAs with one structure, a resident pair of 128-token tiles X, Y against a ring of tile pairs
+// log2 units and delta = do.o, and zeros behind the last sequence.  The second's persistent CTAs work on two
+// kinds of units with one structure, a resident pair of 128-token tiles X, Y against a ring of tile pairs
 // A, B (D = head_dim):
-//   keys    (DKV): X = K, Y = V of a key tile; A = Q, B = dO over the query tiles of every head of
-//                  the group:  S^T = X A^T, dP^T = Y B^T, dV += P^T B, dK += dS^T A
-//   queries:       X = Q, Y = dO of a query tile and head; A = K, B = V over its key tiles:
-//                  S = X A^T, dP = Y B^T, dQ += dS A
+//   keys    : X = K, Y = V of a key tile; A = Q, B = dO over the query tiles of the group's heads (or a share
+//             of them):  S^T = X A^T, dP^T = Y B^T, dV += P^T B, dK += dS^T A
+//   queries : X = Q, Y = dO of a query tile and head; A = K, B = V over its key tiles:
+//             S = X A^T, dP = Y B^T, dQ += dS A
 // S and dP are recomputed by both kinds (7 products instead of 5): that buys dQ, dK and dV summed in
-// TMEM in a fixed order, with no fp32 dQ buffer in memory and no atomics.  P and dS overwrite S and dP
-// in TMEM as 16-bit values and are the A operands of the second products from there.
+// TMEM in a fixed order, with no fp32 dQ buffer in memory and no atomics on values.  P and dS overwrite S and
+// dP in TMEM as 16-bit values and are the A operands of the second products from there.
 //   warps 0-7  elementwise: thread (row = TMEM lane, half of the columns)
-//   warp 8     TMA; in DKV CTAs also the query rows' (lse, delta) into shared memory
+//   warp 8     takes units, TMA; for key tiles also the query rows' (lse, delta) into shared memory
 //   warp 9     TMEM allocation, MMA issue
 //
 // fp16 range: dS is rounded to the operand type with a power-of-two scale 2^k that puts the largest
@@ -334,6 +335,9 @@ struct AttnWork {
   float2* row;    // [heads][tokens]: lse log2(e), delta
   float2* tile;   // [heads][slots]: max |dO_i|, max |delta_i| of a query tile
   float* vmax;    // [kv_heads][slots]: max |V_j| of a key tile
+  unsigned* next;     // the next unit of work
+  unsigned* tickets;  // [slots][kv_heads]: shares of a key tile that are done
+  float* parts;       // [slots][kv_heads][split]: their sums
 };
 
 __device__ __forceinline__ float at_half_warp_sum(float v) {
@@ -352,6 +356,10 @@ __global__ void __launch_bounds__(AT_PREP_THREADS)
   const int slot = int(blockIdx.x / p.heads), h = blockIdx.x % p.heads;
   const int grp = p.heads / p.kv_heads, hk = h / grp;
   const bool first = h % grp == 0;
+  if (threadIdx.x == 0) {
+    if (blockIdx.x == 0) *w.next = 0;
+    if (first) w.tickets[slot * p.kv_heads + hk] = 0;
+  }
   const AttnTile t = at_find(p, slot);
   if (t.i0 >= t.len) return;
   const int n = min(AT_TILE, t.len - t.i0);
@@ -424,10 +432,10 @@ __global__ void __launch_bounds__(AT_PREP_THREADS)
   }
 }
 
-// Whole warp: the exponent k of a (sequence, key/value head)'s dS scale.
-__device__ __forceinline__ int at_ds_exponent(const AttnParams& p, const AttnWork& w, const AttnTile& t, int slot, int hk) {
+// Whole warp: the exponent k of the dS scale for a tile (slot, at i0) of a sequence and a key/value head.
+__device__ __forceinline__ int at_ds_exponent(const AttnParams& p, const AttnWork& w, int slot, int i0, int len, int hk) {
   const int lane = threadIdx.x & 31, grp = p.heads / p.kv_heads;
-  const int first = slot - (t.i0 >> 7), tiles = (t.len + AT_TILE - 1) >> 7;
+  const int first = slot - (i0 >> 7), tiles = (len + AT_TILE - 1) >> 7;
   float m_do = 0.f, m_dl = 0.f, m_v = 0.f;
   for (int i = lane; i < grp * tiles; i += 32) {
     const int g = i / tiles;
@@ -456,62 +464,81 @@ struct AttnBwdSmem {
   static constexpr int Y = TILE;
   static constexpr int A = 2 * TILE;
   static constexpr int B = 4 * TILE;
-  static constexpr int AUX = 6 * TILE;             // [2][128] -lse, [2][128] -delta (scaled)
-  static constexpr int BAR = AUX + 4 * AT_TILE * 4;
-  // a_full[2], a_empty[2], b_full[2], b_empty[2], aux_full[2], aux_empty[2], xy_full, s_full, p_ready, dp_full,
-  // ds_ready, done
-  static constexpr int NBAR = 18;
+  static constexpr int OUT = 6 * TILE;             // 2 KB per elementwise warp: rows on their way out
+  static constexpr int AUX = OUT + 8 * 2048;       // [2][128] -lse, [2][128] -delta (scaled)
+  static constexpr int UNIT = AUX + 4 * AT_TILE * 4;  // [2] AttnUnit
+  static constexpr int BAR = UNIT + 2 * 64;
+  // a_full[2], a_empty[2], b_full[2], b_empty[2], aux_full[2], aux_empty[2], unit_full[2], unit_empty[2], xy_full,
+  // xy_empty, s_full, p_ready, dp_full, ds_ready, acc_full, acc_empty, joined, ticketed, drained
+  static constexpr int NBAR = 27;
   static constexpr int MISC = BAR + NBAR * 8;
   static constexpr int ALLOC = MISC + 16 + 1024;  // slack to align the base to 1024 B
 };
 static_assert(AttnBwdSmem<2>::ALLOC <= 232448, "shared memory budget");
 
-// Row pitch (floats) of a DKV CTA's sums in shared memory, dK beside dV: 16 bytes more than the
-// features, so the 16-byte stores of a warp's 32 rows fall into different banks.
-template <int DC>
-constexpr int AT_JOIN_PITCH = 2 * DC * 64 + 4;
-static_assert(AT_TILE * AT_JOIN_PITCH<2> * 4 <= AttnBwdSmem<2>::AUX && AT_TILE * AT_JOIN_PITCH<1> * 4 <= AttnBwdSmem<1>::AUX,
-              "the sums fit where the tiles were");
-
 // TMEM columns (512): S | P, dP | dS, and the two sums.
 constexpr int AT_TM_S = 0, AT_TM_DP = 128, AT_TM_DV = 256, AT_TM_DX = 384;
-
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t cluster_addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
-  return v;
-}
 
 struct AttnBwdMaps {
   CUtensorMap q, k, v, dout;
 };
 
-template <typename T, int DC, bool DKV>
-__device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const AttnParams& p, const AttnWork& w, int slot, int h,
-                                              int split, int rank, T* __restrict__ g0, T* __restrict__ g1, uint8_t* smem,
-                                              uint32_t sbase) {
+// One unit of work: a key tile and a share of its group's heads, or a query tile and a head.
+enum { AT_UNIT_QUERIES = 0, AT_UNIT_KEYS = 1, AT_UNIT_END = 2 };
+struct AttnUnit {
+  int kind, a, len, i0;  // the resident tile: tokens a + [i0, i0 + 128) of a sequence of len
+  int h, hk, rank;       // head of X and Y; key/value head; rank among the CTAs that share a key tile
+  int yt0, nt, n;        // the ring's first tile, its tiles per head, ring items
+  int h0;                // first query head of a key tile's share
+  int k_exp;             // dS is scaled by 2^k_exp
+  int join;              // the key tile's number among those that are shared
+};
+static_assert(sizeof(AttnUnit) <= 64, "one slot of the unit ring");
+
+// Adds up the key tile's sums over the CTAs that share it: float4 groups of four features of [dK | dV] by rows.
+template <int DC>
+__device__ __forceinline__ float4* at_part(float* parts, int join, int split, int rank) {
+  return reinterpret_cast<float4*>(parts) + (int64_t(join) * split + rank) * (DC * 32) * AT_TILE;
+}
+
+// Persistent: every CTA takes units from a counter, the longest kind first (key tiles with a group's heads;
+// of a causal sequence the first key tiles, which the most queries see, and the last query tiles), so that
+// the next unit's tiles are on their way and its first scores done while this unit's sums are stored.
+template <typename T, int DC>
+__global__ void __launch_bounds__(AT_BWD_THREADS, 1)
+    attn_bwd_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_constant__ AttnParams p, const AttnWork w,
+                    const int split, T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dv) {
   using L = AttnBwdSmem<DC>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t sbase = smem_u32(smem);
   uint64_t* a_full = reinterpret_cast<uint64_t*>(smem + L::BAR);
   uint64_t* a_empty = a_full + 2;
   uint64_t* b_full = a_empty + 2;
   uint64_t* b_empty = b_full + 2;
   uint64_t* aux_full = b_empty + 2;
   uint64_t* aux_empty = aux_full + 2;
-  uint64_t* xy_full = aux_empty + 2;
-  uint64_t* s_full = xy_full + 1;
+  uint64_t* unit_full = aux_empty + 2;
+  uint64_t* unit_empty = unit_full + 2;
+  uint64_t* xy_full = unit_empty + 2;
+  uint64_t* xy_empty = xy_full + 1;
+  uint64_t* s_full = xy_empty + 1;
   uint64_t* p_ready = s_full + 1;
   uint64_t* dp_full = p_ready + 1;
   uint64_t* ds_ready = dp_full + 1;
-  uint64_t* done = ds_ready + 1;
+  uint64_t* acc_full = ds_ready + 1;
+  uint64_t* acc_empty = acc_full + 1;
+  uint64_t* joined = acc_empty + 1;
+  uint64_t* ticketed = joined + 1;
+  uint64_t* drained = ticketed + 1;
   float* aux_lse = reinterpret_cast<float*>(smem + L::AUX);
   float* aux_dl = aux_lse + 2 * AT_TILE;
+  AttnUnit* units = reinterpret_cast<AttnUnit*>(smem + L::UNIT);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC + 4);
+  volatile int* ticket = reinterpret_cast<volatile int*>(smem + L::MISC + 8);
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-  const int grp = p.heads / p.kv_heads, hk = DKV ? h : h / grp;
-
-  const AttnTile t = at_find(p, slot);
-  if (t.tail || t.i0 >= t.len) return;  // rows behind the last sequence: the prep launch's
+  const int grp = p.heads / p.kv_heads;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -521,13 +548,20 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
       mbar_init(&b_empty[i], 1);
       mbar_init(&aux_full[i], 32);
       mbar_init(&aux_empty[i], 256);
+      mbar_init(&unit_full[i], 1);
+      mbar_init(&unit_empty[i], 9);
     }
     mbar_init(xy_full, 1);
+    mbar_init(xy_empty, 1);
     mbar_init(s_full, 1);
     mbar_init(p_ready, 256);
     mbar_init(dp_full, 1);
     mbar_init(ds_ready, 256);
-    mbar_init(done, 1);
+    mbar_init(acc_full, 1);
+    mbar_init(acc_empty, 256);
+    mbar_init(joined, 256);
+    mbar_init(ticketed, 1);
+    mbar_init(drained, 1);
     fence_barrier_init();
     *abort_flag = 0;
   }
@@ -535,77 +569,133 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
+  if (threadIdx.x == 256) {
+    prefetch_tma_desc(&maps.q);
+    prefetch_tma_desc(&maps.k);
+    prefetch_tma_desc(&maps.v);
+    prefetch_tma_desc(&maps.dout);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  grid_dep_wait();  // programmatic launch: no global access before the wait
 
-  // the ring's tiles (relative to a) and iterations
-  const int x_last = min(t.i0 + AT_TILE, t.len) - 1;
-  const int back = DKV ? p.right : p.left, ahead = DKV ? p.left : p.right;  // the window seen from X's side
-  const int y_lo = back < 0 ? 0 : max(0, t.i0 - back);
-  const int y_hi = ahead < 0 ? t.len - 1 : min(t.len - 1, x_last + ahead);
-  const int yt0 = y_lo >> 7, nt = (y_hi >> 7) - yt0 + 1;
-  // a DKV CTA's share of the group's heads
-  const int n = DKV ? nt * (grp / split) : nt;
-  const int h0 = DKV ? hk * grp + rank * (grp / split) : 0;
-  int k_exp = 0;
-  float sc = at_pow2(-int(at_p_shift<T>()));
-  auto ds_scale = [&] {
-    if (at_p_shift<T>() == 0.f) return;
-    k_exp = at_ds_exponent(p, w, t, slot, hk);
-    sc = at_pow2(k_exp - int(at_p_shift<T>()));
+  bool ok = true;
+  auto wait = [&](uint64_t* bar, uint32_t parity, int where) {  // whole warp
+    ok = __all_sync(0xffffffffu, ok && at_wait(bar, parity, abort_flag, where));
+    return ok;
   };
 
   if (warp == 8) {
-    // ---------------------------------------------------------------- TMA
-    bool ok = true;
-    int issued = 0;
-    if (lane == 0) {
-      mbar_arrive_expect_tx(xy_full, 2 * L::TILE);
-      for (int c = 0; c < DC; ++c) {
-        tma_load_3d(sbase + L::X + c * AT_BOX, DKV ? &maps.k : &maps.q, xy_full, c * 64, h, t.a + t.i0);
-        tma_load_3d(sbase + L::Y + c * AT_BOX, DKV ? &maps.v : &maps.dout, xy_full, c * 64, h, t.a + t.i0);
-      }
-    }
-    for (int it = 0; ok && it < n; ++it) {
-      const int s = it & 1;
-      const uint32_t ph = ((it >> 1) & 1) ^ 1;
-      const int hy = DKV ? h0 + it / nt : hk;
-      const int y0 = (yt0 + (DKV ? it % nt : it)) * AT_TILE;
-      ok = __all_sync(0xffffffffu, at_wait(&a_empty[s], ph, abort_flag, 11) && at_wait(&b_empty[s], ph, abort_flag, 12));
-      if (!ok) break;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&a_full[s], L::TILE);
-        for (int c = 0; c < DC; ++c)
-          tma_load_3d(sbase + L::A + s * L::TILE + c * AT_BOX, DKV ? &maps.q : &maps.k, &a_full[s], c * 64, hy, t.a + y0);
-        mbar_arrive_expect_tx(&b_full[s], L::TILE);
-        for (int c = 0; c < DC; ++c)
-          tma_load_3d(sbase + L::B + s * L::TILE + c * AT_BOX, DKV ? &maps.dout : &maps.v, &b_full[s], c * 64, hy, t.a + y0);
-      }
-      ++issued;
-      if (DKV) {
-        const float2* src = w.row + int64_t(hy) * p.tokens + t.a;
-        float2 x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)  // p = 0 behind the end
-          x[e] = y0 + e * 32 + lane < t.len ? src[y0 + e * 32 + lane] : make_float2(INFINITY, 0.f);
-        if (it == 0) ds_scale();  // while the first tiles are on their way
-        ok = __all_sync(0xffffffffu, at_wait(&aux_empty[s], ph, abort_flag, 13));
-        if (!ok) break;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          aux_lse[s * AT_TILE + e * 32 + lane] = at_p_shift<T>() - x[e].x;
-          aux_dl[s * AT_TILE + e * 32 + lane] = -x[e].y * sc;
+    // ---------------------------------------------------------------- units and TMA
+    const unsigned n_keys = unsigned(p.slots) * unsigned(p.kv_heads) * unsigned(split);
+    const unsigned n_all = n_keys + unsigned(p.slots) * unsigned(p.heads);
+    unsigned loads = 0, aux = 0;  // ring items so far
+    int k = 0;                    // units so far
+    for (;; ++k) {
+      // the next unit that is not empty
+      AttnUnit u;
+      u.kind = AT_UNIT_END;
+      int slot = 0;
+      for (;;) {
+        unsigned at = 0;
+        if (lane == 0) at = atomicAdd(w.next, 1u);
+        at = __shfl_sync(0xffffffffu, at, 0);
+        if (at >= n_all) break;
+        const bool keys = at < n_keys;
+        int h;
+        if (keys) {
+          u.rank = int(at % unsigned(split));
+          const unsigned b = at / unsigned(split);
+          u.join = int(b);
+          slot = int(b / unsigned(p.kv_heads));
+          h = int(b % unsigned(p.kv_heads));
+        } else {
+          u.rank = 0;
+          u.join = 0;
+          slot = p.slots - 1 - int((at - n_keys) / unsigned(p.heads));
+          h = int((at - n_keys) % unsigned(p.heads));
         }
-        mbar_arrive(&aux_full[s]);
+        const AttnTile t = at_find(p, slot);
+        if (t.tail || t.i0 >= t.len) continue;  // rows behind the last sequence: the prep launch's
+        u.kind = keys ? AT_UNIT_KEYS : AT_UNIT_QUERIES;
+        u.a = t.a;
+        u.len = t.len;
+        u.i0 = t.i0;
+        u.h = h;
+        u.hk = keys ? h : h / grp;
+        u.h0 = keys ? h * grp + u.rank * (grp / split) : 0;
+        const int back = keys ? p.right : p.left, ahead = keys ? p.left : p.right;  // the window seen from X's side
+        const int last = min(t.i0 + AT_TILE, t.len) - 1;
+        const int lo = back < 0 ? 0 : max(0, t.i0 - back), hi = ahead < 0 ? t.len - 1 : min(t.len - 1, last + ahead);
+        u.yt0 = lo >> 7;
+        u.nt = (hi >> 7) - u.yt0 + 1;
+        u.n = keys ? u.nt * (grp / split) : u.nt;
+        break;
+      }
+      const bool keys = u.kind == AT_UNIT_KEYS;
+      u.k_exp = 0;
+      if (at_p_shift<T>() != 0.f && u.kind != AT_UNIT_END) u.k_exp = at_ds_exponent(p, w, slot, u.i0, u.len, u.hk);
+      if (!wait(&unit_empty[k & 1], ((k >> 1) & 1) ^ 1, 10)) break;
+      if (lane == 0) {
+        units[k & 1] = u;
+        mbar_arrive(&unit_full[k & 1]);
+      }
+      if (u.kind == AT_UNIT_END) break;
+      if (!wait(xy_empty, (k & 1) ^ 1, 9)) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(xy_full, 2 * L::TILE);
+        for (int c = 0; c < DC; ++c) {
+          tma_load_3d(sbase + L::X + c * AT_BOX, keys ? &maps.k : &maps.q, xy_full, c * 64, u.h, u.a + u.i0);
+          tma_load_3d(sbase + L::Y + c * AT_BOX, keys ? &maps.v : &maps.dout, xy_full, c * 64, u.h, u.a + u.i0);
+        }
+      }
+      const float sc = at_pow2(u.k_exp - int(at_p_shift<T>()));
+      for (int it = 0; it < u.n; ++it) {
+        const int s = loads & 1;
+        const uint32_t ph = ((loads >> 1) & 1) ^ 1;
+        const int hy = keys ? u.h0 + it / u.nt : u.hk;
+        const int y0 = (u.yt0 + (keys ? it % u.nt : it)) * AT_TILE;
+        if (!wait(&a_empty[s], ph, 11) || !wait(&b_empty[s], ph, 12)) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&a_full[s], L::TILE);
+          for (int c = 0; c < DC; ++c)
+            tma_load_3d(sbase + L::A + s * L::TILE + c * AT_BOX, keys ? &maps.q : &maps.k, &a_full[s], c * 64, hy, u.a + y0);
+          mbar_arrive_expect_tx(&b_full[s], L::TILE);
+          for (int c = 0; c < DC; ++c)
+            tma_load_3d(sbase + L::B + s * L::TILE + c * AT_BOX, keys ? &maps.dout : &maps.v, &b_full[s], c * 64, hy,
+                        u.a + y0);
+        }
+        ++loads;
+        if (keys) {
+          const float2* src = w.row + int64_t(hy) * p.tokens + u.a;
+          float2 x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)  // p = 0 behind the end
+            x[e] = y0 + e * 32 + lane < u.len ? src[y0 + e * 32 + lane] : make_float2(INFINITY, 0.f);
+          const int sa = aux & 1;
+          if (!wait(&aux_empty[sa], ((aux >> 1) & 1) ^ 1, 13)) break;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            aux_lse[sa * AT_TILE + e * 32 + lane] = at_p_shift<T>() - x[e].x;
+            aux_dl[sa * AT_TILE + e * 32 + lane] = -x[e].y * sc;
+          }
+          mbar_arrive(&aux_full[sa]);
+          ++aux;
+        }
+      }
+      if (!ok) {
+        ++k;
+        break;
       }
     }
-    if (*abort_flag && lane == 0) {
-      at_drain(xy_full, 0);
-      for (int it = max(0, issued - 2); it < issued; ++it) {
-        at_drain(&a_full[it & 1], (it >> 1) & 1);
-        at_drain(&b_full[it & 1], (it >> 1) & 1);
+    // an abandoned CTA's loads must have landed before its shared memory goes
+    if (!ok && lane == 0) {
+      if (k > 0) at_drain(xy_full, (k - 1) & 1);
+      for (unsigned i = loads > 2 ? loads - 2 : 0; i < loads; ++i) {
+        at_drain(&a_full[i & 1], (i >> 1) & 1);
+        at_drain(&b_full[i & 1], (i >> 1) & 1);
       }
     }
   } else if (warp == 9) {
@@ -617,6 +707,7 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
     const uint64_t dx = smem_desc_sw128(sbase + L::X, 16, 1024), dy = smem_desc_sw128(sbase + L::Y, 16, 1024);
     const uint64_t da = smem_desc_sw128(sbase + L::A, 16, 1024), db = smem_desc_sw128(sbase + L::B, 16, 1024);
     const uint64_t ta = smem_desc_sw128(sbase + L::A, AT_BOX, 1024), tb = smem_desc_sw128(sbase + L::B, AT_BOX, 1024);
+    constexpr uint64_t STEP = uint64_t(L::TILE >> 4);
     // d (128 x 128) = x a^T over head_dim
     auto scores = [&](uint32_t d, uint64_t x, uint64_t a) {
 #pragma unroll
@@ -632,263 +723,252 @@ __device__ __forceinline__ void attn_bwd_role(const AttnBwdMaps& maps, const Att
       for (int k = 0; k < AT_TILE / 16; ++k)
         at_mma_ts(lead, d, pm + (k >> 2) * 64 + (k & 3) * 8, b + uint64_t(k * (2048 >> 4)), id_g, acc || k > 0);
     };
-    constexpr uint64_t STEP = uint64_t(L::TILE >> 4);
-    bool ok = true;
-    auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
-      ok = __all_sync(0xffffffffu, ok && at_wait(bar, parity, abort_flag, where));
-      if (ok) tc_fence_after();
-      return ok;
-    };
-    if (wait(xy_full, 0, 15) && wait(&a_full[0], 0, 16)) {
-      scores(tmem + AT_TM_S, dx, da);
+    unsigned r = 0;  // ring items so far
+    // S and dP of ring item i, overwriting P and dS of the one before: MMAs of one thread run in order
+    auto s_of = [&](unsigned i) {
+      if (!wait(&a_full[i & 1], (i >> 1) & 1, 16)) return false;
+      tc_fence_after();
+      scores(tmem + AT_TM_S, dx, da + (i & 1) * STEP);
       at_commit(lead, s_full);
-      if (wait(&b_full[0], 0, 17)) {
-        scores(tmem + AT_TM_DP, dy, db);
-        at_commit(lead, dp_full);
-        if (!DKV) at_commit(lead, &b_empty[0]);
+      return true;
+    };
+    auto dp_of = [&](unsigned i, bool keys) {
+      if (!wait(&b_full[i & 1], (i >> 1) & 1, 17)) return false;
+      tc_fence_after();
+      scores(tmem + AT_TM_DP, dy, db + (i & 1) * STEP);
+      at_commit(lead, dp_full);
+      if (!keys) at_commit(lead, &b_empty[i & 1]);
+      return true;
+    };
+    for (int k = 0;; ++k) {
+      if (!wait(&unit_full[k & 1], (k >> 1) & 1, 15)) break;
+      const int kind = __shfl_sync(0xffffffffu, units[k & 1].kind, 0), n = __shfl_sync(0xffffffffu, units[k & 1].n, 0);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&unit_empty[k & 1]);
+      if (kind == AT_UNIT_END) break;
+      const bool keys = kind == AT_UNIT_KEYS;
+      if (!wait(xy_full, k & 1, 18) || !s_of(r) || !dp_of(r, keys)) break;
+      if (n == 1) at_commit(lead, xy_empty);
+      for (int it = 0; it < n; ++it, ++r) {
+        const bool more = it + 1 < n;
+        if (!wait(p_ready, r & 1, 19)) break;
+        // the sums of the unit before have been read
+        if (it == 0 && !wait(acc_empty, (k & 1) ^ 1, 20)) break;
+        tc_fence_after();
+        if (keys) {
+          sum(tmem + AT_TM_DV, tmem + AT_TM_S, tb + (r & 1) * STEP, it > 0);
+          at_commit(lead, &b_empty[r & 1]);
+        }
+        if (more && !s_of(r + 1)) break;
+        if (!wait(ds_ready, r & 1, 21)) break;
+        tc_fence_after();
+        sum(tmem + AT_TM_DX, tmem + AT_TM_DP, ta + (r & 1) * STEP, it > 0);
+        at_commit(lead, &a_empty[r & 1]);
+        if (more && !dp_of(r + 1, keys)) break;
+        if (it + 2 == n) at_commit(lead, xy_empty);  // no more scores of this unit
       }
+      if (!ok) break;
+      at_commit(lead, acc_full);
     }
-    for (int it = 0; ok && it < n; ++it) {
-      const int s = it & 1, s1 = s ^ 1;
-      const uint32_t ph = it & 1, ph1 = ((it + 1) >> 1) & 1;
-      const bool more = it + 1 < n;
-      if (!wait(p_ready, ph, 18)) break;
-      if (DKV) {
-        sum(tmem + AT_TM_DV, tmem + AT_TM_S, tb + s * STEP, it > 0);
-        at_commit(lead, &b_empty[s]);
-      }
-      if (more) {
-        if (!wait(&a_full[s1], ph1, 19)) break;
-        scores(tmem + AT_TM_S, dx, da + s1 * STEP);  // after the product that reads P: MMAs run in order
-        at_commit(lead, s_full);
-      }
-      if (!wait(ds_ready, ph, 20)) break;
-      sum(tmem + AT_TM_DX, tmem + AT_TM_DP, ta + s * STEP, it > 0);
-      at_commit(lead, &a_empty[s]);
-      if (more) {
-        if (!wait(&b_full[s1], ph1, 21)) break;
-        scores(tmem + AT_TM_DP, dy, db + s1 * STEP);
-        at_commit(lead, dp_full);
-        if (!DKV) at_commit(lead, &b_empty[s1]);
-      }
+    if (!ok) {  // nothing in flight when TMEM and shared memory go
+      at_commit(lead, drained);
+      at_drain(drained, 0);
     }
-    at_commit(lead, done);
-    at_drain(done, 0);  // nothing in flight when TMEM and shared memory go
   } else {
     // ---------------------------------------------------------------- elementwise
     const int half = warp >> 2;  // columns [64 half, 64 half + 64)
-    const int r = (warp & 3) * 32 + lane;
-    const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
+    const int w0 = (warp & 3) * 32, row = w0 + lane;
+    const uint32_t lane_off = uint32_t(w0) << 16;
     const uint32_t t_s = tmem + AT_TM_S + lane_off + half * 64, t_dp = tmem + AT_TM_DP + lane_off + half * 64;
-    const int x = t.i0 + r;  // this thread's row, relative to a
     const float sl2 = p.scale * AT_LOG2E;
-    const int see_lo = back < 0 ? 0 : x - back;
-    const int see_hi = ahead < 0 ? t.len - 1 : min(t.len - 1, x + ahead);
-    uint64_t row_lse = 0, row_dl = 0;  // twice each
-    ds_scale();
-    if (!DKV) {
-      const float2 v = x < t.len ? w.row[int64_t(h) * p.tokens + t.a + x] : make_float2(INFINITY, 0.f);
-      row_lse = f2_pack(at_p_shift<T>() - v.x, at_p_shift<T>() - v.x);
-      row_dl = f2_pack(-v.y * sc, -v.y * sc);
-    }
-    bool ok = true;
-    for (int it = 0; it < n; ++it) {
-      const int s = it & 1;
-      const int y0 = (yt0 + (DKV ? it % nt : it)) * AT_TILE + half * 64;
-      ok = at_wait(s_full, it & 1, abort_flag, 22);
-      if (DKV) ok = ok && at_wait(&aux_full[s], (it >> 1) & 1, abort_flag, 23);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      tc_fence_after();
-      const bool cut = y0 + 64 > t.len || (ahead >= 0 && y0 + 63 > t.i0 + ahead) ||
-                       (back >= 0 && y0 < t.i0 + AT_TILE - 1 - back);
-      // rows of other sequences behind a ragged ring tile must add nothing to a sum over its tokens: Q's and dO's
-      // in DKV CTAs, K's in the others (V only meets scores that are masked).  The scores that read the tiles
-      // are done by then.
-      const int end = t.len - (y0 - half * 64);
-      if (end < AT_TILE) {
-        if (DKV) {
-          ok = at_wait(dp_full, it & 1, abort_flag, 14);
-          if (!__all_sync(0xffffffffu, ok)) break;
-          at_zero_rows<DC, AT_TILE, 256>(smem + L::B + s * L::TILE, end, threadIdx.x);
-        }
-        at_zero_rows<DC, AT_TILE, 256>(smem + L::A + s * L::TILE, end, threadIdx.x);
-      }
-      uint32_t sv[64];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(t_s + c * 32, *reinterpret_cast<uint32_t(*)[32]>(sv + c * 32));
-      tmem_ld_wait();
-      if (!DKV) {
-        tc_fence_before();
-        mbar_arrive(p_ready);  // the scores are in registers: the next tile's may overwrite them
-      }
-      uint64_t pv[32];
-      const uint64_t sl2x2 = f2_pack(sl2, sl2);
-      const ulonglong2* la = reinterpret_cast<const ulonglong2*>(aux_lse + s * AT_TILE + half * 64);
-#pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        ulonglong2 l4 = make_ulonglong2(row_lse, row_lse);
-        if (DKV) l4 = la[c];
-        const float2 x = f2_unpack(f2_fma(f2_pack_u(sv[4 * c], sv[4 * c + 1]), sl2x2, l4.x));
-        const float2 y = f2_unpack(f2_fma(f2_pack_u(sv[4 * c + 2], sv[4 * c + 3]), sl2x2, l4.y));
-        pv[2 * c] = f2_pack(at_exp2(x.x), at_exp2(x.y));
-        pv[2 * c + 1] = f2_pack(at_exp2(y.x), at_exp2(y.y));
-      }
-      if (cut) {
-#pragma unroll
-        for (int c = 0; c < 64; c += 2) {
-          const float2 v = f2_unpack(pv[c >> 1]);
-          pv[c >> 1] = f2_pack(y0 + c < see_lo || y0 + c > see_hi ? 0.f : v.x,
-                               y0 + c + 1 < see_lo || y0 + c + 1 > see_hi ? 0.f : v.y);
-        }
-      }
-      if (DKV) {
-        uint32_t pk[32];
-#pragma unroll
-        for (int k = 0; k < 32; ++k) {
-          const float2 v = f2_unpack(pv[k]);
-          pk[k] = at_pack<T>(v.x, v.y);  // the MMA's operand type
-        }
-        tmem_st_32x32b_x32(t_s, pk);
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(p_ready);
-      }
-      ok = at_wait(dp_full, it & 1, abort_flag, 24);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      tc_fence_after();
-      uint32_t dv[64];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(t_dp + c * 32, *reinterpret_cast<uint32_t(*)[32]>(dv + c * 32));
-      tmem_ld_wait();
+    const uint64_t sl2x2 = f2_pack(sl2, sl2);
+    uint8_t* buf = smem + L::OUT + warp * 2048;
+    unsigned r = 0, aux = 0;
+    int joins = 0;
+    // One unit's ring items.
+    auto items = [&](auto keys_tag, const AttnUnit& u) {
+      constexpr bool KEYS = decltype(keys_tag)::value;
+      const int x = u.i0 + row;  // this thread's row, relative to a
+      const float sc = at_pow2(u.k_exp - int(at_p_shift<T>()));
       const uint64_t scx2 = f2_pack(sc, sc);
-      const ulonglong2* ld = reinterpret_cast<const ulonglong2*>(aux_dl + s * AT_TILE + half * 64);
-#pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        ulonglong2 d4 = make_ulonglong2(row_dl, row_dl);
-        if (DKV) d4 = ld[c];
-        pv[2 * c] = f2_mul(pv[2 * c], f2_fma(f2_pack_u(dv[4 * c], dv[4 * c + 1]), scx2, d4.x));
-        pv[2 * c + 1] = f2_mul(pv[2 * c + 1], f2_fma(f2_pack_u(dv[4 * c + 2], dv[4 * c + 3]), scx2, d4.y));
+      const int back = KEYS ? p.right : p.left, ahead = KEYS ? p.left : p.right;
+      const int see_lo = back < 0 ? 0 : x - back;
+      const int see_hi = ahead < 0 ? u.len - 1 : min(u.len - 1, x + ahead);
+      uint64_t row_lse = 0, row_dl = 0;  // twice each
+      if (!KEYS) {
+        const float2 v = x < u.len ? w.row[int64_t(u.h) * p.tokens + u.a + x] : make_float2(INFINITY, 0.f);
+        row_lse = f2_pack(at_p_shift<T>() - v.x, at_p_shift<T>() - v.x);
+        row_dl = f2_pack(-v.y * sc, -v.y * sc);
       }
-      if (cut) {  // a hidden pair adds nothing, whatever its dP is
+      for (int it = 0; it < u.n; ++it, ++r) {
+        const int s = r & 1, sa = aux & 1;
+        const int y0 = (u.yt0 + (KEYS ? it % u.nt : it)) * AT_TILE + half * 64;
+        if (!wait(s_full, r & 1, 22)) return;
+        if (KEYS && !wait(&aux_full[sa], (aux >> 1) & 1, 23)) return;
+        tc_fence_after();
+        const bool cut = y0 + 64 > u.len || (ahead >= 0 && y0 + 63 > u.i0 + ahead) ||
+                         (back >= 0 && y0 < u.i0 + AT_TILE - 1 - back);
+        // rows of other sequences behind a ragged ring tile must add nothing to a sum over its tokens: Q's and dO's
+        // for a key tile, K's for a query tile (V only meets scores that are masked).  The scores that read the
+        // tiles are done by then.
+        const int end = u.len - (y0 - half * 64);
+        if (end < AT_TILE) {
+          if (KEYS) {
+            if (!wait(dp_full, r & 1, 14)) return;
+            at_zero_rows<DC, AT_TILE, 256>(smem + L::B + s * L::TILE, end, threadIdx.x);
+          }
+          at_zero_rows<DC, AT_TILE, 256>(smem + L::A + s * L::TILE, end, threadIdx.x);
+        }
+        uint32_t sv[64];
 #pragma unroll
-        for (int c = 0; c < 64; c += 2) {
-          const float2 v = f2_unpack(pv[c >> 1]);
-          pv[c >> 1] = f2_pack(y0 + c < see_lo || y0 + c > see_hi ? 0.f : v.x,
-                               y0 + c + 1 < see_lo || y0 + c + 1 > see_hi ? 0.f : v.y);
+        for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(t_s + c * 32, *reinterpret_cast<uint32_t(*)[32]>(sv + c * 32));
+        tmem_ld_wait();
+        if (!KEYS) {
+          tc_fence_before();
+          mbar_arrive(p_ready);  // the scores are in registers: the next tile's may overwrite them
+        }
+        uint64_t pv[32];
+        const ulonglong2* la = reinterpret_cast<const ulonglong2*>(aux_lse + sa * AT_TILE + half * 64);
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          ulonglong2 l4 = make_ulonglong2(row_lse, row_lse);
+          if (KEYS) l4 = la[c];
+          const float2 f = f2_unpack(f2_fma(f2_pack_u(sv[4 * c], sv[4 * c + 1]), sl2x2, l4.x));
+          const float2 g = f2_unpack(f2_fma(f2_pack_u(sv[4 * c + 2], sv[4 * c + 3]), sl2x2, l4.y));
+          pv[2 * c] = f2_pack(at_exp2(f.x), at_exp2(f.y));
+          pv[2 * c + 1] = f2_pack(at_exp2(g.x), at_exp2(g.y));
+        }
+        auto hide = [&] {  // 0 where the pair is not visible, whatever is there
+#pragma unroll
+          for (int c = 0; c < 64; c += 2) {
+            const float2 v = f2_unpack(pv[c >> 1]);
+            pv[c >> 1] = f2_pack(y0 + c < see_lo || y0 + c > see_hi ? 0.f : v.x,
+                                 y0 + c + 1 < see_lo || y0 + c + 1 > see_hi ? 0.f : v.y);
+          }
+        };
+        auto put = [&](uint32_t taddr) {  // rounded to the MMA's operand type
+          uint32_t pk[32];
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            const float2 v = f2_unpack(pv[k]);
+            pk[k] = at_pack<T>(v.x, v.y);
+          }
+          tmem_st_32x32b_x32(taddr, pk);
+          tmem_st_wait();
+          tc_fence_before();
+        };
+        if (cut) hide();
+        if (KEYS) {
+          put(t_s);
+          mbar_arrive(p_ready);
+        }
+        if (!wait(dp_full, r & 1, 24)) return;
+        tc_fence_after();
+        uint32_t dpv[64];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(t_dp + c * 32, *reinterpret_cast<uint32_t(*)[32]>(dpv + c * 32));
+        tmem_ld_wait();
+        const ulonglong2* ld = reinterpret_cast<const ulonglong2*>(aux_dl + sa * AT_TILE + half * 64);
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          ulonglong2 d4 = make_ulonglong2(row_dl, row_dl);
+          if (KEYS) d4 = ld[c];
+          pv[2 * c] = f2_mul(pv[2 * c], f2_fma(f2_pack_u(dpv[4 * c], dpv[4 * c + 1]), scx2, d4.x));
+          pv[2 * c + 1] = f2_mul(pv[2 * c + 1], f2_fma(f2_pack_u(dpv[4 * c + 2], dpv[4 * c + 3]), scx2, d4.y));
+        }
+        if (cut) hide();
+        put(t_dp);
+        mbar_arrive(ds_ready);
+        if (KEYS) {
+          mbar_arrive(&aux_empty[sa]);
+          ++aux;
         }
       }
-      uint32_t pk[32];
-#pragma unroll
-      for (int k = 0; k < 32; ++k) {
-        const float2 v = f2_unpack(pv[k]);
-        pk[k] = at_pack<T>(v.x, v.y);
-      }
-      tmem_st_32x32b_x32(t_dp, pk);
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(ds_ready);
-      if (DKV) mbar_arrive(&aux_empty[s]);
-    }
-    if (__all_sync(0xffffffffu, ok)) ok = at_wait(done, 0, abort_flag, 25);
-    if (__all_sync(0xffffffffu, ok)) {
+    };
+    for (int k = 0;; ++k) {
+      if (!wait(&unit_full[k & 1], (k >> 1) & 1, 25)) break;
+      const AttnUnit u = units[k & 1];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&unit_empty[k & 1]);
+      if (u.kind == AT_UNIT_END) break;
+      const bool keys = u.kind == AT_UNIT_KEYS;
+      if (keys) items(std::true_type{}, u);
+      else items(std::false_type{}, u);
+      if (!ok || !wait(acc_full, k & 1, 26)) break;
       tc_fence_after();
-      const float fx = p.scale * at_pow2(-k_exp);
-      if (DKV && split > 1) {
-        // fp32 to this CTA's shared memory (its tiles are done with): [128 rows][dK | dV]
+      const int rows = u.len - u.i0 - w0;  // of this warp's 32
+      const float fx = p.scale * at_pow2(-u.k_exp);
+      if (!keys) {
+        const int c0 = half * DC * 32;
+        T* to = dq + (int64_t(u.a + u.i0 + w0) * p.heads + u.h) * p.head_dim + c0;
+#pragma unroll
+        for (int c = 0; c < DC * 32; c += 32)
+          at_store_rows<T, 32>(tmem + AT_TM_DX + lane_off + c0 + c, buf, to + c, int64_t(p.heads) * p.head_dim, rows,
+                               p.head_dim - c0 - c, fx);
+      } else {
         const uint32_t from = tmem + (half == 0 ? AT_TM_DX : AT_TM_DV) + lane_off;
         const float f = half == 0 ? fx : at_pow2(-int(at_p_shift<T>()));
-        float* row = reinterpret_cast<float*>(smem) + r * AT_JOIN_PITCH<DC> + half * DC * 64;
-#pragma unroll 1
-        for (int c = 0; c < DC * 64; c += 32) {
-          uint32_t o[32];
-          tmem_ld_32x32b_x32(from + c, o);
-          tmem_ld_wait();
+        T* to = (half == 0 ? dk : dv) + (int64_t(u.a + u.i0 + w0) * p.kv_heads + u.h) * p.head_dim;
+        const int64_t pitch = int64_t(p.kv_heads) * p.head_dim;
+        if (split == 1) {
 #pragma unroll
-          for (int k = 0; k < 32; k += 4)
-            *reinterpret_cast<float4*>(row + c + k) =
-                make_float4(__uint_as_float(o[k]) * f, __uint_as_float(o[k + 1]) * f, __uint_as_float(o[k + 2]) * f,
-                            __uint_as_float(o[k + 3]) * f);
-        }
-      } else {
-        // the tiles' memory is free: every MMA is done
-        const int heads = DKV ? p.kv_heads : p.heads, w0 = (warp & 3) * 32;
-        const int64_t first = (int64_t(t.a + t.i0 + w0) * heads + h) * p.head_dim, pitch = int64_t(heads) * p.head_dim;
-        uint8_t* buf = smem + warp * 32 * DC * 128;
-        if (DKV) {
-          at_store_rows<T, DC * 64>(tmem + (half == 0 ? AT_TM_DX : AT_TM_DV) + lane_off, buf, (half == 0 ? g0 : g1) + first, pitch,
-                           t.len - t.i0 - w0, p.head_dim, half == 0 ? fx : at_pow2(-int(at_p_shift<T>())));
+          for (int c = 0; c < DC * 64; c += 32)
+            at_store_rows<T, 32>(from + c, buf, to + c, pitch, rows, p.head_dim - c, f);
         } else {
-          const int c0 = half * DC * 32, cols = min(p.head_dim - c0, DC * 32);
-          if (cols > 0)
-            at_store_rows<T, DC * 32>(tmem + AT_TM_DX + lane_off + c0, buf, g0 + first + c0, pitch, t.len - t.i0 - w0, cols, fx);
+          // this share's sums to memory; whoever comes last adds all of them up, share by share
+          float4* mine = at_part<DC>(w.parts, u.join, split, u.rank) + half * DC * 16 * AT_TILE + row;
+#pragma unroll 1
+          for (int c = 0; c < DC * 64; c += 32) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(from + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              mine[(c + e) / 4 * AT_TILE] = make_float4(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f,
+                                                        __uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f);
+          }
+          __threadfence();
+          mbar_arrive(joined);
+          if (!wait(joined, joins & 1, 27)) break;
+          if (threadIdx.x == 0) {
+            *ticket = int(atomicAdd(w.tickets + u.join, 1u));
+            __threadfence();
+            mbar_arrive(ticketed);
+          }
+          if (!wait(ticketed, joins & 1, 28)) break;
+          ++joins;
+          if (*ticket == split - 1) {
+            const float4* all = at_part<DC>(w.parts, u.join, split, 0) + half * DC * 16 * AT_TILE + row;
+#pragma unroll 1
+            for (int c = 0; c < DC * 64; c += 32) {
+              float4 v[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] = __ldcg(all + (c / 4 + e) * AT_TILE);
+#pragma unroll 1
+              for (int q = 1; q < split; ++q) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  const float4 y = __ldcg(all + int64_t(q) * (DC * 32) * AT_TILE + (c / 4 + e) * AT_TILE);
+                  v[e].x += y.x, v[e].y += y.y, v[e].z += y.z, v[e].w += y.w;
+                }
+              }
+#pragma unroll
+              for (int e = 0; e < 8; e += 2)
+                if (lane < rows && c + e * 4 < p.head_dim)
+                  *reinterpret_cast<uint4*>(to + lane * pitch + c + e * 4) =
+                      make_uint4(at_pack<T>(v[e].x, v[e].y), at_pack<T>(v[e].z, v[e].w), at_pack<T>(v[e + 1].x, v[e + 1].y),
+                                 at_pack<T>(v[e + 1].z, v[e + 1].w));
+            }
+          }
         }
       }
+      tc_fence_before();
+      mbar_arrive(acc_empty);
     }
     tc_fence_before();
   }
   __syncthreads();
   if (warp == 9) tmem_dealloc(tmem, 512);
-  if (DKV && split > 1) {
-    // the cluster's CTAs add up their heads' sums, rank by rank, each a share of the 8-feature pieces
-    cluster_sync_all();
-    if (warp < 8) {
-      const int per = 2 * DC * 8, live = min(AT_TILE, t.len - t.i0);
-      for (int i = rank * 256 + threadIdx.x; i < live * per; i += split * 256) {
-        const int row = i / per, c = (i % per) * 8;  // column of [dK | dV]
-        const int f = c & (DC * 64 - 1);
-        if (f >= p.head_dim) continue;
-        const uint32_t at = sbase + uint32_t(row * AT_JOIN_PITCH<DC> + c) * 4;
-        float4 v[8][2];  // all peers' loads in flight
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-          if (q < split) {
-            const uint32_t peer = mapa_shared(at, q);
-            v[q][0] = ld_cluster_f4(peer);
-            v[q][1] = ld_cluster_f4(peer + 16);
-          }
-        float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-          if (q < split) {
-            sum[0] += v[q][0].x, sum[1] += v[q][0].y, sum[2] += v[q][0].z, sum[3] += v[q][0].w;
-            sum[4] += v[q][1].x, sum[5] += v[q][1].y, sum[6] += v[q][1].z, sum[7] += v[q][1].w;
-          }
-        T* to = (c < DC * 64 ? g0 : g1) + (int64_t(t.a + t.i0 + row) * p.kv_heads + h) * p.head_dim + f;
-        *reinterpret_cast<uint4*>(to) = make_uint4(at_pack<T>(sum[0], sum[1]), at_pack<T>(sum[2], sum[3]),
-                                                   at_pack<T>(sum[4], sum[5]), at_pack<T>(sum[6], sum[7]));
-      }
-    }
-    cluster_sync_all();  // no CTA leaves while its sums are read
-  }
-}
-
-template <typename T, int DC>
-__global__ void __launch_bounds__(AT_BWD_THREADS, 1)
-    attn_bwd_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_constant__ AttnParams p, const AttnWork w,
-                    int split, T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dv) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  if (threadIdx.x == 256) {
-    prefetch_tma_desc(&maps.q);
-    prefetch_tma_desc(&maps.k);
-    prefetch_tma_desc(&maps.v);
-    prefetch_tma_desc(&maps.dout);
-  }
-  grid_dep_wait();  // programmatic launch: no global access before the wait
-  // the CTAs of key tiles first, a causal sequence's first tiles, which the most queries see,
-  // before its last; the query tiles the other way round.  `split` CTAs (a cluster) share a key
-  // tile's heads; the grid is a multiple of it.
-  const unsigned n_dkv = unsigned(p.slots) * unsigned(p.kv_heads) * unsigned(split);
-  if (blockIdx.x < n_dkv) {
-    const unsigned b = blockIdx.x / split;
-    attn_bwd_role<T, DC, true>(maps, p, w, b / p.kv_heads, b % p.kv_heads, split, blockIdx.x % split, dk, dv, smem,
-                               smem_u32(smem));
-  } else {
-    const unsigned b = blockIdx.x - n_dkv;
-    if (b >= unsigned(p.slots) * unsigned(p.heads)) return;
-    attn_bwd_role<T, DC, false>(maps, p, w, p.slots - 1 - int(b / p.heads), b % p.heads, 1, 0, dq, nullptr, smem,
-                                smem_u32(smem));
-  }
 }
 
 static bool attn_strides_ok(int64_t stride, int64_t head_stride, const nf4b_attn& a, int heads) {
@@ -1003,28 +1083,22 @@ extern "C" int nf4b_attn_error_flag(int* value, int reset) {
   return NF4B_OK;
 }
 
-static int64_t attn_work(int64_t tokens, int64_t slots, int64_t heads, int64_t kv_heads, void* base, AttnWork* w) {
-  const int64_t rows = heads * tokens * 8, tiles = heads * slots * 8, vmax = kv_heads * slots * 4;
-  if (w != nullptr) {
-    char* b = static_cast<char*>(base);
-    w->row = reinterpret_cast<float2*>(b);
-    w->tile = reinterpret_cast<float2*>(b + rows);
-    w->vmax = reinterpret_cast<float*>(b + rows + tiles);
+static int attn_sms() {
+  static int cached[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (cached[dev] == 0) {
+    int v = 0;
+    cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
+    cached[dev] = v > 0 ? v : 148;
   }
-  return (rows + tiles + vmax + 15) / 16 * 16;
+  return cached[dev];
 }
 
-extern "C" int64_t nf4b_attn_bwd_work_bytes(int64_t tokens, int32_t rows, int32_t heads, int32_t kv_heads) {
-  if (tokens < 0 || rows < 0 || heads <= 0 || kv_heads <= 0 || tokens > 0x3FFFFFFF || rows > 0x3FFFFFFF ||
-      heads > 65535 || heads % kv_heads != 0)
-    return -1;
-  return attn_work(tokens, at_slots(tokens, rows, 7), heads, kv_heads, nullptr, nullptr);
-}
-
-// CTAs that share a key tile's heads: the divisor of the group (at most 8, a cluster) with the
-// shortest estimated time on 148 SMs, from an average sequence: the longer of all CTAs' work
-// shared out and the longest key-tile CTA.  In microseconds, as measured: about 4 of set-up and
-// store for a CTA, 1 more for the join, 1.2 a key-tile step, 0.9 a query-tile step.
+// CTAs that share a key tile's heads: the divisor of the group with the shortest estimated time on 148 SMs,
+// from an average sequence: the longer of all units' work shared out and the longest key-tile unit.  In
+// microseconds, as measured: about 3 of start and store for a unit, 3 more for a shared one, 1.6 a key-tile
+// step, 1.2 a query-tile step.
 static int attn_split(const nf4b_attn& a) {
   const int grp = a.heads / a.kv_heads;
   const double len = double(a.tokens) / (a.rows > 0 ? a.rows : 1);
@@ -1034,11 +1108,13 @@ static int attn_split(const nf4b_attn& a) {
   const double tiles = double(a.tokens) / AT_TILE + 0.5 * a.rows;
   int best = 1;
   double best_us = 0;
-  for (int c = 1; c <= 8 && c <= grp; ++c) {
-    if (grp % c != 0) continue;
-    const double keys = tiles * a.kv_heads * c * (4.0 + (c > 1 ? 1.0 : 0.0) + 1.2 * mean * (grp / c));
-    const double queries = tiles * a.heads * (4.0 + 0.9 * mean);
-    const double all = (keys + queries) / 148, longest = 5.0 + 1.2 * most * (grp / c);
+  for (int c = 1; c <= grp; ++c) {
+    // (the shares' sums: 1 KB a key row, share and 128 features)
+    if (grp % c != 0 || (c > 1 && double(at_slots(a.tokens, a.rows, 7)) * a.kv_heads * c > 4096)) continue;
+    const double one = 3.0 + (c > 1 ? 3.0 : 0.0);
+    const double keys = tiles * a.kv_heads * c * (one + 1.6 * mean * (grp / c));
+    const double queries = tiles * a.heads * (3.0 + 1.2 * mean);
+    const double all = (keys + queries) / 148, longest = one + 1.6 * most * (grp / c);
     const double us = all > longest ? all : longest;
     if (c == 1 || us < best_us) {
       best = c;
@@ -1046,13 +1122,39 @@ static int attn_split(const nf4b_attn& a) {
     }
   }
   const char* v = std::getenv("STEW_ATTN_SPLIT");
-  if (v != nullptr && v[0] >= '1' && v[0] <= '8' && grp % (v[0] - '0') == 0) best = v[0] - '0';
+  if (v != nullptr && v[0] >= '1' && v[0] <= '9' && grp % (v[0] - '0') == 0) best = v[0] - '0';
   return best;
+}
+
+static int64_t attn_work(const nf4b_attn& a, int split, void* base, AttnWork* w) {
+  const int64_t slots = at_slots(a.tokens, a.rows, 7), pairs = slots * a.kv_heads;
+  char* b = static_cast<char*>(base);
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    char* here = b + at;
+    at += (bytes + 15) / 16 * 16;
+    return here;
+  };
+  AttnWork x;
+  x.row = reinterpret_cast<float2*>(take(a.heads * a.tokens * 8));
+  x.tile = reinterpret_cast<float2*>(take(a.heads * slots * 8));
+  x.vmax = reinterpret_cast<float*>(take(pairs * 4));
+  x.next = reinterpret_cast<unsigned*>(take(4));
+  x.tickets = reinterpret_cast<unsigned*>(take(pairs * 4));
+  x.parts = reinterpret_cast<float*>(take(split > 1 ? pairs * split * AT_TILE * (a.head_dim > 64 ? 256 : 128) * 4 : 0));
+  if (w != nullptr) *w = x;
+  return at;
+}
+
+extern "C" int64_t nf4b_attn_bwd_work_bytes(const nf4b_attn* args) {
+  nf4b_attn a;
+  if (attn_checks(args, &a) != NF4B_OK) return -1;
+  return attn_work(a, attn_split(a), nullptr, nullptr);
 }
 
 template <typename T, int DC>
 static int attn_bwd_launch(const nf4b_attn& a, const void* out, const float* lse, const void* dout, void* dq, void* dk,
-                           void* dv, void* work, cudaStream_t s) {
+                           void* dv, void* work, int split, cudaStream_t s) {
   AttnBwdMaps m;
   int st = attn_tmap(&m.q, a, a.q, a.heads, a.q_stride, a.q_head_stride, AT_TILE);
   if (st == NF4B_OK) st = attn_tmap(&m.k, a, a.k, a.kv_heads, a.k_stride, a.k_head_stride, AT_TILE);
@@ -1063,27 +1165,14 @@ static int attn_bwd_launch(const nf4b_attn& a, const void* out, const float* lse
   if (st != NF4B_OK) return st;
   const AttnParams p = attn_params(a, 7, AT_SINGLE);
   AttnWork w;
-  attn_work(a.tokens, p.slots, a.heads, a.kv_heads, work, &w);
+  attn_work(a, split, work, &w);
   T *tq = static_cast<T*>(dq), *tk = static_cast<T*>(dk), *tv = static_cast<T*>(dv);
   NF4B_CUDA_TRY(launch_pdl(attn_prep_kernel<T>, dim3(unsigned(p.slots) * unsigned(a.heads)), dim3(AT_PREP_THREADS),
                            size_t(0), s, p, static_cast<const T*>(out), static_cast<const T*>(dout), lse,
                            static_cast<const T*>(a.v), a.v_stride, a.v_head_stride, w, tq, tk, tv));
-  const int split = attn_split(a);
-  const int64_t ctas = int64_t(p.slots) * (int64_t(a.kv_heads) * split + a.heads);
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned((ctas + split - 1) / split * split));
-  cfg.blockDim = dim3(AT_BWD_THREADS);
-  cfg.dynamicSmemBytes = AttnBwdSmem<DC>::ALLOC;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = unsigned(split);
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled(s) ? 2 : 1;
-  NF4B_CUDA_TRY(cudaLaunchKernelEx(&cfg, attn_bwd_kernel<T, DC>, m, p, w, split, tq, tk, tv));
+  const int64_t units = int64_t(p.slots) * (int64_t(a.kv_heads) * split + a.heads), sms = attn_sms();
+  NF4B_CUDA_TRY(launch_pdl(attn_bwd_kernel<T, DC>, dim3(unsigned(units < sms ? units : sms)), dim3(AT_BWD_THREADS),
+                           size_t(AttnBwdSmem<DC>::ALLOC), s, m, p, w, split, tq, tk, tv));
   return launch_status("attn_bwd_kernel launch");
 }
 
@@ -1097,16 +1186,15 @@ extern "C" int nf4b_attn_bwd(const nf4b_attn* args, const void* out, const float
   NF4B_RETURN_IF(!aligned(out, 16) || !aligned(lse, 16) || !aligned(dout, 16) || !aligned(dq, 16) || !aligned(dk, 16) ||
                      !aligned(dv, 16) || !aligned(work, 16),
                  NF4B_ERR_ALIGNMENT);
-  const int64_t need = nf4b_attn_bwd_work_bytes(a.tokens, a.rows, a.heads, a.kv_heads);
-  NF4B_RETURN_IF(need < 0, NF4B_ERR_UNSUPPORTED);
-  NF4B_RETURN_IF(work_bytes < need, NF4B_ERR_INVALID_ARG);
+  const int split = attn_split(a);
+  NF4B_RETURN_IF(work_bytes < attn_work(a, split, nullptr, nullptr), NF4B_ERR_INVALID_ARG);
   st = check_device();
   if (st != NF4B_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool wide = a.head_dim > 64;
   if (a.dtype == NF4B_F16)
-    return wide ? attn_bwd_launch<__half, 2>(a, out, lse, dout, dq, dk, dv, work, s)
-                : attn_bwd_launch<__half, 1>(a, out, lse, dout, dq, dk, dv, work, s);
-  return wide ? attn_bwd_launch<__nv_bfloat16, 2>(a, out, lse, dout, dq, dk, dv, work, s)
-              : attn_bwd_launch<__nv_bfloat16, 1>(a, out, lse, dout, dq, dk, dv, work, s);
+    return wide ? attn_bwd_launch<__half, 2>(a, out, lse, dout, dq, dk, dv, work, split, s)
+                : attn_bwd_launch<__half, 1>(a, out, lse, dout, dq, dk, dv, work, split, s);
+  return wide ? attn_bwd_launch<__nv_bfloat16, 2>(a, out, lse, dout, dq, dk, dv, work, split, s)
+              : attn_bwd_launch<__nv_bfloat16, 1>(a, out, lse, dout, dq, dk, dv, work, split, s);
 }

@@ -216,6 +216,7 @@ template <typename T, int MAX>
 __device__ __forceinline__ void at_store_rows(uint32_t taddr, uint8_t* buf, T* out, int64_t stride, int rows, int cols, float f) {
   const int lane = threadIdx.x & 31;
   constexpr int VEC = MAX / 8;  // 16-byte pieces of a row: 4, 8 or 16
+  __syncwarp();  // the rows before are out
   auto place = [&](int r, int c) { return buf + r * (2 * MAX) + (c ^ (VEC >= 8 ? r & 7 : (r >> 1) & 3)) * 16; };
 #pragma unroll
   for (int c = 0; c < MAX; c += 32) {

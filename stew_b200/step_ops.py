@@ -215,14 +215,14 @@ class _PackedAttention(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, cu, out, lse = ctx.saved_tensors
         dev, dt = q.device, q.dtype
-        n, hq, _ = q.shape
+        n = q.shape[0]
         dout = _aligned_c(dout if dout.dtype == dt else dout.to(dt))
         dq = torch.empty(q.shape, dtype=dt, device=dev)
         dk = torch.empty(k.shape, dtype=dt, device=dev)
         dv = torch.empty(v.shape, dtype=dt, device=dev)
         if n:
             L = _lib.lib()
-            wb = L.nf4b_attn_bwd_work_bytes(n, cu.numel() - 1, hq, k.shape[1])
+            wb = L.nf4b_attn_bwd_work_bytes(ctx.rec)
             work = torch.empty(wb, dtype=torch.uint8, device=dev)
             # the record's addresses are those of the saved tensors, which the graph keeps alive
             _launch(L.nf4b_attn_bwd, "nf4b_attn_bwd", dev, ctx.rec, out.data_ptr(), lse.data_ptr(), dout.data_ptr(),

@@ -45,9 +45,11 @@ def test_attention_entry_refuses_buffers():
     assert L.nf4b_attn_fwd(None, 256, 256, None) == _lib.NF4B_ERR_INVALID_ARG
     assert L.nf4b_attn_fwd(a, None, 256, None) == _lib.NF4B_ERR_INVALID_ARG
     assert L.nf4b_attn_fwd(a, 264, 256, None) == _lib.NF4B_ERR_ALIGNMENT
-    need = L.nf4b_attn_bwd_work_bytes(10, 1, 4, 2)
-    assert need >= 10 * 4 * 4
-    assert L.nf4b_attn_bwd_work_bytes(10, 1, 4, 3) == -1 and L.nf4b_attn_bwd_work_bytes(-1, 1, 4, 2) == -1
+    need = L.nf4b_attn_bwd_work_bytes(a)
+    assert need >= 10 * 4 * 8
+    for bad in (dict(kv_heads=3), dict(tokens=-1), dict(head_dim=60), dict(k_stride=4)):
+        assert L.nf4b_attn_bwd_work_bytes(ctypes.byref(_attn(**bad))) == -1
+    assert L.nf4b_attn_bwd_work_bytes(None) == -1
     assert L.nf4b_attn_bwd(a, 256, 256, 256, 256, 256, 256, 256, need - 1, None) == _lib.NF4B_ERR_INVALID_ARG
     assert L.nf4b_attn_bwd(a, 256, 256, 256, 256, 256, 256, None, need, None) == _lib.NF4B_ERR_INVALID_ARG
     assert L.nf4b_attn_bwd(a, 256, 256, 256, 256, 264, 256, 256, need, None) == _lib.NF4B_ERR_ALIGNMENT
