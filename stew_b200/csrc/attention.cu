@@ -336,7 +336,7 @@ struct AttnWork {
   float2* tile;   // [heads][slots]: max |dO_i|, max |delta_i| of a query tile
   float* vmax;    // [kv_heads][slots]: max |V_j| of a key tile
   unsigned* next;     // the next unit of work
-  unsigned* tickets;  // [slots][kv_heads]: shares of a key tile that are done
+  unsigned* tickets;  // [slots][kv_heads]: warps of a key tile's shares that are done
   float* parts;       // [slots][kv_heads][split]: their sums
 };
 
@@ -469,8 +469,8 @@ struct AttnBwdSmem {
   static constexpr int UNIT = AUX + 4 * AT_TILE * 4;  // [2] AttnUnit
   static constexpr int BAR = UNIT + 2 * 64;
   // a_full[2], a_empty[2], b_full[2], b_empty[2], aux_full[2], aux_empty[2], unit_full[2], unit_empty[2], xy_full,
-  // xy_empty, s_full, p_ready, dp_full, ds_ready, acc_full, acc_empty, joined, ticketed, drained
-  static constexpr int NBAR = 27;
+  // xy_empty, s_full, p_ready, dp_full, ds_ready, acc_full, acc_empty, drained
+  static constexpr int NBAR = 25;
   static constexpr int MISC = BAR + NBAR * 8;
   static constexpr int ALLOC = MISC + 16 + 1024;  // slack to align the base to 1024 B
 };
@@ -483,11 +483,13 @@ struct AttnBwdMaps {
   CUtensorMap q, k, v, dout;
 };
 
-// One unit of work: a key tile and a share of its group's heads, or a query tile and a head.
-enum { AT_UNIT_QUERIES = 0, AT_UNIT_KEYS = 1, AT_UNIT_END = 2 };
+// One unit of work: a key tile and a share of its group's heads, a query tile and a head, or a piece of the
+// sum over a key tile's shares.
+enum { AT_UNIT_QUERIES = 0, AT_UNIT_KEYS = 1, AT_UNIT_JOIN = 2, AT_UNIT_END = 3 };
+constexpr int AT_PIECES = 8;  // pieces of that sum
 struct AttnUnit {
   int kind, a, len, i0;  // the resident tile: tokens a + [i0, i0 + 128) of a sequence of len
-  int h, hk, rank;       // head of X and Y; key/value head; rank among the CTAs that share a key tile
+  int h, hk, rank;       // head of X and Y; key/value head; the share of a key tile, or the piece of a sum
   int yt0, nt, n;        // the ring's first tile, its tiles per head, ring items
   int h0;                // first query head of a key tile's share
   int k_exp;             // dS is scaled by 2^k_exp
@@ -495,15 +497,17 @@ struct AttnUnit {
 };
 static_assert(sizeof(AttnUnit) <= 64, "one slot of the unit ring");
 
-// Adds up the key tile's sums over the CTAs that share it: float4 groups of four features of [dK | dV] by rows.
+// A share's sums: groups of four features of [dK | dV], by rows.
 template <int DC>
 __device__ __forceinline__ float4* at_part(float* parts, int join, int split, int rank) {
   return reinterpret_cast<float4*>(parts) + (int64_t(join) * split + rank) * (DC * 32) * AT_TILE;
 }
 
 // Persistent: every CTA takes units from a counter, the longest kind first (key tiles with a group's heads;
-// of a causal sequence the first key tiles, which the most queries see, and the last query tiles), so that
-// the next unit's tiles are on their way and its first scores done while this unit's sums are stored.
+// of a causal sequence the first key tiles, which the most queries see, and the last query tiles; then the
+// sums over shares), so that the next unit's tiles are on their way and its first scores done while this
+// unit's sums are stored.  A sum waits for its shares; they come before it in the order, so each is in the
+// hands of a CTA that runs and does not wait.
 template <typename T, int DC>
 __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
     attn_bwd_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_constant__ AttnParams p, const AttnWork w,
@@ -528,15 +532,12 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
   uint64_t* ds_ready = dp_full + 1;
   uint64_t* acc_full = ds_ready + 1;
   uint64_t* acc_empty = acc_full + 1;
-  uint64_t* joined = acc_empty + 1;
-  uint64_t* ticketed = joined + 1;
-  uint64_t* drained = ticketed + 1;
+  uint64_t* drained = acc_empty + 1;
   float* aux_lse = reinterpret_cast<float*>(smem + L::AUX);
   float* aux_dl = aux_lse + 2 * AT_TILE;
   AttnUnit* units = reinterpret_cast<AttnUnit*>(smem + L::UNIT);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC + 4);
-  volatile int* ticket = reinterpret_cast<volatile int*>(smem + L::MISC + 8);
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int grp = p.heads / p.kv_heads;
 
@@ -559,8 +560,6 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
     mbar_init(ds_ready, 256);
     mbar_init(acc_full, 1);
     mbar_init(acc_empty, 256);
-    mbar_init(joined, 256);
-    mbar_init(ticketed, 1);
     mbar_init(drained, 1);
     fence_barrier_init();
     *abort_flag = 0;
@@ -590,42 +589,52 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
   if (warp == 8) {
     // ---------------------------------------------------------------- units and TMA
     const unsigned n_keys = unsigned(p.slots) * unsigned(p.kv_heads) * unsigned(split);
-    const unsigned n_all = n_keys + unsigned(p.slots) * unsigned(p.heads);
+    const unsigned n_main = n_keys + unsigned(p.slots) * unsigned(p.heads);
+    const unsigned n_all = n_main + (split > 1 ? unsigned(p.slots) * unsigned(p.kv_heads) * AT_PIECES : 0u);
     unsigned loads = 0, aux = 0;  // ring items so far
-    int k = 0;                    // units so far
+    int k = 0, tiles = 0;         // units so far; those of them with tiles
     for (;; ++k) {
-      // the next unit that is not empty
+      // the next unit that is not empty; the first is the CTA's number
       AttnUnit u;
       u.kind = AT_UNIT_END;
       int slot = 0;
-      for (;;) {
-        unsigned at = 0;
-        if (lane == 0) at = atomicAdd(w.next, 1u);
-        at = __shfl_sync(0xffffffffu, at, 0);
+      for (bool start = k == 0;; start = false) {
+        unsigned at = blockIdx.x;
+        if (!start) {
+          if (lane == 0) at = gridDim.x + atomicAdd(w.next, 1u);
+          at = __shfl_sync(0xffffffffu, at, 0);
+        }
         if (at >= n_all) break;
-        const bool keys = at < n_keys;
-        int h;
-        if (keys) {
+        if (at < n_keys) {
+          u.kind = AT_UNIT_KEYS;
           u.rank = int(at % unsigned(split));
-          const unsigned b = at / unsigned(split);
-          u.join = int(b);
-          slot = int(b / unsigned(p.kv_heads));
-          h = int(b % unsigned(p.kv_heads));
-        } else {
-          u.rank = 0;
-          u.join = 0;
+          u.join = int(at / unsigned(split));
+        } else if (at < n_main) {
+          u.kind = AT_UNIT_QUERIES;
+          u.rank = u.join = 0;
           slot = p.slots - 1 - int((at - n_keys) / unsigned(p.heads));
-          h = int((at - n_keys) % unsigned(p.heads));
+          u.h = int((at - n_keys) % unsigned(p.heads));
+          u.hk = u.h / grp;
+          u.h0 = 0;
+        } else {
+          u.kind = AT_UNIT_JOIN;
+          u.rank = int((at - n_main) % AT_PIECES);
+          u.join = int((at - n_main) / AT_PIECES);
+        }
+        if (u.kind != AT_UNIT_QUERIES) {
+          slot = int(unsigned(u.join) / unsigned(p.kv_heads));
+          u.h = u.hk = int(unsigned(u.join) % unsigned(p.kv_heads));
+          u.h0 = u.h * grp + u.rank * (grp / split);
         }
         const AttnTile t = at_find(p, slot);
-        if (t.tail || t.i0 >= t.len) continue;  // rows behind the last sequence: the prep launch's
-        u.kind = keys ? AT_UNIT_KEYS : AT_UNIT_QUERIES;
+        if (t.tail || t.i0 >= t.len) {  // rows behind the last sequence: the prep launch's
+          u.kind = AT_UNIT_END;
+          continue;
+        }
         u.a = t.a;
         u.len = t.len;
         u.i0 = t.i0;
-        u.h = h;
-        u.hk = keys ? h : h / grp;
-        u.h0 = keys ? h * grp + u.rank * (grp / split) : 0;
+        const bool keys = u.kind == AT_UNIT_KEYS;
         const int back = keys ? p.right : p.left, ahead = keys ? p.left : p.right;  // the window seen from X's side
         const int last = min(t.i0 + AT_TILE, t.len) - 1;
         const int lo = back < 0 ? 0 : max(0, t.i0 - back), hi = ahead < 0 ? t.len - 1 : min(t.len - 1, last + ahead);
@@ -634,23 +643,39 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
         u.n = keys ? u.nt * (grp / split) : u.nt;
         break;
       }
-      const bool keys = u.kind == AT_UNIT_KEYS;
+      const bool keys = u.kind == AT_UNIT_KEYS, main = keys || u.kind == AT_UNIT_QUERIES;
       u.k_exp = 0;
-      if (at_p_shift<T>() != 0.f && u.kind != AT_UNIT_END) u.k_exp = at_ds_exponent(p, w, slot, u.i0, u.len, u.hk);
+      if (main) {
+        if (!wait(xy_empty, (tiles & 1) ^ 1, 9)) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(xy_full, 2 * L::TILE);
+          for (int c = 0; c < DC; ++c) {
+            tma_load_3d(sbase + L::X + c * AT_BOX, keys ? &maps.k : &maps.q, xy_full, c * 64, u.h, u.a + u.i0);
+            tma_load_3d(sbase + L::Y + c * AT_BOX, keys ? &maps.v : &maps.dout, xy_full, c * 64, u.h, u.a + u.i0);
+          }
+        }
+        ++tiles;
+        if (at_p_shift<T>() != 0.f) u.k_exp = at_ds_exponent(p, w, slot, u.i0, u.len, u.hk);
+      } else if (u.kind == AT_UNIT_JOIN) {
+        const long long t0 = clock64();
+        const volatile unsigned* done = w.tickets + u.join;
+        while (ok && *done < 8u * unsigned(split)) {  // every elementwise warp of every share
+          if (*abort_flag || clock64() - t0 > kAttnWaitCycles) {
+            *abort_flag = 1;
+            atomicExch(&g_attn_error, 27);
+            ok = false;
+          }
+        }
+        __threadfence();
+        ok = __all_sync(0xffffffffu, ok);
+      }
       if (!wait(&unit_empty[k & 1], ((k >> 1) & 1) ^ 1, 10)) break;
       if (lane == 0) {
         units[k & 1] = u;
         mbar_arrive(&unit_full[k & 1]);
       }
       if (u.kind == AT_UNIT_END) break;
-      if (!wait(xy_empty, (k & 1) ^ 1, 9)) break;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(xy_full, 2 * L::TILE);
-        for (int c = 0; c < DC; ++c) {
-          tma_load_3d(sbase + L::X + c * AT_BOX, keys ? &maps.k : &maps.q, xy_full, c * 64, u.h, u.a + u.i0);
-          tma_load_3d(sbase + L::Y + c * AT_BOX, keys ? &maps.v : &maps.dout, xy_full, c * 64, u.h, u.a + u.i0);
-        }
-      }
+      if (!main) continue;
       const float sc = at_pow2(u.k_exp - int(at_p_shift<T>()));
       for (int it = 0; it < u.n; ++it) {
         const int s = loads & 1;
@@ -685,14 +710,11 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
           ++aux;
         }
       }
-      if (!ok) {
-        ++k;
-        break;
-      }
+      if (!ok) break;
     }
     // an abandoned CTA's loads must have landed before its shared memory goes
     if (!ok && lane == 0) {
-      if (k > 0) at_drain(xy_full, (k - 1) & 1);
+      if (tiles > 0) at_drain(xy_full, (tiles - 1) & 1);
       for (unsigned i = loads > 2 ? loads - 2 : 0; i < loads; ++i) {
         at_drain(&a_full[i & 1], (i >> 1) & 1);
         at_drain(&b_full[i & 1], (i >> 1) & 1);
@@ -723,7 +745,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
       for (int k = 0; k < AT_TILE / 16; ++k)
         at_mma_ts(lead, d, pm + (k >> 2) * 64 + (k & 3) * 8, b + uint64_t(k * (2048 >> 4)), id_g, acc || k > 0);
     };
-    unsigned r = 0;  // ring items so far
+    unsigned r = 0, m = 0;  // ring items and units with tiles so far
     // S and dP of ring item i, overwriting P and dS of the one before: MMAs of one thread run in order
     auto s_of = [&](unsigned i) {
       if (!wait(&a_full[i & 1], (i >> 1) & 1, 16)) return false;
@@ -746,14 +768,15 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&unit_empty[k & 1]);
       if (kind == AT_UNIT_END) break;
+      if (kind == AT_UNIT_JOIN) continue;
       const bool keys = kind == AT_UNIT_KEYS;
-      if (!wait(xy_full, k & 1, 18) || !s_of(r) || !dp_of(r, keys)) break;
+      if (!wait(xy_full, m & 1, 18) || !s_of(r) || !dp_of(r, keys)) break;
       if (n == 1) at_commit(lead, xy_empty);
       for (int it = 0; it < n; ++it, ++r) {
         const bool more = it + 1 < n;
         if (!wait(p_ready, r & 1, 19)) break;
         // the sums of the unit before have been read
-        if (it == 0 && !wait(acc_empty, (k & 1) ^ 1, 20)) break;
+        if (it == 0 && !wait(acc_empty, (m & 1) ^ 1, 20)) break;
         tc_fence_after();
         if (keys) {
           sum(tmem + AT_TM_DV, tmem + AT_TM_S, tb + (r & 1) * STEP, it > 0);
@@ -769,6 +792,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
       }
       if (!ok) break;
       at_commit(lead, acc_full);
+      ++m;
     }
     if (!ok) {  // nothing in flight when TMEM and shared memory go
       at_commit(lead, drained);
@@ -783,8 +807,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
     const float sl2 = p.scale * AT_LOG2E;
     const uint64_t sl2x2 = f2_pack(sl2, sl2);
     uint8_t* buf = smem + L::OUT + warp * 2048;
-    unsigned r = 0, aux = 0;
-    int joins = 0;
+    unsigned r = 0, aux = 0, m = 0;
     // One unit's ring items.
     auto items = [&](auto keys_tag, const AttnUnit& u) {
       constexpr bool KEYS = decltype(keys_tag)::value;
@@ -876,7 +899,8 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
           pv[2 * c] = f2_mul(pv[2 * c], f2_fma(f2_pack_u(dpv[4 * c], dpv[4 * c + 1]), scx2, d4.x));
           pv[2 * c + 1] = f2_mul(pv[2 * c + 1], f2_fma(f2_pack_u(dpv[4 * c + 2], dpv[4 * c + 3]), scx2, d4.y));
         }
-        if (cut) hide();
+        // (inside the sequence p = 0 has done it)
+        if (y0 + 64 > u.len) hide();
         put(t_dp);
         mbar_arrive(ds_ready);
         if (KEYS) {
@@ -891,10 +915,39 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&unit_empty[k & 1]);
       if (u.kind == AT_UNIT_END) break;
+      if (u.kind == AT_UNIT_JOIN) {
+        // piece u.rank of the features of [dK | dV], share by share; thread: a row, half of the piece
+        constexpr int N = DC * 32 / AT_PIECES / 2;  // groups of four features
+        const int jr = threadIdx.x & (AT_TILE - 1), g0 = (u.rank * 2 + (threadIdx.x >> 7)) * N;
+        const float4* from = at_part<DC>(w.parts, u.join, split, 0) + g0 * AT_TILE + jr;
+        const int f0 = g0 * 4 & (DC * 64 - 1);
+        if (jr < u.len - u.i0 && f0 < p.head_dim) {
+          float4 v[N];
+#pragma unroll
+          for (int e = 0; e < N; ++e) v[e] = __ldcg(from + e * AT_TILE);
+#pragma unroll 4
+          for (int q = 1; q < split; ++q) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+              const float4 y = __ldcg(from + (int64_t(q) * (DC * 32) + e) * AT_TILE);
+              v[e].x += y.x, v[e].y += y.y, v[e].z += y.z, v[e].w += y.w;
+            }
+          }
+          T* to = (g0 < DC * 16 ? dk : dv) + (int64_t(u.a + u.i0 + jr) * p.kv_heads + u.h) * p.head_dim + f0;
+#pragma unroll
+          for (int e = 0; e < N; e += 2)
+            if (f0 + e * 4 < p.head_dim)
+              *reinterpret_cast<uint4*>(to + e * 4) =
+                  make_uint4(at_pack<T>(v[e].x, v[e].y), at_pack<T>(v[e].z, v[e].w), at_pack<T>(v[e + 1].x, v[e + 1].y),
+                             at_pack<T>(v[e + 1].z, v[e + 1].w));
+        }
+        continue;
+      }
       const bool keys = u.kind == AT_UNIT_KEYS;
       if (keys) items(std::true_type{}, u);
       else items(std::false_type{}, u);
-      if (!ok || !wait(acc_full, k & 1, 26)) break;
+      if (!ok || !wait(acc_full, m & 1, 26)) break;
+      ++m;
       tc_fence_after();
       const int rows = u.len - u.i0 - w0;  // of this warp's 32
       const float fx = p.scale * at_pow2(-u.k_exp);
@@ -908,16 +961,14 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
       } else {
         const uint32_t from = tmem + (half == 0 ? AT_TM_DX : AT_TM_DV) + lane_off;
         const float f = half == 0 ? fx : at_pow2(-int(at_p_shift<T>()));
-        T* to = (half == 0 ? dk : dv) + (int64_t(u.a + u.i0 + w0) * p.kv_heads + u.h) * p.head_dim;
-        const int64_t pitch = int64_t(p.kv_heads) * p.head_dim;
         if (split == 1) {
+          T* to = (half == 0 ? dk : dv) + (int64_t(u.a + u.i0 + w0) * p.kv_heads + u.h) * p.head_dim;
 #pragma unroll
           for (int c = 0; c < DC * 64; c += 32)
-            at_store_rows<T, 32>(from + c, buf, to + c, pitch, rows, p.head_dim - c, f);
-        } else {
-          // this share's sums to memory; whoever comes last adds all of them up, share by share
+            at_store_rows<T, 32>(from + c, buf, to + c, int64_t(p.kv_heads) * p.head_dim, rows, p.head_dim - c, f);
+        } else if (rows > 0) {
           float4* mine = at_part<DC>(w.parts, u.join, split, u.rank) + half * DC * 16 * AT_TILE + row;
-#pragma unroll 1
+#pragma unroll
           for (int c = 0; c < DC * 64; c += 32) {
             uint32_t o[32];
             tmem_ld_32x32b_x32(from + c, o);
@@ -927,43 +978,15 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
               mine[(c + e) / 4 * AT_TILE] = make_float4(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f,
                                                         __uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f);
           }
-          __threadfence();
-          mbar_arrive(joined);
-          if (!wait(joined, joins & 1, 27)) break;
-          if (threadIdx.x == 0) {
-            *ticket = int(atomicAdd(w.tickets + u.join, 1u));
-            __threadfence();
-            mbar_arrive(ticketed);
-          }
-          if (!wait(ticketed, joins & 1, 28)) break;
-          ++joins;
-          if (*ticket == split - 1) {
-            const float4* all = at_part<DC>(w.parts, u.join, split, 0) + half * DC * 16 * AT_TILE + row;
-#pragma unroll 1
-            for (int c = 0; c < DC * 64; c += 32) {
-              float4 v[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] = __ldcg(all + (c / 4 + e) * AT_TILE);
-#pragma unroll 1
-              for (int q = 1; q < split; ++q) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  const float4 y = __ldcg(all + int64_t(q) * (DC * 32) * AT_TILE + (c / 4 + e) * AT_TILE);
-                  v[e].x += y.x, v[e].y += y.y, v[e].z += y.z, v[e].w += y.w;
-                }
-              }
-#pragma unroll
-              for (int e = 0; e < 8; e += 2)
-                if (lane < rows && c + e * 4 < p.head_dim)
-                  *reinterpret_cast<uint4*>(to + lane * pitch + c + e * 4) =
-                      make_uint4(at_pack<T>(v[e].x, v[e].y), at_pack<T>(v[e].z, v[e].w), at_pack<T>(v[e + 1].x, v[e + 1].y),
-                                 at_pack<T>(v[e + 1].z, v[e + 1].w));
-            }
-          }
         }
       }
       tc_fence_before();
       mbar_arrive(acc_empty);
+      if (keys && split > 1) {  // this warp's part of the share is in memory
+        __threadfence();
+        __syncwarp();
+        if (lane == 0) atomicAdd(w.tickets + u.join, 1u);
+      }
     }
     tc_fence_before();
   }
@@ -989,7 +1012,7 @@ static int attn_checks(const nf4b_attn* in, nf4b_attn* a) {
   NF4B_RETURN_IF(a->head_dim % 8 != 0 || a->head_dim > AT_MAX_DIM, NF4B_ERR_UNSUPPORTED);
   NF4B_RETURN_IF(a->tokens > 0x3FFFFFFF || a->rows > 0x3FFFFFFF || a->heads > 65535, NF4B_ERR_UNSUPPORTED);
   // CTAs of a launch
-  NF4B_RETURN_IF(at_slots(a->tokens, a->rows, 7) * 2 * a->heads + 8 > 0x7FFFFFFF, NF4B_ERR_UNSUPPORTED);
+  NF4B_RETURN_IF(at_slots(a->tokens, a->rows, 7) * (2 + AT_PIECES) * a->heads > 0x3FFFFFFF, NF4B_ERR_UNSUPPORTED);
   if (a->tokens == 0) return NF4B_OK;
   NF4B_RETURN_IF(!a->q || !a->k || !a->v || !a->cu, NF4B_ERR_INVALID_ARG);
   NF4B_RETURN_IF(!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->cu, 4), NF4B_ERR_ALIGNMENT);
@@ -1097,7 +1120,7 @@ static int attn_sms() {
 
 // CTAs that share a key tile's heads: the divisor of the group with the shortest estimated time on 148 SMs,
 // from an average sequence: the longer of all units' work shared out and the longest key-tile unit.  In
-// microseconds, as measured: about 3 of start and store for a unit, 3 more for a shared one, 1.6 a key-tile
+// microseconds, as measured: about 3 of start and store for a unit, 2 more for a shared one, 1.6 a key-tile
 // step, 1.2 a query-tile step.
 static int attn_split(const nf4b_attn& a) {
   const int grp = a.heads / a.kv_heads;
@@ -1111,7 +1134,7 @@ static int attn_split(const nf4b_attn& a) {
   for (int c = 1; c <= grp; ++c) {
     // (the shares' sums: 1 KB a key row, share and 128 features)
     if (grp % c != 0 || (c > 1 && double(at_slots(a.tokens, a.rows, 7)) * a.kv_heads * c > 4096)) continue;
-    const double one = 3.0 + (c > 1 ? 3.0 : 0.0);
+    const double one = 3.0 + (c > 1 ? 2.0 : 0.0);
     const double keys = tiles * a.kv_heads * c * (one + 1.6 * mean * (grp / c));
     const double queries = tiles * a.heads * (3.0 + 1.2 * mean);
     const double all = (keys + queries) / 148, longest = one + 1.6 * most * (grp / c);
@@ -1170,7 +1193,8 @@ static int attn_bwd_launch(const nf4b_attn& a, const void* out, const float* lse
   NF4B_CUDA_TRY(launch_pdl(attn_prep_kernel<T>, dim3(unsigned(p.slots) * unsigned(a.heads)), dim3(AT_PREP_THREADS),
                            size_t(0), s, p, static_cast<const T*>(out), static_cast<const T*>(dout), lse,
                            static_cast<const T*>(a.v), a.v_stride, a.v_head_stride, w, tq, tk, tv));
-  const int64_t units = int64_t(p.slots) * (int64_t(a.kv_heads) * split + a.heads), sms = attn_sms();
+  const int64_t units = int64_t(p.slots) * (int64_t(a.kv_heads) * (split > 1 ? split + AT_PIECES : 1) + a.heads);
+  const int64_t sms = attn_sms();
   NF4B_CUDA_TRY(launch_pdl(attn_bwd_kernel<T, DC>, dim3(unsigned(units < sms ? units : sms)), dim3(AT_BWD_THREADS),
                            size_t(AttnBwdSmem<DC>::ALLOC), s, m, p, w, split, tq, tk, tv));
   return launch_status("attn_bwd_kernel launch");
