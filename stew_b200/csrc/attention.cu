@@ -188,12 +188,14 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1)
       const int sv = (2 * i + 1) % L::RING;
       if (!arrived(2 * i + 1) || (i + 2 < nt && !arrived(2 * i + 4))) break;
       const uint64_t dv = dv0 + uint64_t(sv * (L::TILE >> 4));
+      const int j0 = (jt0 + i) * AT_KEYS;
       for (int g = 0; g <= both; ++g) {
         if (!wait(&p_ready[2 * g + (i & 1)], (i >> 1) & 1, 6)) break;
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < AT_KEYS / 16; ++k)
-          at_mma_ts(lead, tmem + (2 + g) * AT_TILE, tmem + g * AT_TILE + (i & 1) * AT_KEYS + k * 8,
+          if (j0 + k * 16 < t.len)  // nothing behind the sequence's end
+            at_mma_ts(lead, tmem + (2 + g) * AT_TILE, tmem + g * AT_TILE + (i & 1) * AT_KEYS + k * 8,
                     dv + uint64_t(k * (2048 >> 4)), id_o, i > 0 || k > 0);
         at_commit(lead, &o_done[g]);
         if (i + 1 == nt) {
@@ -221,6 +223,8 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1)
     const uint64_t sl2x2 = f2_pack(sl2, sl2);
     const int see_lo = p.left < 0 ? 0 : i - p.left;
     const int see_hi = p.right < 0 ? t.len - 1 : min(t.len - 1, i + p.right);
+    const int lo_max = p.left < 0 ? 0 : i0 + w0 + 31 - p.left;  // what all rows of the warp see
+    const int hi_min = p.right < 0 ? t.len - 1 : min(t.len - 1, i0 + w0 + p.right);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int it = 0; it < nt; ++it) {
@@ -232,13 +236,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1)
 #pragma unroll
       for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(t_s + b * AT_KEYS + c * 32, s[c]);
       tmem_ld_wait();
-      // tiles that the window or the sequence's end cuts (the same for the whole query tile)
-      if (j0 + AT_KEYS > t.len || (p.right >= 0 && j0 + AT_KEYS - 1 > i0 + p.right) ||
-          (p.left >= 0 && j0 < i0 + AT_TILE - 1 - p.left)) {
-#pragma unroll
-        for (int c = 0; c < AT_KEYS; ++c)
-          if (j0 + c < see_lo || j0 + c > see_hi) s[c >> 5][c & 31] = 0xff800000u;  // -inf
-      }
+      at_hide<4>(j0, see_lo, see_hi, lo_max, hi_min, [&](int c) { s[c >> 5][c & 31] = 0xff800000u; });  // -inf
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int c = 0; c < AT_KEYS; c += 2)
@@ -283,6 +281,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1)
         ok = at_wait(&full[x % L::RING], (x / L::RING) & 1, abort_flag, 2);
         if (!__all_sync(0xffffffffu, ok)) break;
         at_zero_rows<DC, AT_KEYS, 128>(smem + L::KV + (x % L::RING) * L::TILE, t.len - j0, threadIdx.x & 127);
+        fence_proxy_async_smem();
       }
       tmem_st_wait();
       tc_fence_before();
@@ -366,55 +365,73 @@ __global__ void __launch_bounds__(AT_PREP_THREADS)
   const int sub = threadIdx.x & 15, f = sub * 8;  // this thread's 8 features
   const bool in = f < p.head_dim;
   float m_do = 0.f, m_dl = 0.f, m_v = 0.f;
-  for (int r0 = 0; r0 < AT_TILE; r0 += AT_PREP_THREADS / 16) {
-    const int r = r0 + (threadIdx.x >> 4);
-    const bool live = r < n && in;
-    const int64_t row = t.a + t.i0 + r;
-    const int64_t off = (row * p.heads + h) * p.head_dim + f, koff = (row * p.kv_heads + hk) * p.head_dim + f;
-    if (t.tail) {
-      if (live) {
-        *reinterpret_cast<uint4*>(dq + off) = make_uint4(0, 0, 0, 0);
-        if (first) {
-          *reinterpret_cast<uint4*>(dk + koff) = make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(dv + koff) = make_uint4(0, 0, 0, 0);
-        }
+  const int r0 = threadIdx.x >> 4;
+  constexpr int STEP = AT_PREP_THREADS / 16, N = AT_TILE / STEP;  // rows a thread works on: r0 + k STEP
+  const int64_t row0 = t.a + t.i0 + r0;
+  if (t.tail) {
+    for (int k = 0; k < N; ++k) {
+      const int64_t row = row0 + k * STEP;
+      if (r0 + k * STEP >= n || !in) continue;
+      *reinterpret_cast<uint4*>(dq + (row * p.heads + h) * p.head_dim + f) = make_uint4(0, 0, 0, 0);
+      if (first) {
+        *reinterpret_cast<uint4*>(dk + (row * p.kv_heads + hk) * p.head_dim + f) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(dv + (row * p.kv_heads + hk) * p.head_dim + f) = make_uint4(0, 0, 0, 0);
       }
-      continue;
     }
-    float dot = 0.f, nd = 0.f, nv = 0.f;
-    if (live) {
-      const uint4 o4 = *reinterpret_cast<const uint4*>(out + off), d4 = *reinterpret_cast<const uint4*>(dout + off);
-      const uint32_t* o = reinterpret_cast<const uint32_t*>(&o4);
-      const uint32_t* d = reinterpret_cast<const uint32_t*>(&d4);
+    return;
+  }
+  uint4 o4[N], d4[N];  // every load under way before the first sum
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 a = at_unpack<T>(o[i]), b = at_unpack<T>(d[i]);
-        dot = fmaf(a.x, b.x, fmaf(a.y, b.y, dot));
-        nd = fmaf(b.x, b.x, fmaf(b.y, b.y, nd));
-      }
-      if (first && at_p_shift<T>() != 0.f) {
-        const uint4 v4 = *reinterpret_cast<const uint4*>(v + row * v_stride + hk * v_head_stride + f);
-        const uint32_t* x = reinterpret_cast<const uint32_t*>(&v4);
+  for (int k = 0; k < N; ++k) {
+    const bool live = r0 + k * STEP < n && in;
+    const int64_t off = ((row0 + k * STEP) * p.heads + h) * p.head_dim + f;
+    o4[k] = live ? *reinterpret_cast<const uint4*>(out + off) : make_uint4(0, 0, 0, 0);
+    d4[k] = live ? *reinterpret_cast<const uint4*>(dout + off) : make_uint4(0, 0, 0, 0);
+  }
+  constexpr bool SCALED = at_p_shift<T>() != 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 a = at_unpack<T>(x[i]);
-          nv = fmaf(a.x, a.x, fmaf(a.y, a.y, nv));
-        }
-      }
+  for (int k = 0; k < N; ++k) {
+    const uint32_t* o = reinterpret_cast<const uint32_t*>(&o4[k]);
+    const uint32_t* d = reinterpret_cast<const uint32_t*>(&d4[k]);
+    float dot = 0.f, nd = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 a = at_unpack<T>(o[i]), b = at_unpack<T>(d[i]);
+      dot = fmaf(a.x, b.x, fmaf(a.y, b.y, dot));
+      nd = fmaf(b.x, b.x, fmaf(b.y, b.y, nd));
     }
     dot = at_half_warp_sum(dot);
-    if (r < n && sub == 0) {
-      const float l = lse[int64_t(h) * p.tokens + row];
+    if (r0 + k * STEP < n && sub == 0) {
+      const int64_t at = int64_t(h) * p.tokens + row0 + k * STEP;
+      const float l = lse[at];
       // a row without weight (lse = -inf) must give p = 0
-      w.row[int64_t(h) * p.tokens + row] = make_float2(l == -INFINITY ? INFINITY : l * AT_LOG2E, dot);
+      w.row[at] = make_float2(l == -INFINITY ? INFINITY : l * AT_LOG2E, dot);
     }
-    if (at_p_shift<T>() != 0.f) {
+    if (SCALED) {
       m_do = fmaxf(m_do, at_half_warp_sum(nd));
       m_dl = fmaxf(m_dl, fabsf(dot));
+    }
+  }
+  if (SCALED && first) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const bool live = r0 + k * STEP < n && in;
+      o4[k] = live ? *reinterpret_cast<const uint4*>(v + (row0 + k * STEP) * v_stride + hk * v_head_stride + f)
+                   : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const uint32_t* x = reinterpret_cast<const uint32_t*>(&o4[k]);
+      float nv = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 a = at_unpack<T>(x[i]);
+        nv = fmaf(a.x, a.x, fmaf(a.y, a.y, nv));
+      }
       m_v = fmaxf(m_v, at_half_warp_sum(nv));
     }
   }
-  if (t.tail || at_p_shift<T>() == 0.f) return;
+  if (!SCALED) return;
   __shared__ float s_max[3][AT_PREP_THREADS / 16];
   if (sub == 0) {
     s_max[0][threadIdx.x >> 4] = m_do;
@@ -468,9 +485,9 @@ struct AttnBwdSmem {
   static constexpr int AUX = OUT + 8 * 2048;       // [2][128] -lse, [2][128] -delta (scaled)
   static constexpr int UNIT = AUX + 4 * AT_TILE * 4;  // [2] AttnUnit
   static constexpr int BAR = UNIT + 2 * 64;
-  // a_full[2], a_empty[2], b_full[2], b_empty[2], aux_full[2], aux_empty[2], unit_full[2], unit_empty[2], xy_full,
+  // a_full[2], a_empty[2], b_full[2], b_empty[2], aux_empty[2], unit_full[2], unit_empty[2], xy_full,
   // xy_empty, s_full, p_ready, dp_full, ds_ready, acc_full, acc_empty, drained
-  static constexpr int NBAR = 25;
+  static constexpr int NBAR = 23;
   static constexpr int MISC = BAR + NBAR * 8;
   static constexpr int ALLOC = MISC + 16 + 1024;  // slack to align the base to 1024 B
 };
@@ -520,8 +537,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
   uint64_t* a_empty = a_full + 2;
   uint64_t* b_full = a_empty + 2;
   uint64_t* b_empty = b_full + 2;
-  uint64_t* aux_full = b_empty + 2;
-  uint64_t* aux_empty = aux_full + 2;
+  uint64_t* aux_empty = b_empty + 2;
   uint64_t* unit_full = aux_empty + 2;
   uint64_t* unit_empty = unit_full + 2;
   uint64_t* xy_full = unit_empty + 2;
@@ -543,12 +559,11 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&a_full[i], 1);
+      mbar_init(&a_full[i], 2);  // the tile, and the producer once the rows' (lse, delta) are there
       mbar_init(&a_empty[i], 1);
       mbar_init(&b_full[i], 1);
       mbar_init(&b_empty[i], 1);
-      mbar_init(&aux_full[i], 32);
-      mbar_init(&aux_empty[i], 256);
+      mbar_init(&aux_empty[i], 8);
       mbar_init(&unit_full[i], 1);
       mbar_init(&unit_empty[i], 9);
     }
@@ -591,7 +606,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
     const unsigned n_keys = unsigned(p.slots) * unsigned(p.kv_heads) * unsigned(split);
     const unsigned n_main = n_keys + unsigned(p.slots) * unsigned(p.heads);
     const unsigned n_all = n_main + (split > 1 ? unsigned(p.slots) * unsigned(p.kv_heads) * AT_PIECES : 0u);
-    unsigned loads = 0, aux = 0;  // ring items so far
+    unsigned loads = 0, issued = 0, aux = 0;  // ring items so far, also those under way
     int k = 0, tiles = 0;         // units so far; those of them with tiles
     for (;; ++k) {
       // the next unit that is not empty; the first is the CTA's number
@@ -644,6 +659,22 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
         break;
       }
       const bool keys = u.kind == AT_UNIT_KEYS, main = keys || u.kind == AT_UNIT_QUERIES;
+      auto load = [&](int hy, int y0) {  // ring item `loads`
+        const int s = loads & 1;
+        const uint32_t ph = ((loads >> 1) & 1) ^ 1;
+        if (!wait(&a_empty[s], ph, 11) || !wait(&b_empty[s], ph, 12)) return false;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&a_full[s], L::TILE);
+          for (int c = 0; c < DC; ++c)
+            tma_load_3d(sbase + L::A + s * L::TILE + c * AT_BOX, keys ? &maps.q : &maps.k, &a_full[s], c * 64, hy, u.a + y0);
+          mbar_arrive_expect_tx(&b_full[s], L::TILE);
+          for (int c = 0; c < DC; ++c)
+            tma_load_3d(sbase + L::B + s * L::TILE + c * AT_BOX, keys ? &maps.dout : &maps.v, &b_full[s], c * 64, hy,
+                        u.a + y0);
+        }
+        issued = loads + 1;
+        return true;
+      };
       u.k_exp = 0;
       if (main) {
         if (!wait(xy_empty, (tiles & 1) ^ 1, 9)) break;
@@ -655,6 +686,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
           }
         }
         ++tiles;
+        if (!load(keys ? u.h0 : u.hk, u.yt0 * AT_TILE)) break;  // the ring's first tiles before anything else
         if (at_p_shift<T>() != 0.f) u.k_exp = at_ds_exponent(p, w, slot, u.i0, u.len, u.hk);
       } else if (u.kind == AT_UNIT_JOIN) {
         const long long t0 = clock64();
@@ -677,37 +709,29 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
       if (u.kind == AT_UNIT_END) break;
       if (!main) continue;
       const float sc = at_pow2(u.k_exp - int(at_p_shift<T>()));
-      for (int it = 0; it < u.n; ++it) {
-        const int s = loads & 1;
-        const uint32_t ph = ((loads >> 1) & 1) ^ 1;
-        const int hy = keys ? u.h0 + it / u.nt : u.hk;
-        const int y0 = (u.yt0 + (keys ? it % u.nt : it)) * AT_TILE;
-        if (!wait(&a_empty[s], ph, 11) || !wait(&b_empty[s], ph, 12)) break;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&a_full[s], L::TILE);
-          for (int c = 0; c < DC; ++c)
-            tma_load_3d(sbase + L::A + s * L::TILE + c * AT_BOX, keys ? &maps.q : &maps.k, &a_full[s], c * 64, hy, u.a + y0);
-          mbar_arrive_expect_tx(&b_full[s], L::TILE);
-          for (int c = 0; c < DC; ++c)
-            tma_load_3d(sbase + L::B + s * L::TILE + c * AT_BOX, keys ? &maps.dout : &maps.v, &b_full[s], c * 64, hy,
-                        u.a + y0);
-        }
-        ++loads;
+      int hy = keys ? u.h0 : u.hk, yt = 0;
+      for (int it = 0; it < u.n; ++it, ++loads) {
+        const int s = loads & 1, y0 = (u.yt0 + yt) * AT_TILE;
+        if (it > 0 && !load(hy, y0)) break;
         if (keys) {
           const float2* src = w.row + int64_t(hy) * p.tokens + u.a;
           float2 x[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e)  // p = 0 behind the end
             x[e] = y0 + e * 32 + lane < u.len ? src[y0 + e * 32 + lane] : make_float2(INFINITY, 0.f);
-          const int sa = aux & 1;
-          if (!wait(&aux_empty[sa], ((aux >> 1) & 1) ^ 1, 13)) break;
+          if (!wait(&aux_empty[aux & 1], ((aux >> 1) & 1) ^ 1, 13)) break;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            aux_lse[sa * AT_TILE + e * 32 + lane] = at_p_shift<T>() - x[e].x;
-            aux_dl[sa * AT_TILE + e * 32 + lane] = -x[e].y * sc;
+            aux_lse[(aux & 1) * AT_TILE + e * 32 + lane] = at_p_shift<T>() - x[e].x;
+            aux_dl[(aux & 1) * AT_TILE + e * 32 + lane] = -x[e].y * sc;
           }
-          mbar_arrive(&aux_full[sa]);
           ++aux;
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(&a_full[s]);
+        if (++yt == u.nt) {
+          yt = 0;
+          ++hy;
         }
       }
       if (!ok) break;
@@ -715,7 +739,8 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
     // an abandoned CTA's loads must have landed before its shared memory goes
     if (!ok && lane == 0) {
       if (tiles > 0) at_drain(xy_full, (tiles - 1) & 1);
-      for (unsigned i = loads > 2 ? loads - 2 : 0; i < loads; ++i) {
+      if (issued > loads) mbar_arrive(&a_full[loads & 1]);
+      for (unsigned i = issued > 2 ? issued - 2 : 0; i < issued; ++i) {
         at_drain(&a_full[i & 1], (i >> 1) & 1);
         at_drain(&b_full[i & 1], (i >> 1) & 1);
       }
@@ -724,71 +749,78 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
     // ---------------------------------------------------------------- MMA
     const uint32_t lead = elect_one();
     const int kd = (p.head_dim + 15) / 16;
-    const uint32_t id_s = at_idesc<T>(AT_TILE, false);
     const uint32_t id_g = at_idesc<T>(kd * 16, true);
     const uint64_t dx = smem_desc_sw128(sbase + L::X, 16, 1024), dy = smem_desc_sw128(sbase + L::Y, 16, 1024);
     const uint64_t da = smem_desc_sw128(sbase + L::A, 16, 1024), db = smem_desc_sw128(sbase + L::B, 16, 1024);
     const uint64_t ta = smem_desc_sw128(sbase + L::A, AT_BOX, 1024), tb = smem_desc_sw128(sbase + L::B, AT_BOX, 1024);
     constexpr uint64_t STEP = uint64_t(L::TILE >> 4);
-    // d (128 x 128) = x a^T over head_dim
-    auto scores = [&](uint32_t d, uint64_t x, uint64_t a) {
+    // d (128 x the ring tile's tokens) = x a^T over head_dim
+    auto scores = [&](uint32_t d, uint64_t x, uint64_t a, int steps) {
+      const uint32_t id = at_idesc<T>(steps * 16, false);
 #pragma unroll
       for (int k = 0; k < DC * 4; ++k) {
         const uint64_t off = uint64_t((k >> 2) * (AT_BOX >> 4) + (k & 3) * 2);
-        if (k < kd) at_mma_ss(lead, d, x + off, a + off, id_s, k > 0);
+        if (k < kd) at_mma_ss(lead, d, x + off, a + off, id, k > 0);
       }
     };
-    // d (128 x head_dim) += p b over the ring tile's 128 tokens; each half of the columns of p lies
+    // d (128 x head_dim) += p b over the ring tile's tokens; each half of the columns of p lies
     // at the start of its own half of the scores it overwrote
-    auto sum = [&](uint32_t d, uint32_t pm, uint64_t b, bool acc) {
+    auto sum = [&](uint32_t d, uint32_t pm, uint64_t b, bool acc, int steps) {
 #pragma unroll
       for (int k = 0; k < AT_TILE / 16; ++k)
-        at_mma_ts(lead, d, pm + (k >> 2) * 64 + (k & 3) * 8, b + uint64_t(k * (2048 >> 4)), id_g, acc || k > 0);
+        if (k < steps) at_mma_ts(lead, d, pm + (k >> 2) * 64 + (k & 3) * 8, b + uint64_t(k * (2048 >> 4)), id_g, acc || k > 0);
     };
     unsigned r = 0, m = 0;  // ring items and units with tiles so far
     // S and dP of ring item i, overwriting P and dS of the one before: MMAs of one thread run in order
-    auto s_of = [&](unsigned i) {
+    auto s_of = [&](unsigned i, int steps) {
       if (!wait(&a_full[i & 1], (i >> 1) & 1, 16)) return false;
       tc_fence_after();
-      scores(tmem + AT_TM_S, dx, da + (i & 1) * STEP);
+      scores(tmem + AT_TM_S, dx, da + (i & 1) * STEP, steps);
       at_commit(lead, s_full);
       return true;
     };
-    auto dp_of = [&](unsigned i, bool keys) {
+    auto dp_of = [&](unsigned i, bool keys, int steps) {
       if (!wait(&b_full[i & 1], (i >> 1) & 1, 17)) return false;
       tc_fence_after();
-      scores(tmem + AT_TM_DP, dy, db + (i & 1) * STEP);
+      scores(tmem + AT_TM_DP, dy, db + (i & 1) * STEP, steps);
       at_commit(lead, dp_full);
       if (!keys) at_commit(lead, &b_empty[i & 1]);
       return true;
     };
     for (int k = 0;; ++k) {
       if (!wait(&unit_full[k & 1], (k >> 1) & 1, 15)) break;
-      const int kind = __shfl_sync(0xffffffffu, units[k & 1].kind, 0), n = __shfl_sync(0xffffffffu, units[k & 1].n, 0);
+      auto of_unit = [&](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+      const int kind = of_unit(units[k & 1].kind), n = of_unit(units[k & 1].n), nt = of_unit(units[k & 1].nt);
+      const int tokens = of_unit(units[k & 1].len - units[k & 1].yt0 * AT_TILE);  // from the ring's first tile on
       __syncwarp();
       if (lane == 0) mbar_arrive(&unit_empty[k & 1]);
       if (kind == AT_UNIT_END) break;
       if (kind == AT_UNIT_JOIN) continue;
       const bool keys = kind == AT_UNIT_KEYS;
-      if (!wait(xy_full, m & 1, 18) || !s_of(r) || !dp_of(r, keys)) break;
+      // MMAs over 16 tokens each: nothing behind the sequence's end
+      int yt = 0, steps = (min(tokens, AT_TILE) + 15) >> 4;
+      if (!wait(xy_full, m & 1, 18) || !s_of(r, steps) || !dp_of(r, keys, steps)) break;
       if (n == 1) at_commit(lead, xy_empty);
       for (int it = 0; it < n; ++it, ++r) {
         const bool more = it + 1 < n;
+        if (++yt == nt) yt = 0;
+        const int next = (min(tokens - yt * AT_TILE, AT_TILE) + 15) >> 4;
         if (!wait(p_ready, r & 1, 19)) break;
         // the sums of the unit before have been read
         if (it == 0 && !wait(acc_empty, (m & 1) ^ 1, 20)) break;
         tc_fence_after();
         if (keys) {
-          sum(tmem + AT_TM_DV, tmem + AT_TM_S, tb + (r & 1) * STEP, it > 0);
+          sum(tmem + AT_TM_DV, tmem + AT_TM_S, tb + (r & 1) * STEP, it > 0, steps);
           at_commit(lead, &b_empty[r & 1]);
         }
-        if (more && !s_of(r + 1)) break;
+        if (more && !s_of(r + 1, next)) break;
         if (!wait(ds_ready, r & 1, 21)) break;
         tc_fence_after();
-        sum(tmem + AT_TM_DX, tmem + AT_TM_DP, ta + (r & 1) * STEP, it > 0);
+        sum(tmem + AT_TM_DX, tmem + AT_TM_DP, ta + (r & 1) * STEP, it > 0, steps);
         at_commit(lead, &a_empty[r & 1]);
-        if (more && !dp_of(r + 1, keys)) break;
+        if (more && !dp_of(r + 1, keys, next)) break;
         if (it + 2 == n) at_commit(lead, xy_empty);  // no more scores of this unit
+        steps = next;
       }
       if (!ok) break;
       at_commit(lead, acc_full);
@@ -815,32 +847,59 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
       const float sc = at_pow2(u.k_exp - int(at_p_shift<T>()));
       const uint64_t scx2 = f2_pack(sc, sc);
       const int back = KEYS ? p.right : p.left, ahead = KEYS ? p.left : p.right;
-      const int see_lo = back < 0 ? 0 : x - back;
+      const int see_lo = back < 0 ? 0 : x - back, x0 = u.i0 + w0;
       const int see_hi = ahead < 0 ? u.len - 1 : min(u.len - 1, x + ahead);
+      // what all, and what any of the warp's rows see
+      const int lo_max = back < 0 ? 0 : x0 + 31 - back, lo_min = back < 0 ? 0 : x0 - back;
+      const int hi_min = ahead < 0 ? u.len - 1 : min(u.len - 1, x0 + ahead);
+      const int hi_max = ahead < 0 ? u.len - 1 : min(u.len - 1, x0 + 31 + ahead);
       uint64_t row_lse = 0, row_dl = 0;  // twice each
       if (!KEYS) {
         const float2 v = x < u.len ? w.row[int64_t(u.h) * p.tokens + u.a + x] : make_float2(INFINITY, 0.f);
         row_lse = f2_pack(at_p_shift<T>() - v.x, at_p_shift<T>() - v.x);
         row_dl = f2_pack(-v.y * sc, -v.y * sc);
       }
+      int yt = 0;
       for (int it = 0; it < u.n; ++it, ++r) {
         const int s = r & 1, sa = aux & 1;
-        const int y0 = (u.yt0 + (KEYS ? it % u.nt : it)) * AT_TILE + half * 64;
+        const int tile0 = (u.yt0 + yt) * AT_TILE, y0 = tile0 + half * 64;
+        if (++yt == u.nt) yt = 0;
         if (!wait(s_full, r & 1, 22)) return;
-        if (KEYS && !wait(&aux_full[sa], (aux >> 1) & 1, 23)) return;
         tc_fence_after();
-        const bool cut = y0 + 64 > u.len || (ahead >= 0 && y0 + 63 > u.i0 + ahead) ||
-                         (back >= 0 && y0 < u.i0 + AT_TILE - 1 - back);
         // rows of other sequences behind a ragged ring tile must add nothing to a sum over its tokens: Q's and dO's
         // for a key tile, K's for a query tile (V only meets scores that are masked).  The scores that read the
         // tiles are done by then.
-        const int end = u.len - (y0 - half * 64);
+        const int end = u.len - tile0;
         if (end < AT_TILE) {
           if (KEYS) {
             if (!wait(dp_full, r & 1, 14)) return;
             at_zero_rows<DC, AT_TILE, 256>(smem + L::B + s * L::TILE, end, threadIdx.x);
           }
           at_zero_rows<DC, AT_TILE, 256>(smem + L::A + s * L::TILE, end, threadIdx.x);
+          fence_proxy_async_smem();
+        }
+        // no token in this half (no MMA reads it), or none that the warp's rows see
+        if (y0 >= u.len || y0 + 63 < lo_min || y0 > hi_max) {
+          uint32_t zeros[32];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) zeros[c] = 0;
+          if (KEYS) {
+            tmem_st_32x32b_x32(t_s, zeros);
+            tmem_st_wait();
+          }
+          tc_fence_before();
+          mbar_arrive(p_ready);
+          if (!wait(dp_full, r & 1, 24)) return;
+          tc_fence_after();
+          tmem_st_32x32b_x32(t_dp, zeros);
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(ds_ready);
+          if (KEYS) {
+            if (lane == 0) mbar_arrive(&aux_empty[sa]);
+            ++aux;
+          }
+          continue;
         }
         uint32_t sv[64];
 #pragma unroll
@@ -851,6 +910,12 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
           mbar_arrive(p_ready);  // the scores are in registers: the next tile's may overwrite them
         }
         uint64_t pv[32];
+        auto hide = [&] {  // 0 where the pair is not visible, whatever is there
+          at_hide<4>(y0, see_lo, see_hi, lo_max, hi_min, [&](int c) {
+            const float2 v = f2_unpack(pv[c >> 1]);
+            pv[c >> 1] = c & 1 ? f2_pack(v.x, 0.f) : f2_pack(0.f, v.y);
+          });
+        };
         const ulonglong2* la = reinterpret_cast<const ulonglong2*>(aux_lse + sa * AT_TILE + half * 64);
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
@@ -861,14 +926,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
           pv[2 * c] = f2_pack(at_exp2(f.x), at_exp2(f.y));
           pv[2 * c + 1] = f2_pack(at_exp2(g.x), at_exp2(g.y));
         }
-        auto hide = [&] {  // 0 where the pair is not visible, whatever is there
-#pragma unroll
-          for (int c = 0; c < 64; c += 2) {
-            const float2 v = f2_unpack(pv[c >> 1]);
-            pv[c >> 1] = f2_pack(y0 + c < see_lo || y0 + c > see_hi ? 0.f : v.x,
-                                 y0 + c + 1 < see_lo || y0 + c + 1 > see_hi ? 0.f : v.y);
-          }
-        };
+        hide();
         auto put = [&](uint32_t taddr) {  // rounded to the MMA's operand type
           uint32_t pk[32];
 #pragma unroll
@@ -880,7 +938,6 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
           tmem_st_wait();
           tc_fence_before();
         };
-        if (cut) hide();
         if (KEYS) {
           put(t_s);
           mbar_arrive(p_ready);
@@ -899,12 +956,12 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
           pv[2 * c] = f2_mul(pv[2 * c], f2_fma(f2_pack_u(dpv[4 * c], dpv[4 * c + 1]), scx2, d4.x));
           pv[2 * c + 1] = f2_mul(pv[2 * c + 1], f2_fma(f2_pack_u(dpv[4 * c + 2], dpv[4 * c + 3]), scx2, d4.y));
         }
-        // (inside the sequence p = 0 has done it)
-        if (y0 + 64 > u.len) hide();
+        if (y0 + 64 > u.len) hide();  // tokens of another sequence (inside this one p = 0 has done it)
         put(t_dp);
         mbar_arrive(ds_ready);
         if (KEYS) {
-          mbar_arrive(&aux_empty[sa]);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&aux_empty[sa]);
           ++aux;
         }
       }

@@ -195,17 +195,31 @@ __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap
       : "memory");
 }
 
-// N threads (this one `id`): zeros in rows [first, ROWS) of a [ROWS tokens][DC x 64 features] tile that
-// has arrived, so that the rows of other sequences behind a ragged tile add nothing to a product over
-// tokens (0 x their NaN would).  The 128-byte swizzle permutes inside a row only.  The writes are made
-// visible to the MMAs of the thread that this one arrives at next.
+// N threads (this one `id`): zeros in the rows from `first` to the next multiple of 16 (the tokens of one MMA;
+// those behind it are not multiplied) of a [ROWS tokens][DC x 64 features] tile that has arrived, so that the rows of other sequences behind a ragged tile add nothing to a product over
+// tokens (0 x their NaN would).  The 128-byte swizzle permutes inside a row only.  (The caller makes the
+// writes visible to the MMAs: fence_proxy_async_smem.)
 template <int DC, int ROWS, int N>
 __device__ __forceinline__ void at_zero_rows(uint8_t* tile, int first, int id) {
 #pragma unroll
   for (int c = 0; c < DC; ++c)
-    for (int at = first * 128 + id * 16; at < ROWS * 128; at += N * 16)
+    for (int at = first * 128 + id * 16; at < ((first + 15) & ~15) * 128; at += N * 16)
       *reinterpret_cast<uint4*>(tile + c * ROWS * 128 + at) = make_uint4(0, 0, 0, 0);
-  fence_proxy_async_smem();
+}
+
+// The columns [c0, c0 + 16 G) of a warp's 32 rows, 16 at a time, that some row does not see: kill(c) for
+// every column c the thread's row does not see (lo, hi: what it sees; lo_max, hi_min: what all 32 rows see).
+template <int G, typename F>
+__device__ __forceinline__ void at_hide(int c0, int lo, int hi, int lo_max, int hi_min, F kill) {
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const int b = c0 + g * 16;
+    if (b >= lo_max && b + 15 <= hi_min) continue;  // the same for the whole warp
+    const int l = lo - b, h = hi - b;
+#pragma unroll
+    for (int c = 0; c < 16; ++c)
+      if (c < l || c > h) kill(g * 16 + c);
+  }
 }
 
 // Whole warp: `cols` fp32 columns (a multiple of 8, at most MAX) from TMEM column `taddr` on of the warp's 32
