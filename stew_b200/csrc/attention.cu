@@ -33,29 +33,31 @@ constexpr int AT_KBOX = AT_KEYS * 128;       // bytes of its 64-feature TMA box
 // What a CTA's two query tiles are: one only (few tiles: an SM each), two heads of a group, or two
 // neighbouring tiles of a head (heads that share no keys).
 enum { AT_SINGLE = 0, AT_HEADS = 1, AT_TILES = 2 };
-template <int DC>
+template <int DC, bool PAIR>
 struct AttnFwdSmem {
   static constexpr int QTILE = DC * AT_BOX;
   static constexpr int TILE = DC * AT_KBOX;
-  static constexpr int RING = 10;
+  static constexpr int RING = PAIR || DC == 1 ? 10 : 4;
   static constexpr int Q = 0;
-  static constexpr int KV = 2 * QTILE;
+  static constexpr int KV = (PAIR ? 2 : 1) * QTILE;
   static constexpr int BAR = KV + RING * TILE;
   // full[RING], empty[RING], q_full, s_full[2][2], p_ready[2][2], o_done[2], o_full[2]
   static constexpr int NBAR = 2 * RING + 13;
   static constexpr int MISC = BAR + NBAR * 8;
   static constexpr int ALLOC = MISC + 16 + 1024;  // slack to align the base to 1024 B
 };
-static_assert(AttnFwdSmem<2>::ALLOC <= 232448, "shared memory budget");
-constexpr int AT_FWD_THREADS = 320;
+static_assert(AttnFwdSmem<2, true>::ALLOC <= 232448, "shared memory budget");
+static_assert(AttnFwdSmem<2, false>::ALLOC <= 115712 && AttnFwdSmem<1, false>::ALLOC <= 115712, "two CTAs on an SM");
 constexpr float AT_LAZY = 8.f;  // log2 growth of the maximum that O tolerates unscaled
 
-template <typename T, int DC>
-__global__ void __launch_bounds__(AT_FWD_THREADS, 1)
+template <typename T, int DC, bool PAIR>
+__global__ void __launch_bounds__(PAIR ? 320 : 192, PAIR ? 1 : 2)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttnParams p, T* __restrict__ out,
                     float* __restrict__ lse) {
-  using L = AttnFwdSmem<DC>;
+  using L = AttnFwdSmem<DC, PAIR>;
+  constexpr int SOFT = PAIR ? 8 : 4, THREADS = (SOFT + 2) * 32;  // softmax warps
+  constexpr int TM_O = (PAIR ? 2 : 1) * AT_TILE, TM_COLS = 2 * TM_O;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t sbase = smem_u32(smem);
@@ -70,7 +72,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC + 4);
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 256) {
+  if (threadIdx.x == SOFT * 32) {
     prefetch_tma_desc(&tm_q);
     prefetch_tma_desc(&tm_k);
     prefetch_tma_desc(&tm_v);
@@ -84,15 +86,15 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1)
   const int hk = h0 / grp, step_h = p.pair == AT_HEADS, step_i = p.pair == AT_TILES ? AT_TILE : 0;
   const AttnTile t = at_find(p, slot);
   if (t.i0 >= t.len) return;
-  const int both = p.pair == AT_HEADS ? (h0 + 1) / grp == hk : p.pair == AT_TILES && t.i0 + AT_TILE < t.len;
+  const int both = !PAIR ? 0 : p.pair == AT_HEADS ? (h0 + 1) / grp == hk : t.i0 + AT_TILE < t.len;
   if (t.tail) {
     const int n = min(1 << p.shift, t.len - t.i0), vec = p.head_dim / 8;
     for (int h = h0; h <= h0 + (both & step_h); ++h) {
-      for (int i = threadIdx.x; i < n * vec; i += AT_FWD_THREADS) {
+      for (int i = threadIdx.x; i < n * vec; i += THREADS) {
         const int64_t row = t.a + t.i0 + i / vec;
         *reinterpret_cast<uint4*>(out + (row * p.heads + h) * p.head_dim + (i % vec) * 8) = make_uint4(0, 0, 0, 0);
       }
-      for (int i = threadIdx.x; i < n; i += AT_FWD_THREADS) lse[int64_t(h) * p.tokens + t.a + t.i0 + i] = -INFINITY;
+      for (int i = threadIdx.x; i < n; i += THREADS) lse[int64_t(h) * p.tokens + t.a + t.i0 + i] = -INFINITY;
     }
     return;
   }
@@ -114,14 +116,14 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1)
     fence_barrier_init();
     *abort_flag = 0;
   }
-  if (warp == 9) {
-    tmem_alloc(tmem_slot, 512);
+  if (warp == SOFT + 1) {
+    tmem_alloc(tmem_slot, TM_COLS);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // per query tile g: scores at [128 g, 128 g + 128), O at 256 + 128 g
+  // per query tile g: scores at [128 g, 128 g + 128), O at TM_O + 128 g
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   // both tiles' keys [j_lo, j_hi] (relative to a), in tiles of 64 from a multiple of 64 on
@@ -130,7 +132,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1)
   const int j_hi = p.right < 0 ? t.len - 1 : min(t.len - 1, i_last + p.right);
   const int jt0 = j_lo / AT_KEYS, nt = j_hi / AT_KEYS - jt0 + 1;
 
-  if (warp == 8) {
+  if (warp == SOFT) {
     // ---------------------------------------------------------------- TMA
     int issued = 0;
     if (lane == 0) {
@@ -153,7 +155,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1)
         for (int x = max(0, issued - L::RING); x < issued; ++x) at_drain(&full[x % L::RING], (x / L::RING) & 1);
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == SOFT + 1) {
     // ---------------------------------------------------------------- MMA
     const uint32_t lead = elect_one();
     const int kd = (p.head_dim + 15) / 16;               // K steps of the scores
@@ -195,7 +197,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1)
 #pragma unroll
         for (int k = 0; k < AT_KEYS / 16; ++k)
           if (j0 + k * 16 < t.len)  // nothing behind the sequence's end
-            at_mma_ts(lead, tmem + (2 + g) * AT_TILE, tmem + g * AT_TILE + (i & 1) * AT_KEYS + k * 8,
+            at_mma_ts(lead, tmem + TM_O + g * AT_TILE, tmem + g * AT_TILE + (i & 1) * AT_KEYS + k * 8,
                     dv + uint64_t(k * (2048 >> 4)), id_o, i > 0 || k > 0);
         at_commit(lead, &o_done[g]);
         if (i + 1 == nt) {
@@ -216,7 +218,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1)
     // ---------------------------------------------------------------- softmax
     const int g = warp >> 2, w0 = (warp & 3) * 32;
     const uint32_t lane_off = uint32_t(w0) << 16;
-    const uint32_t t_s = tmem + lane_off + g * AT_TILE, t_o = tmem + lane_off + (2 + g) * AT_TILE;
+    const uint32_t t_s = tmem + lane_off + g * AT_TILE, t_o = tmem + lane_off + TM_O + g * AT_TILE;
     const int h = h0 + g * step_h, i0 = t.i0 + g * step_i;
     const int i = i0 + w0 + lane;  // this thread's query row, relative to a
     const float sl2 = p.scale * AT_LOG2E;
@@ -300,7 +302,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1)
     tc_fence_before();
   }
   __syncthreads();
-  if (warp == 9) tmem_dealloc(tmem, 512);
+  if (warp == SOFT + 1) tmem_dealloc(tmem, TM_COLS);
 }
 
 // ------------------------------------------------------------------ backward
@@ -345,107 +347,97 @@ __device__ __forceinline__ float at_half_warp_sum(float v) {
   return v;
 }
 
-// One CTA per (128-token tile, head), half a warp per row; reads O, dO (and V once per group).
+// One CTA per (128-token tile, head), half a warp per row; reads O and dO.  Further CTAs per (tile, key/value
+// head) read V.
 template <typename T>
 __global__ void __launch_bounds__(AT_PREP_THREADS)
     attn_prep_kernel(const __grid_constant__ AttnParams p, const T* __restrict__ out, const T* __restrict__ dout,
                      const float* __restrict__ lse, const T* __restrict__ v, int64_t v_stride, int64_t v_head_stride,
                      AttnWork w, T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dv) {
   grid_dep_wait();  // programmatic launch: no global access before the wait
-  const int slot = int(blockIdx.x / p.heads), h = blockIdx.x % p.heads;
-  const int grp = p.heads / p.kv_heads, hk = h / grp;
-  const bool first = h % grp == 0;
+  const int per_slot = p.heads + p.kv_heads;
+  const int slot = int(blockIdx.x / per_slot), h = blockIdx.x % per_slot, hk = h - p.heads;
+  const bool keys = hk >= 0;
   if (threadIdx.x == 0) {
     if (blockIdx.x == 0) *w.next = 0;
-    if (first) w.tickets[slot * p.kv_heads + hk] = 0;
+    if (keys) w.tickets[slot * p.kv_heads + hk] = 0;
   }
   const AttnTile t = at_find(p, slot);
   if (t.i0 >= t.len) return;
-  const int n = min(AT_TILE, t.len - t.i0);
-  const int sub = threadIdx.x & 15, f = sub * 8;  // this thread's 8 features
-  const bool in = f < p.head_dim;
-  float m_do = 0.f, m_dl = 0.f, m_v = 0.f;
-  const int r0 = threadIdx.x >> 4;
+  constexpr bool SCALED = at_p_shift<T>() != 0.f;
   constexpr int STEP = AT_PREP_THREADS / 16, N = AT_TILE / STEP;  // rows a thread works on: r0 + k STEP
+  const int n = min(AT_TILE, t.len - t.i0);
+  const int sub = threadIdx.x & 15, f = sub * 8, r0 = threadIdx.x >> 4;  // this thread's 8 features, first row
   const int64_t row0 = t.a + t.i0 + r0;
+  auto live = [&](int k) { return r0 + k * STEP < n && f < p.head_dim; };
   if (t.tail) {
+    const uint4 z = make_uint4(0, 0, 0, 0);
     for (int k = 0; k < N; ++k) {
-      const int64_t row = row0 + k * STEP;
-      if (r0 + k * STEP >= n || !in) continue;
-      *reinterpret_cast<uint4*>(dq + (row * p.heads + h) * p.head_dim + f) = make_uint4(0, 0, 0, 0);
-      if (first) {
-        *reinterpret_cast<uint4*>(dk + (row * p.kv_heads + hk) * p.head_dim + f) = make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(dv + (row * p.kv_heads + hk) * p.head_dim + f) = make_uint4(0, 0, 0, 0);
+      if (!live(k)) continue;
+      if (keys) {
+        const int64_t off = ((row0 + k * STEP) * p.kv_heads + hk) * p.head_dim + f;
+        *reinterpret_cast<uint4*>(dk + off) = z;
+        *reinterpret_cast<uint4*>(dv + off) = z;
+      } else {
+        *reinterpret_cast<uint4*>(dq + ((row0 + k * STEP) * p.heads + h) * p.head_dim + f) = z;
       }
     }
     return;
   }
-  uint4 o4[N], d4[N];  // every load under way before the first sum
+  if (keys && !SCALED) return;
+  uint4 x4[N], d4[N];  // every load under way before the first sum
+  float l[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) {
-    const bool live = r0 + k * STEP < n && in;
-    const int64_t off = ((row0 + k * STEP) * p.heads + h) * p.head_dim + f;
-    o4[k] = live ? *reinterpret_cast<const uint4*>(out + off) : make_uint4(0, 0, 0, 0);
-    d4[k] = live ? *reinterpret_cast<const uint4*>(dout + off) : make_uint4(0, 0, 0, 0);
+    x4[k] = d4[k] = make_uint4(0, 0, 0, 0);
+    l[k] = 0.f;
+    const int64_t row = row0 + k * STEP;
+    if (!live(k)) continue;
+    if (keys) {
+      x4[k] = *reinterpret_cast<const uint4*>(v + row * v_stride + hk * v_head_stride + f);
+    } else {
+      const int64_t off = (row * p.heads + h) * p.head_dim + f;
+      x4[k] = *reinterpret_cast<const uint4*>(out + off);
+      d4[k] = *reinterpret_cast<const uint4*>(dout + off);
+      if (sub == 0) l[k] = lse[int64_t(h) * p.tokens + row];
+    }
   }
-  constexpr bool SCALED = at_p_shift<T>() != 0.f;
+  float m_norm = 0.f, m_dl = 0.f;
 #pragma unroll
   for (int k = 0; k < N; ++k) {
-    const uint32_t* o = reinterpret_cast<const uint32_t*>(&o4[k]);
-    const uint32_t* d = reinterpret_cast<const uint32_t*>(&d4[k]);
+    const uint32_t* x = reinterpret_cast<const uint32_t*>(&x4[k]);
+    const uint32_t* d = reinterpret_cast<const uint32_t*>(keys ? &x4[k] : &d4[k]);
     float dot = 0.f, nd = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 a = at_unpack<T>(o[i]), b = at_unpack<T>(d[i]);
+      const float2 a = at_unpack<T>(x[i]), b = at_unpack<T>(d[i]);
       dot = fmaf(a.x, b.x, fmaf(a.y, b.y, dot));
       nd = fmaf(b.x, b.x, fmaf(b.y, b.y, nd));
     }
-    dot = at_half_warp_sum(dot);
-    if (r0 + k * STEP < n && sub == 0) {
-      const int64_t at = int64_t(h) * p.tokens + row0 + k * STEP;
-      const float l = lse[at];
+    if (!keys) {
+      dot = at_half_warp_sum(dot);
       // a row without weight (lse = -inf) must give p = 0
-      w.row[at] = make_float2(l == -INFINITY ? INFINITY : l * AT_LOG2E, dot);
-    }
-    if (SCALED) {
-      m_do = fmaxf(m_do, at_half_warp_sum(nd));
+      if (r0 + k * STEP < n && sub == 0)
+        w.row[int64_t(h) * p.tokens + row0 + k * STEP] = make_float2(l[k] == -INFINITY ? INFINITY : l[k] * AT_LOG2E, dot);
       m_dl = fmaxf(m_dl, fabsf(dot));
     }
-  }
-  if (SCALED && first) {
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const bool live = r0 + k * STEP < n && in;
-      o4[k] = live ? *reinterpret_cast<const uint4*>(v + (row0 + k * STEP) * v_stride + hk * v_head_stride + f)
-                   : make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const uint32_t* x = reinterpret_cast<const uint32_t*>(&o4[k]);
-      float nv = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 a = at_unpack<T>(x[i]);
-        nv = fmaf(a.x, a.x, fmaf(a.y, a.y, nv));
-      }
-      m_v = fmaxf(m_v, at_half_warp_sum(nv));
-    }
+    if (SCALED) m_norm = fmaxf(m_norm, at_half_warp_sum(nd));
   }
   if (!SCALED) return;
-  __shared__ float s_max[3][AT_PREP_THREADS / 16];
+  __shared__ float s_max[2][AT_PREP_THREADS / 16];
   if (sub == 0) {
-    s_max[0][threadIdx.x >> 4] = m_do;
-    s_max[1][threadIdx.x >> 4] = m_dl;
-    s_max[2][threadIdx.x >> 4] = m_v;
+    s_max[0][r0] = m_norm;
+    s_max[1][r0] = m_dl;
   }
   __syncthreads();
-  if (threadIdx.x < 3) {
-    float m = 0.f;
-    for (int i = 0; i < AT_PREP_THREADS / 16; ++i) m = fmaxf(m, s_max[threadIdx.x][i]);
-    const int64_t at = int64_t(h) * p.slots + slot;
-    if (threadIdx.x == 0) w.tile[at].x = sqrtf(m);
-    if (threadIdx.x == 1) w.tile[at].y = m;
-    if (threadIdx.x == 2 && first) w.vmax[int64_t(hk) * p.slots + slot] = sqrtf(m);
+  if (threadIdx.x == 0) {
+    float m = 0.f, e = 0.f;
+    for (int i = 0; i < AT_PREP_THREADS / 16; ++i) {
+      m = fmaxf(m, s_max[0][i]);
+      e = fmaxf(e, s_max[1][i]);
+    }
+    if (keys) w.vmax[int64_t(hk) * p.slots + slot] = sqrtf(m);
+    else w.tile[int64_t(h) * p.slots + slot] = make_float2(sqrtf(m), e);
   }
 }
 
@@ -486,8 +478,8 @@ struct AttnBwdSmem {
   static constexpr int UNIT = AUX + 4 * AT_TILE * 4;  // [2] AttnUnit
   static constexpr int BAR = UNIT + 2 * 64;
   // a_full[2], a_empty[2], b_full[2], b_empty[2], aux_empty[2], unit_full[2], unit_empty[2], xy_full,
-  // xy_empty, s_full, p_ready, dp_full, ds_ready, acc_full, acc_empty, drained
-  static constexpr int NBAR = 23;
+  // xy_empty, s_full, p_ready, dp_full, ds_ready, acc_full, acc_empty, drained, exp_full[2]
+  static constexpr int NBAR = 25;
   static constexpr int MISC = BAR + NBAR * 8;
   static constexpr int ALLOC = MISC + 16 + 1024;  // slack to align the base to 1024 B
 };
@@ -503,13 +495,12 @@ struct AttnBwdMaps {
 // One unit of work: a key tile and a share of its group's heads, a query tile and a head, or a piece of the
 // sum over a key tile's shares.
 enum { AT_UNIT_QUERIES = 0, AT_UNIT_KEYS = 1, AT_UNIT_JOIN = 2, AT_UNIT_END = 3 };
-constexpr int AT_PIECES = 8;  // pieces of that sum
+constexpr int AT_PIECES = 4;  // pieces of that sum
 struct AttnUnit {
   int kind, a, len, i0;  // the resident tile: tokens a + [i0, i0 + 128) of a sequence of len
   int h, hk, rank;       // head of X and Y; key/value head; the share of a key tile, or the piece of a sum
   int yt0, nt, n;        // the ring's first tile, its tiles per head, ring items
   int h0;                // first query head of a key tile's share
-  int k_exp;             // dS is scaled by 2^k_exp
   int join;              // the key tile's number among those that are shared
 };
 static_assert(sizeof(AttnUnit) <= 64, "one slot of the unit ring");
@@ -549,11 +540,13 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
   uint64_t* acc_full = ds_ready + 1;
   uint64_t* acc_empty = acc_full + 1;
   uint64_t* drained = acc_empty + 1;
+  uint64_t* exp_full = drained + 1;  // [2]: a unit's exponent of the dS scale, which comes after the unit
   float* aux_lse = reinterpret_cast<float*>(smem + L::AUX);
   float* aux_dl = aux_lse + 2 * AT_TILE;
   AttnUnit* units = reinterpret_cast<AttnUnit*>(smem + L::UNIT);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC + 4);
+  int* exponent = reinterpret_cast<int*>(smem + L::MISC + 8);  // [2]
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int grp = p.heads / p.kv_heads;
 
@@ -566,6 +559,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
       mbar_init(&aux_empty[i], 8);
       mbar_init(&unit_full[i], 1);
       mbar_init(&unit_empty[i], 9);
+      mbar_init(&exp_full[i], 1);
     }
     mbar_init(xy_full, 1);
     mbar_init(xy_empty, 1);
@@ -675,7 +669,6 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
         issued = loads + 1;
         return true;
       };
-      u.k_exp = 0;
       if (main) {
         if (!wait(xy_empty, (tiles & 1) ^ 1, 9)) break;
         if (lane == 0) {
@@ -687,7 +680,6 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
         }
         ++tiles;
         if (!load(keys ? u.h0 : u.hk, u.yt0 * AT_TILE)) break;  // the ring's first tiles before anything else
-        if (at_p_shift<T>() != 0.f) u.k_exp = at_ds_exponent(p, w, slot, u.i0, u.len, u.hk);
       } else if (u.kind == AT_UNIT_JOIN) {
         const long long t0 = clock64();
         const volatile unsigned* done = w.tickets + u.join;
@@ -708,7 +700,17 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
       }
       if (u.kind == AT_UNIT_END) break;
       if (!main) continue;
-      const float sc = at_pow2(u.k_exp - int(at_p_shift<T>()));
+      // (slot: units with tiles; the tiles of the unit before have been waited for, so the last reader of this
+      // slot is done)
+      int k_exp = 0;
+      if (at_p_shift<T>() != 0.f) {
+        k_exp = at_ds_exponent(p, w, slot, u.i0, u.len, u.hk);
+        if (lane == 0) {
+          exponent[(tiles - 1) & 1] = k_exp;
+          mbar_arrive(&exp_full[(tiles - 1) & 1]);
+        }
+      }
+      const float sc = at_pow2(k_exp - int(at_p_shift<T>()));
       int hy = keys ? u.h0 : u.hk, yt = 0;
       for (int it = 0; it < u.n; ++it, ++loads) {
         const int s = loads & 1, y0 = (u.yt0 + yt) * AT_TILE;
@@ -841,11 +843,11 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
     uint8_t* buf = smem + L::OUT + warp * 2048;
     unsigned r = 0, aux = 0, m = 0;
     // One unit's ring items.
+    int k_exp = 0;
     auto items = [&](auto keys_tag, const AttnUnit& u) {
       constexpr bool KEYS = decltype(keys_tag)::value;
       const int x = u.i0 + row;  // this thread's row, relative to a
-      const float sc = at_pow2(u.k_exp - int(at_p_shift<T>()));
-      const uint64_t scx2 = f2_pack(sc, sc);
+      float sc = 1.f;
       const int back = KEYS ? p.right : p.left, ahead = KEYS ? p.left : p.right;
       const int see_lo = back < 0 ? 0 : x - back, x0 = u.i0 + w0;
       const int see_hi = ahead < 0 ? u.len - 1 : min(u.len - 1, x + ahead);
@@ -853,12 +855,23 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
       const int lo_max = back < 0 ? 0 : x0 + 31 - back, lo_min = back < 0 ? 0 : x0 - back;
       const int hi_min = ahead < 0 ? u.len - 1 : min(u.len - 1, x0 + ahead);
       const int hi_max = ahead < 0 ? u.len - 1 : min(u.len - 1, x0 + 31 + ahead);
-      uint64_t row_lse = 0, row_dl = 0;  // twice each
+      uint64_t row_lse = 0;  // twice
+      float row_dl = 0.f;
       if (!KEYS) {
         const float2 v = x < u.len ? w.row[int64_t(u.h) * p.tokens + u.a + x] : make_float2(INFINITY, 0.f);
         row_lse = f2_pack(at_p_shift<T>() - v.x, at_p_shift<T>() - v.x);
-        row_dl = f2_pack(-v.y * sc, -v.y * sc);
+        row_dl = -v.y;
       }
+      auto scale = [&](int it) {
+        if (it > 0) return true;
+        if (at_p_shift<T>() != 0.f) {
+          if (!wait(&exp_full[m & 1], (m >> 1) & 1, 29)) return false;
+          k_exp = exponent[m & 1];
+        }
+        sc = at_pow2(k_exp - int(at_p_shift<T>()));
+        row_dl *= sc;
+        return true;
+      };
       int yt = 0;
       for (int it = 0; it < u.n; ++it, ++r) {
         const int s = r & 1, sa = aux & 1;
@@ -889,7 +902,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
           }
           tc_fence_before();
           mbar_arrive(p_ready);
-          if (!wait(dp_full, r & 1, 24)) return;
+          if (!scale(it) || !wait(dp_full, r & 1, 24)) return;
           tc_fence_after();
           tmem_st_32x32b_x32(t_dp, zeros);
           tmem_st_wait();
@@ -942,8 +955,9 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
           put(t_s);
           mbar_arrive(p_ready);
         }
-        if (!wait(dp_full, r & 1, 24)) return;
+        if (!scale(it) || !wait(dp_full, r & 1, 24)) return;
         tc_fence_after();
+        const uint64_t scx2 = f2_pack(sc, sc), row_dl2 = f2_pack(row_dl, row_dl);
         uint32_t dpv[64];
 #pragma unroll
         for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(t_dp + c * 32, *reinterpret_cast<uint32_t(*)[32]>(dpv + c * 32));
@@ -951,7 +965,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
         const ulonglong2* ld = reinterpret_cast<const ulonglong2*>(aux_dl + sa * AT_TILE + half * 64);
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
-          ulonglong2 d4 = make_ulonglong2(row_dl, row_dl);
+          ulonglong2 d4 = make_ulonglong2(row_dl2, row_dl2);
           if (KEYS) d4 = ld[c];
           pv[2 * c] = f2_mul(pv[2 * c], f2_fma(f2_pack_u(dpv[4 * c], dpv[4 * c + 1]), scx2, d4.x));
           pv[2 * c + 1] = f2_mul(pv[2 * c + 1], f2_fma(f2_pack_u(dpv[4 * c + 2], dpv[4 * c + 3]), scx2, d4.y));
@@ -982,7 +996,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
           float4 v[N];
 #pragma unroll
           for (int e = 0; e < N; ++e) v[e] = __ldcg(from + e * AT_TILE);
-#pragma unroll 4
+#pragma unroll 2
           for (int q = 1; q < split; ++q) {
 #pragma unroll
             for (int e = 0; e < N; ++e) {
@@ -1007,7 +1021,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
       ++m;
       tc_fence_after();
       const int rows = u.len - u.i0 - w0;  // of this warp's 32
-      const float fx = p.scale * at_pow2(-u.k_exp);
+      const float fx = p.scale * at_pow2(-k_exp);
       if (!keys) {
         const int c0 = half * DC * 32;
         T* to = dq + (int64_t(u.a + u.i0 + w0) * p.heads + u.h) * p.head_dim + c0;
@@ -1117,24 +1131,32 @@ static int attn_smem(K kernel, int bytes, bool (&done)[64]) {
   return NF4B_OK;
 }
 
-template <typename T, int DC>
-static int attn_fwd_launch(const nf4b_attn& a, void* out, float* lse, cudaStream_t s) {
+template <typename T, int DC, bool PAIR>
+static int attn_fwd_launch(const nf4b_attn& a, int kind, void* out, float* lse, cudaStream_t s) {
   CUtensorMap q, k, v;
   int st = attn_tmap(&q, a, a.q, a.heads, a.q_stride, a.q_head_stride, AT_TILE);
   if (st == NF4B_OK) st = attn_tmap(&k, a, a.k, a.kv_heads, a.k_stride, a.k_head_stride, AT_KEYS);
   if (st == NF4B_OK) st = attn_tmap(&v, a, a.v, a.kv_heads, a.v_stride, a.v_head_stride, AT_KEYS);
   static bool done[64] = {false};
-  if (st == NF4B_OK) st = attn_smem(attn_fwd_kernel<T, DC>, AttnFwdSmem<DC>::ALLOC, done);
+  if (st == NF4B_OK) st = attn_smem(attn_fwd_kernel<T, DC, PAIR>, AttnFwdSmem<DC, PAIR>::ALLOC, done);
   if (st != NF4B_OK) return st;
-  // pairs of query tiles once there are more tiles than SMs; with fewer an SM each is quicker
-  const int grp = a.heads / a.kv_heads;
-  const bool many = (double(a.tokens) / AT_TILE + 0.5 * a.rows) * a.heads > 148;
-  const int pair = !many ? AT_SINGLE : grp > 1 ? AT_HEADS : AT_TILES;
-  const AttnParams p = attn_params(a, pair == AT_TILES ? 8 : 7, pair);
-  const unsigned per_slot = unsigned(pair == AT_HEADS ? a.kv_heads * ((grp + 1) / 2) : a.heads);
-  NF4B_CUDA_TRY(launch_pdl(attn_fwd_kernel<T, DC>, dim3(unsigned(p.slots) * per_slot), dim3(AT_FWD_THREADS),
-                           size_t(AttnFwdSmem<DC>::ALLOC), s, q, k, v, p, static_cast<T*>(out), lse));
+  const AttnParams p = attn_params(a, kind == AT_TILES ? 8 : 7, kind);
+  const unsigned per_slot = unsigned(kind == AT_HEADS ? a.kv_heads * ((a.heads / a.kv_heads + 1) / 2) : a.heads);
+  NF4B_CUDA_TRY(launch_pdl(attn_fwd_kernel<T, DC, PAIR>, dim3(unsigned(p.slots) * per_slot), dim3(PAIR ? 320 : 192),
+                           size_t(AttnFwdSmem<DC, PAIR>::ALLOC), s, q, k, v, p, static_cast<T*>(out), lse));
   return launch_status("attn_fwd_kernel launch");
+}
+
+template <typename T>
+static int attn_fwd_pick(const nf4b_attn& a, void* out, float* lse, cudaStream_t s) {
+  const int grp = a.heads / a.kv_heads;
+  bool pair = (double(a.tokens) / AT_TILE + 0.5 * a.rows) * a.heads > 148;
+  const char* e = std::getenv("STEW_ATTN_PAIR");
+  if (e) pair = e[0] == '1';
+  const int kind = !pair ? AT_SINGLE : grp > 1 ? AT_HEADS : AT_TILES;
+  if (a.head_dim > 64)
+    return pair ? attn_fwd_launch<T, 2, true>(a, kind, out, lse, s) : attn_fwd_launch<T, 2, false>(a, kind, out, lse, s);
+  return pair ? attn_fwd_launch<T, 1, true>(a, kind, out, lse, s) : attn_fwd_launch<T, 1, false>(a, kind, out, lse, s);
 }
 
 extern "C" int nf4b_attn_fwd(const nf4b_attn* args, void* out, float* lse, void* stream) {
@@ -1147,10 +1169,7 @@ extern "C" int nf4b_attn_fwd(const nf4b_attn* args, void* out, float* lse, void*
   st = check_device();
   if (st != NF4B_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool wide = a.head_dim > 64;
-  if (a.dtype == NF4B_F16)
-    return wide ? attn_fwd_launch<__half, 2>(a, out, lse, s) : attn_fwd_launch<__half, 1>(a, out, lse, s);
-  return wide ? attn_fwd_launch<__nv_bfloat16, 2>(a, out, lse, s) : attn_fwd_launch<__nv_bfloat16, 1>(a, out, lse, s);
+  return a.dtype == NF4B_F16 ? attn_fwd_pick<__half>(a, out, lse, s) : attn_fwd_pick<__nv_bfloat16>(a, out, lse, s);
 }
 
 extern "C" int nf4b_attn_error_flag(int* value, int reset) {
@@ -1247,7 +1266,8 @@ static int attn_bwd_launch(const nf4b_attn& a, const void* out, const float* lse
   AttnWork w;
   attn_work(a, split, work, &w);
   T *tq = static_cast<T*>(dq), *tk = static_cast<T*>(dk), *tv = static_cast<T*>(dv);
-  NF4B_CUDA_TRY(launch_pdl(attn_prep_kernel<T>, dim3(unsigned(p.slots) * unsigned(a.heads)), dim3(AT_PREP_THREADS),
+  NF4B_CUDA_TRY(launch_pdl(attn_prep_kernel<T>, dim3(unsigned(p.slots) * unsigned(a.heads + a.kv_heads)),
+                           dim3(AT_PREP_THREADS),
                            size_t(0), s, p, static_cast<const T*>(out), static_cast<const T*>(dout), lse,
                            static_cast<const T*>(a.v), a.v_stride, a.v_head_stride, w, tq, tk, tv));
   const int64_t units = int64_t(p.slots) * (int64_t(a.kv_heads) * (split > 1 ? split + AT_PIECES : 1) + a.heads);
