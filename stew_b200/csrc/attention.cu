@@ -238,7 +238,8 @@ __global__ void __launch_bounds__(PAIR ? 320 : 192, PAIR ? 1 : 2)
 #pragma unroll
       for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(t_s + b * AT_KEYS + c * 32, s[c]);
       tmem_ld_wait();
-      at_hide<4>(j0, see_lo, see_hi, lo_max, hi_min, [&](int c) { s[c >> 5][c & 31] = 0xff800000u; });  // -inf
+      if (j0 < lo_max || j0 + AT_KEYS - 1 > hi_min)
+        at_hide(see_lo - j0, see_hi - j0, [&](int c) { s[c >> 5][c & 31] = 0xff800000u; });  // -inf
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int c = 0; c < AT_KEYS; c += 2)
@@ -924,7 +925,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
         }
         uint64_t pv[32];
         auto hide = [&] {  // 0 where the pair is not visible, whatever is there
-          at_hide<4>(y0, see_lo, see_hi, lo_max, hi_min, [&](int c) {
+          at_hide(see_lo - y0, see_hi - y0, [&](int c) {
             const float2 v = f2_unpack(pv[c >> 1]);
             pv[c >> 1] = c & 1 ? f2_pack(v.x, 0.f) : f2_pack(0.f, v.y);
           });
@@ -939,7 +940,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
           pv[2 * c] = f2_pack(at_exp2(f.x), at_exp2(f.y));
           pv[2 * c + 1] = f2_pack(at_exp2(g.x), at_exp2(g.y));
         }
-        hide();
+        if (y0 < lo_max || y0 + 63 > hi_min) hide();
         auto put = [&](uint32_t taddr) {  // rounded to the MMA's operand type
           uint32_t pk[32];
 #pragma unroll

@@ -207,18 +207,16 @@ __device__ __forceinline__ void at_zero_rows(uint8_t* tile, int first, int id) {
       *reinterpret_cast<uint4*>(tile + c * ROWS * 128 + at) = make_uint4(0, 0, 0, 0);
 }
 
-// The columns [c0, c0 + 16 G) of a warp's 32 rows, 16 at a time, that some row does not see: kill(c) for
-// every column c the thread's row does not see (lo, hi: what it sees; lo_max, hi_min: what all 32 rows see).
-template <int G, typename F>
-__device__ __forceinline__ void at_hide(int c0, int lo, int hi, int lo_max, int hi_min, F kill) {
+// kill(c) for the columns c of [0, 64) outside [lo, hi], from bit masks (a test and a select a column).
+template <typename F>
+__device__ __forceinline__ void at_hide(int lo, int hi, F kill) {
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
-    const int b = c0 + g * 16;
-    if (b >= lo_max && b + 15 <= hi_min) continue;  // the same for the whole warp
-    const int l = lo - b, h = hi - b;
+  for (int w = 0; w < 2; ++w) {
+    const int l = min(max(lo - 32 * w, 0), 32), h = min(max(hi + 1 - 32 * w, 0), 32);  // bits [l, h) stay
+    const uint32_t keep = (h == 32 ? 0xffffffffu : (1u << h) - 1u) & (l == 32 ? 0u : 0xffffffffu << l);
 #pragma unroll
-    for (int c = 0; c < 16; ++c)
-      if (c < l || c > h) kill(g * 16 + c);
+    for (int c = 0; c < 32; ++c)
+      if (!(keep >> c & 1u)) kill(w * 32 + c);
   }
 }
 
