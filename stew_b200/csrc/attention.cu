@@ -16,86 +16,75 @@
 namespace nf4b {
 
 // ------------------------------------------------------------------- forward
-// One CTA per SM works on two 128-token query tiles A and B side by side (two heads of a group, or two
-// neighbouring tiles of a head) over key tiles of 64 tokens, so one tile's softmax runs beside the other's
-// MMAs and every K and V tile that TMA brings in serves both.  TMEM (512 columns): per query tile two
-// buffers of scores S = Q K^T, 64 columns each, and the output O.  The scores of key tile i + 1 are computed
-// while the softmax of tile i runs; its probabilities overwrite its own scores as 16-bit values and are the A
-// operand of P V straight from TMEM.  V's tile is read as an MN-major operand, so nothing is transposed.
-//   warps 0-7  softmax: one thread per query row, warps 0-3 for A, 4-7 for B
-//   warp 8     TMA: Q, then K and V tiles through a ring of slots
-//   warp 9     TMEM allocation, MMA issue
+// One CTA per (128-token query tile, head), over key tiles of 64 tokens; two CTAs on an SM, so one's
+// softmax runs beside the other's MMAs.  TMEM (256 columns): two buffers of scores S = Q K^T, 64
+// columns each, and the output O.  The scores of tile i + 1 are computed while the softmax of tile i
+// runs; its probabilities overwrite its own scores as 16-bit values and are the A operand of P V
+// straight from TMEM.  Q, K and V are TMA tiles in shared memory (V's is read as an MN-major operand,
+// so nothing is transposed).
+//   warps 0-3  softmax: one thread per query row
+//   warp 4     TMA: Q, then K and V tiles through a ring of slots
+//   warp 5     TMEM allocation, MMA issue
 // One pass over the keys with a running maximum m and sum l (Milakov and Gimelshein's online
 // softmax); O is rescaled only when the maximum has grown by more than 2^8, else P may exceed 1
 // (by at most 2^8, far inside fp16's range) and l with it -- the quotient is the same.
 constexpr int AT_KEYS = 64;                  // keys of a tile
 constexpr int AT_KBOX = AT_KEYS * 128;       // bytes of its 64-feature TMA box
-// What a CTA's two query tiles are: one only (few tiles: an SM each), two heads of a group, or two
-// neighbouring tiles of a head (heads that share no keys).
-enum { AT_SINGLE = 0, AT_HEADS = 1, AT_TILES = 2 };
-template <int DC, bool PAIR>
+template <int DC>
 struct AttnFwdSmem {
   static constexpr int QTILE = DC * AT_BOX;
   static constexpr int TILE = DC * AT_KBOX;
-  static constexpr int RING = PAIR || DC == 1 ? 10 : 4;
+  static constexpr int RING = DC == 1 ? 10 : 4;
   static constexpr int Q = 0;
-  static constexpr int KV = (PAIR ? 2 : 1) * QTILE;
+  static constexpr int KV = QTILE;
   static constexpr int BAR = KV + RING * TILE;
-  // full[RING], empty[RING], q_full, s_full[2][2], p_ready[2][2], o_done[2], o_full[2]
-  static constexpr int NBAR = 2 * RING + 13;
+  // full[RING], empty[RING], q_full, s_full[2], p_ready[2], o_done, o_full
+  static constexpr int NBAR = 2 * RING + 7;
   static constexpr int MISC = BAR + NBAR * 8;
   static constexpr int ALLOC = MISC + 16 + 1024;  // slack to align the base to 1024 B
 };
-static_assert(AttnFwdSmem<2, true>::ALLOC <= 232448, "shared memory budget");
-static_assert(AttnFwdSmem<2, false>::ALLOC <= 115712 && AttnFwdSmem<1, false>::ALLOC <= 115712, "two CTAs on an SM");
+static_assert(AttnFwdSmem<2>::ALLOC <= 115712 && AttnFwdSmem<1>::ALLOC <= 115712, "two CTAs on an SM");
+constexpr int AT_FWD_THREADS = 192;
 constexpr float AT_LAZY = 8.f;  // log2 growth of the maximum that O tolerates unscaled
 
-template <typename T, int DC, bool PAIR>
-__global__ void __launch_bounds__(PAIR ? 320 : 192, PAIR ? 1 : 2)
+template <typename T, int DC>
+__global__ void __launch_bounds__(AT_FWD_THREADS, 2)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttnParams p, T* __restrict__ out,
                     float* __restrict__ lse) {
-  using L = AttnFwdSmem<DC, PAIR>;
-  constexpr int SOFT = PAIR ? 8 : 4, THREADS = (SOFT + 2) * 32;  // softmax warps
-  constexpr int TM_O = (PAIR ? 2 : 1) * AT_TILE, TM_COLS = 2 * TM_O;
+  using L = AttnFwdSmem<DC>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t sbase = smem_u32(smem);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR);
   uint64_t* empty = full + L::RING;
   uint64_t* q_full = empty + L::RING;
-  uint64_t* s_full = q_full + 1;    // [query tile][buffer]
-  uint64_t* p_ready = s_full + 4;   // [query tile][buffer]
-  uint64_t* o_done = p_ready + 4;   // [query tile], a phase per P V (at most one behind where it is waited for)
-  uint64_t* o_full = o_done + 2;    // [query tile], after the last
+  uint64_t* s_full = q_full + 1;    // [buffer]
+  uint64_t* p_ready = s_full + 2;   // [buffer]
+  uint64_t* o_done = p_ready + 2;   // a phase per P V (at most one behind where it is waited for)
+  uint64_t* o_full = o_done + 1;    // after the last
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC + 4);
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
 
-  if (threadIdx.x == SOFT * 32) {
+  if (threadIdx.x == 128) {
     prefetch_tma_desc(&tm_q);
     prefetch_tma_desc(&tm_k);
     prefetch_tma_desc(&tm_v);
   }
   grid_dep_wait();  // programmatic launch: no global access before the wait
   // the last slots first: a causal sequence's last tiles see the most keys
-  const int grp = p.heads / p.kv_heads, pairs = (grp + 1) >> 1;
-  const int per_slot = p.pair == AT_HEADS ? p.kv_heads * pairs : p.heads;
-  const int slot = p.slots - 1 - int(blockIdx.x / per_slot), unit = blockIdx.x % per_slot;
-  const int h0 = p.pair == AT_HEADS ? unit / pairs * grp + unit % pairs * 2 : unit;  // tile A's head
-  const int hk = h0 / grp, step_h = p.pair == AT_HEADS, step_i = p.pair == AT_TILES ? AT_TILE : 0;
+  const int slot = p.slots - 1 - int(blockIdx.x / p.heads);
+  const int h = blockIdx.x % p.heads, hk = h / (p.heads / p.kv_heads);
   const AttnTile t = at_find(p, slot);
   if (t.i0 >= t.len) return;
-  const int both = !PAIR ? 0 : p.pair == AT_HEADS ? (h0 + 1) / grp == hk : t.i0 + AT_TILE < t.len;
   if (t.tail) {
-    const int n = min(1 << p.shift, t.len - t.i0), vec = p.head_dim / 8;
-    for (int h = h0; h <= h0 + (both & step_h); ++h) {
-      for (int i = threadIdx.x; i < n * vec; i += THREADS) {
-        const int64_t row = t.a + t.i0 + i / vec;
-        *reinterpret_cast<uint4*>(out + (row * p.heads + h) * p.head_dim + (i % vec) * 8) = make_uint4(0, 0, 0, 0);
-      }
-      for (int i = threadIdx.x; i < n; i += THREADS) lse[int64_t(h) * p.tokens + t.a + t.i0 + i] = -INFINITY;
+    const int n = min(AT_TILE, t.len - t.i0), vec = p.head_dim / 8;
+    for (int i = threadIdx.x; i < n * vec; i += AT_FWD_THREADS) {
+      const int64_t row = t.a + t.i0 + i / vec;
+      *reinterpret_cast<uint4*>(out + (row * p.heads + h) * p.head_dim + (i % vec) * 8) = make_uint4(0, 0, 0, 0);
     }
+    if (threadIdx.x < n) lse[int64_t(h) * p.tokens + t.a + t.i0 + threadIdx.x] = -INFINITY;
     return;
   }
 
@@ -105,42 +94,37 @@ __global__ void __launch_bounds__(PAIR ? 320 : 192, PAIR ? 1 : 2)
       mbar_init(&empty[i], 1);
     }
     mbar_init(q_full, 1);
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_ready[i], 128);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&o_done[i], 1);
-      mbar_init(&o_full[i], 1);
-    }
+    mbar_init(o_done, 1);
+    mbar_init(o_full, 1);
     fence_barrier_init();
     *abort_flag = 0;
   }
-  if (warp == SOFT + 1) {
-    tmem_alloc(tmem_slot, TM_COLS);
+  if (warp == 5) {
+    tmem_alloc(tmem_slot, 256);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // per query tile g: scores at [128 g, 128 g + 128), O at TM_O + 128 g
+  // scores at [0, 128), O behind them
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
-  // both tiles' keys [j_lo, j_hi] (relative to a), in tiles of 64 from a multiple of 64 on
-  const int i_last = min(t.i0 + (both ? step_i : 0) + AT_TILE, t.len) - 1;
+  // the tile's keys [j_lo, j_hi] (relative to a), in tiles of 64 from a multiple of 64 on
+  const int i_last = min(t.i0 + AT_TILE, t.len) - 1;
   const int j_lo = p.left < 0 ? 0 : max(0, t.i0 - p.left);
   const int j_hi = p.right < 0 ? t.len - 1 : min(t.len - 1, i_last + p.right);
   const int jt0 = j_lo / AT_KEYS, nt = j_hi / AT_KEYS - jt0 + 1;
 
-  if (warp == SOFT) {
+  if (warp == 4) {
     // ---------------------------------------------------------------- TMA
     int issued = 0;
     if (lane == 0) {
-      mbar_arrive_expect_tx(q_full, (1 + both) * L::QTILE);
-      for (int g = 0; g <= both; ++g)
-        for (int c = 0; c < DC; ++c)
-          tma_load_3d(sbase + L::Q + g * L::QTILE + c * AT_BOX, &tm_q, q_full, c * 64, h0 + g * step_h,
-                      t.a + t.i0 + g * step_i);
+      mbar_arrive_expect_tx(q_full, L::QTILE);
+      for (int c = 0; c < DC; ++c) tma_load_3d(sbase + L::Q + c * AT_BOX, &tm_q, q_full, c * 64, h, t.a + t.i0);
       for (int x = 0; x < 2 * nt; ++x, ++issued) {
         const int s = x % L::RING;
         if (!at_wait(&empty[s], ((x / L::RING) & 1) ^ 1, abort_flag, 1)) break;
@@ -155,83 +139,73 @@ __global__ void __launch_bounds__(PAIR ? 320 : 192, PAIR ? 1 : 2)
         for (int x = max(0, issued - L::RING); x < issued; ++x) at_drain(&full[x % L::RING], (x / L::RING) & 1);
       }
     }
-  } else if (warp == SOFT + 1) {
+  } else if (warp == 5) {
     // ---------------------------------------------------------------- MMA
     const uint32_t lead = elect_one();
     const int kd = (p.head_dim + 15) / 16;               // K steps of the scores
     const uint32_t id_s = at_idesc<T>(AT_KEYS, false);
     const uint32_t id_o = at_idesc<T>(kd * 16, true);    // N = head_dim rounded up to 16
-    const uint64_t dq0 = smem_desc_sw128(sbase + L::Q, 16, 1024);
+    const uint64_t dq = smem_desc_sw128(sbase + L::Q, 16, 1024);
     const uint64_t dk0 = smem_desc_sw128(sbase + L::KV, 16, 1024);
     const uint64_t dv0 = smem_desc_sw128(sbase + L::KV, AT_KBOX, 1024);
-    bool ok = __all_sync(0xffffffffu, at_wait(q_full, 0, abort_flag, 3));
+    bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
       ok = __all_sync(0xffffffffu, ok && at_wait(bar, parity, abort_flag, where));
       return ok;
     };
     auto arrived = [&](int x) { return wait(&full[x % L::RING], (x / L::RING) & 1, 4); };
-    auto scores = [&](int i, int g) {
-      const uint64_t dk = dk0 + uint64_t((2 * i) % L::RING * (L::TILE >> 4)), dq = dq0 + uint64_t(g * (L::QTILE >> 4));
+    auto scores = [&](int i) {
+      const uint64_t dk = dk0 + uint64_t((2 * i) % L::RING * (L::TILE >> 4));
 #pragma unroll
       for (int k = 0; k < DC * 4; ++k)
         if (k < kd)
-          at_mma_ss(lead, tmem + g * AT_TILE + (i & 1) * AT_KEYS, dq + uint64_t((k >> 2) * (AT_BOX >> 4) + (k & 3) * 2),
+          at_mma_ss(lead, tmem + (i & 1) * AT_KEYS, dq + uint64_t((k >> 2) * (AT_BOX >> 4) + (k & 3) * 2),
                     dk + uint64_t((k >> 2) * (AT_KBOX >> 4) + (k & 3) * 2), id_s, k > 0);
-      at_commit(lead, &s_full[2 * g + (i & 1)]);
-      if (g == both) at_commit(lead, &empty[(2 * i) % L::RING]);
+      at_commit(lead, &s_full[i & 1]);
+      at_commit(lead, &empty[(2 * i) % L::RING]);
     };
-    for (int i = 0; i < 2 && i < nt; ++i) {
+    wait(q_full, 0, 3);
+    for (int i = 0; ok && i < 2 && i < nt; ++i) {
       if (!arrived(2 * i)) break;
       tc_fence_after();
-      for (int g = 0; g <= both; ++g) scores(i, g);
+      scores(i);
     }
-    int last = -1;  // query tiles whose last product is issued
     for (int i = 0; ok && i < nt; ++i) {
       const int sv = (2 * i + 1) % L::RING;
-      if (!arrived(2 * i + 1) || (i + 2 < nt && !arrived(2 * i + 4))) break;
+      if (!arrived(2 * i + 1) || (i + 2 < nt && !arrived(2 * i + 4)) || !wait(&p_ready[i & 1], (i >> 1) & 1, 6)) break;
+      tc_fence_after();
       const uint64_t dv = dv0 + uint64_t(sv * (L::TILE >> 4));
       const int j0 = (jt0 + i) * AT_KEYS;
-      for (int g = 0; g <= both; ++g) {
-        if (!wait(&p_ready[2 * g + (i & 1)], (i >> 1) & 1, 6)) break;
-        tc_fence_after();
 #pragma unroll
-        for (int k = 0; k < AT_KEYS / 16; ++k)
-          if (j0 + k * 16 < t.len)  // nothing behind the sequence's end
-            at_mma_ts(lead, tmem + TM_O + g * AT_TILE, tmem + g * AT_TILE + (i & 1) * AT_KEYS + k * 8,
-                    dv + uint64_t(k * (2048 >> 4)), id_o, i > 0 || k > 0);
-        at_commit(lead, &o_done[g]);
-        if (i + 1 == nt) {
-          at_commit(lead, &o_full[g]);
-          last = g;
-        }
-        if (g == both) at_commit(lead, &empty[sv]);
-        // the scores of tile i + 2 overwrite P of tile i: MMAs of one thread run in order
-        if (i + 2 < nt) scores(i + 2, g);
-      }
+      for (int k = 0; k < AT_KEYS / 16; ++k)
+        if (j0 + k * 16 < t.len)  // nothing behind the sequence's end
+          at_mma_ts(lead, tmem + AT_TILE, tmem + (i & 1) * AT_KEYS + k * 8, dv + uint64_t(k * (2048 >> 4)), id_o,
+                    i > 0 || k > 0);
+      at_commit(lead, o_done);
+      at_commit(lead, &empty[sv]);
+      // the scores of tile i + 2 overwrite P of tile i: MMAs of one thread run in order
+      if (i + 2 < nt) scores(i + 2);
     }
     // nothing in flight when TMEM and shared memory go
-    for (int g = 0; g <= both; ++g) {
-      if (g > last) at_commit(lead, &o_full[g]);
-      at_drain(&o_full[g], 0);
-    }
-  } else if (warp < 4 + 4 * both) {
+    at_commit(lead, o_full);
+    at_drain(o_full, 0);
+  } else {
     // ---------------------------------------------------------------- softmax
-    const int g = warp >> 2, w0 = (warp & 3) * 32;
+    const int w0 = warp * 32;
     const uint32_t lane_off = uint32_t(w0) << 16;
-    const uint32_t t_s = tmem + lane_off + g * AT_TILE, t_o = tmem + lane_off + TM_O + g * AT_TILE;
-    const int h = h0 + g * step_h, i0 = t.i0 + g * step_i;
-    const int i = i0 + w0 + lane;  // this thread's query row, relative to a
+    const uint32_t t_s = tmem + lane_off, t_o = tmem + lane_off + AT_TILE;
+    const int i = t.i0 + threadIdx.x;  // this thread's query row, relative to a
     const float sl2 = p.scale * AT_LOG2E;
     const uint64_t sl2x2 = f2_pack(sl2, sl2);
     const int see_lo = p.left < 0 ? 0 : i - p.left;
     const int see_hi = p.right < 0 ? t.len - 1 : min(t.len - 1, i + p.right);
-    const int lo_max = p.left < 0 ? 0 : i0 + w0 + 31 - p.left;  // what all rows of the warp see
-    const int hi_min = p.right < 0 ? t.len - 1 : min(t.len - 1, i0 + w0 + p.right);
+    const int lo_max = p.left < 0 ? 0 : t.i0 + w0 + 31 - p.left;  // what all rows of the warp see
+    const int hi_min = p.right < 0 ? t.len - 1 : min(t.len - 1, t.i0 + w0 + p.right);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int it = 0; it < nt; ++it) {
       const int j0 = (jt0 + it) * AT_KEYS, b = it & 1;
-      ok = at_wait(&s_full[2 * g + b], (it >> 1) & 1, abort_flag, 7);
+      ok = at_wait(&s_full[b], (it >> 1) & 1, abort_flag, 7);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       uint32_t s[2][32];
@@ -250,7 +224,7 @@ __global__ void __launch_bounds__(PAIR ? 320 : 192, PAIR ? 1 : 2)
       if (it > 0 && __any_sync(0xffffffffu, grow)) {
         const float f = grow ? at_exp2((m - top) * sl2) : 1.f;
         l *= f;
-        ok = at_wait(&o_done[g], (it - 1) & 1, abort_flag, 9);  // the products so far
+        ok = at_wait(o_done, (it - 1) & 1, abort_flag, 9);  // the products so far
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
 #pragma unroll 1
@@ -279,31 +253,31 @@ __global__ void __launch_bounds__(PAIR ? 320 : 192, PAIR ? 1 : 2)
       tmem_st_32x32b_x32(t_s + b * AT_KEYS, pk);
       const float2 l2 = f2_unpack(f2_add(sum[0], sum[1]));
       l += l2.x + l2.y;
-      if (j0 + AT_KEYS > t.len) {  // the ragged last tile: V's rows behind the sequence's end (zeros from either)
+      if (j0 + AT_KEYS > t.len) {  // the ragged last tile: V's rows behind the sequence's end
         const int x = 2 * it + 1;
         ok = at_wait(&full[x % L::RING], (x / L::RING) & 1, abort_flag, 2);
         if (!__all_sync(0xffffffffu, ok)) break;
-        at_zero_rows<DC, AT_KEYS, 128>(smem + L::KV + (x % L::RING) * L::TILE, t.len - j0, threadIdx.x & 127);
+        at_zero_rows<DC, AT_KEYS, 128>(smem + L::KV + (x % L::RING) * L::TILE, t.len - j0, threadIdx.x);
         fence_proxy_async_smem();
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&p_ready[2 * g + b]);
+      mbar_arrive(&p_ready[b]);
     }
-    if (__all_sync(0xffffffffu, ok)) ok = at_wait(&o_full[g], 0, abort_flag, 8);
+    if (__all_sync(0xffffffffu, ok)) ok = at_wait(o_full, 0, abort_flag, 8);
     if (__all_sync(0xffffffffu, ok)) {
       tc_fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      const int64_t row = t.a + i0 + w0;
-      // this tile's MMAs are done: its Q tile's memory is free
-      at_store_rows<T, DC * 64>(t_o, smem + L::Q + g * L::QTILE + w0 * DC * 128, out + (row * p.heads + h) * p.head_dim,
-                                int64_t(p.heads) * p.head_dim, t.len - i0 - w0, p.head_dim, inv);
+      const int64_t row = t.a + t.i0 + w0;
+      // every MMA is done: the Q tile's memory is free
+      at_store_rows<T, DC * 64>(t_o, smem + L::Q + w0 * DC * 128, out + (row * p.heads + h) * p.head_dim,
+                                int64_t(p.heads) * p.head_dim, t.len - t.i0 - w0, p.head_dim, inv);
       if (i < t.len) lse[int64_t(h) * p.tokens + row + lane] = l == 0.f ? -INFINITY : m * p.scale + logf(l);
     }
     tc_fence_before();
   }
   __syncthreads();
-  if (warp == SOFT + 1) tmem_dealloc(tmem, TM_COLS);
+  if (warp == 5) tmem_dealloc(tmem, 256);
 }
 
 // ------------------------------------------------------------------ backward
@@ -883,15 +857,17 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
         // rows of other sequences behind a ragged ring tile must add nothing to a sum over its tokens: Q's and dO's
         // for a key tile, K's for a query tile (V only meets scores that are masked).  The scores that read the
         // tiles are done by then.
-        const int end = u.len - tile0;
-        if (end < AT_TILE) {
+        auto cut_tile = [&] {
+          const int end = u.len - tile0;
+          if (end >= AT_TILE) return true;
           if (KEYS) {
-            if (!wait(dp_full, r & 1, 14)) return;
+            if (!wait(dp_full, r & 1, 14)) return false;
             at_zero_rows<DC, AT_TILE, 256>(smem + L::B + s * L::TILE, end, threadIdx.x);
           }
           at_zero_rows<DC, AT_TILE, 256>(smem + L::A + s * L::TILE, end, threadIdx.x);
           fence_proxy_async_smem();
-        }
+          return true;
+        };
         // no token in this half (no MMA reads it), or none that the warp's rows see
         if (y0 >= u.len || y0 + 63 < lo_min || y0 > hi_max) {
           uint32_t zeros[32];
@@ -901,6 +877,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
             tmem_st_32x32b_x32(t_s, zeros);
             tmem_st_wait();
           }
+          if (!cut_tile()) return;
           tc_fence_before();
           mbar_arrive(p_ready);
           if (!scale(it) || !wait(dp_full, r & 1, 24)) return;
@@ -941,6 +918,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
           pv[2 * c + 1] = f2_pack(at_exp2(g.x), at_exp2(g.y));
         }
         if (y0 < lo_max || y0 + 63 > hi_min) hide();
+        if (!cut_tile()) return;
         auto put = [&](uint32_t taddr) {  // rounded to the MMA's operand type
           uint32_t pk[32];
 #pragma unroll
@@ -1084,7 +1062,7 @@ static int attn_checks(const nf4b_attn* in, nf4b_attn* a) {
   NF4B_RETURN_IF(a->head_dim % 8 != 0 || a->head_dim > AT_MAX_DIM, NF4B_ERR_UNSUPPORTED);
   NF4B_RETURN_IF(a->tokens > 0x3FFFFFFF || a->rows > 0x3FFFFFFF || a->heads > 65535, NF4B_ERR_UNSUPPORTED);
   // CTAs of a launch
-  NF4B_RETURN_IF(at_slots(a->tokens, a->rows, 7) * (2 + AT_PIECES) * a->heads > 0x3FFFFFFF, NF4B_ERR_UNSUPPORTED);
+  NF4B_RETURN_IF(at_slots(a->tokens, a->rows) * (2 + AT_PIECES) * a->heads > 0x3FFFFFFF, NF4B_ERR_UNSUPPORTED);
   if (a->tokens == 0) return NF4B_OK;
   NF4B_RETURN_IF(!a->q || !a->k || !a->v || !a->cu, NF4B_ERR_INVALID_ARG);
   NF4B_RETURN_IF(!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->cu, 4), NF4B_ERR_ALIGNMENT);
@@ -1112,9 +1090,9 @@ static int attn_tmap(CUtensorMap* m, const nf4b_attn& a, const void* base, int h
                          base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-static AttnParams attn_params(const nf4b_attn& a, int shift, int pair) {
-  return AttnParams{a.cu,    int32_t(a.tokens), a.rows, a.heads, a.kv_heads, a.head_dim, a.left,
-                    a.right, int32_t(at_slots(a.tokens, a.rows, shift)), shift, pair, a.scale};
+static AttnParams attn_params(const nf4b_attn& a) {
+  return AttnParams{a.cu,       int32_t(a.tokens), a.rows,  a.heads, a.kv_heads,
+                    a.head_dim, a.left,            a.right, int32_t(at_slots(a.tokens, a.rows)), a.scale};
 }
 
 // Dynamic shared memory of a kernel, set once per device.
@@ -1132,32 +1110,19 @@ static int attn_smem(K kernel, int bytes, bool (&done)[64]) {
   return NF4B_OK;
 }
 
-template <typename T, int DC, bool PAIR>
-static int attn_fwd_launch(const nf4b_attn& a, int kind, void* out, float* lse, cudaStream_t s) {
+template <typename T, int DC>
+static int attn_fwd_launch(const nf4b_attn& a, void* out, float* lse, cudaStream_t s) {
   CUtensorMap q, k, v;
   int st = attn_tmap(&q, a, a.q, a.heads, a.q_stride, a.q_head_stride, AT_TILE);
   if (st == NF4B_OK) st = attn_tmap(&k, a, a.k, a.kv_heads, a.k_stride, a.k_head_stride, AT_KEYS);
   if (st == NF4B_OK) st = attn_tmap(&v, a, a.v, a.kv_heads, a.v_stride, a.v_head_stride, AT_KEYS);
   static bool done[64] = {false};
-  if (st == NF4B_OK) st = attn_smem(attn_fwd_kernel<T, DC, PAIR>, AttnFwdSmem<DC, PAIR>::ALLOC, done);
+  if (st == NF4B_OK) st = attn_smem(attn_fwd_kernel<T, DC>, AttnFwdSmem<DC>::ALLOC, done);
   if (st != NF4B_OK) return st;
-  const AttnParams p = attn_params(a, kind == AT_TILES ? 8 : 7, kind);
-  const unsigned per_slot = unsigned(kind == AT_HEADS ? a.kv_heads * ((a.heads / a.kv_heads + 1) / 2) : a.heads);
-  NF4B_CUDA_TRY(launch_pdl(attn_fwd_kernel<T, DC, PAIR>, dim3(unsigned(p.slots) * per_slot), dim3(PAIR ? 320 : 192),
-                           size_t(AttnFwdSmem<DC, PAIR>::ALLOC), s, q, k, v, p, static_cast<T*>(out), lse));
+  const AttnParams p = attn_params(a);
+  NF4B_CUDA_TRY(launch_pdl(attn_fwd_kernel<T, DC>, dim3(unsigned(p.slots) * unsigned(a.heads)), dim3(AT_FWD_THREADS),
+                           size_t(AttnFwdSmem<DC>::ALLOC), s, q, k, v, p, static_cast<T*>(out), lse));
   return launch_status("attn_fwd_kernel launch");
-}
-
-template <typename T>
-static int attn_fwd_pick(const nf4b_attn& a, void* out, float* lse, cudaStream_t s) {
-  const int grp = a.heads / a.kv_heads;
-  bool pair = (double(a.tokens) / AT_TILE + 0.5 * a.rows) * a.heads > 148;
-  const char* e = std::getenv("STEW_ATTN_PAIR");
-  if (e) pair = e[0] == '1';
-  const int kind = !pair ? AT_SINGLE : grp > 1 ? AT_HEADS : AT_TILES;
-  if (a.head_dim > 64)
-    return pair ? attn_fwd_launch<T, 2, true>(a, kind, out, lse, s) : attn_fwd_launch<T, 2, false>(a, kind, out, lse, s);
-  return pair ? attn_fwd_launch<T, 1, true>(a, kind, out, lse, s) : attn_fwd_launch<T, 1, false>(a, kind, out, lse, s);
 }
 
 extern "C" int nf4b_attn_fwd(const nf4b_attn* args, void* out, float* lse, void* stream) {
@@ -1170,7 +1135,10 @@ extern "C" int nf4b_attn_fwd(const nf4b_attn* args, void* out, float* lse, void*
   st = check_device();
   if (st != NF4B_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return a.dtype == NF4B_F16 ? attn_fwd_pick<__half>(a, out, lse, s) : attn_fwd_pick<__nv_bfloat16>(a, out, lse, s);
+  const bool wide = a.head_dim > 64;
+  if (a.dtype == NF4B_F16)
+    return wide ? attn_fwd_launch<__half, 2>(a, out, lse, s) : attn_fwd_launch<__half, 1>(a, out, lse, s);
+  return wide ? attn_fwd_launch<__nv_bfloat16, 2>(a, out, lse, s) : attn_fwd_launch<__nv_bfloat16, 1>(a, out, lse, s);
 }
 
 extern "C" int nf4b_attn_error_flag(int* value, int reset) {
@@ -1210,7 +1178,7 @@ static int attn_split(const nf4b_attn& a) {
   double best_us = 0;
   for (int c = 1; c <= grp; ++c) {
     // (the shares' sums: 1 KB a key row, share and 128 features)
-    if (grp % c != 0 || (c > 1 && double(at_slots(a.tokens, a.rows, 7)) * a.kv_heads * c > 4096)) continue;
+    if (grp % c != 0 || (c > 1 && double(at_slots(a.tokens, a.rows)) * a.kv_heads * c > 4096)) continue;
     const double one = 3.0 + (c > 1 ? 2.0 : 0.0);
     const double keys = tiles * a.kv_heads * c * (one + 1.6 * mean * (grp / c));
     const double queries = tiles * a.heads * (3.0 + 1.2 * mean);
@@ -1227,7 +1195,7 @@ static int attn_split(const nf4b_attn& a) {
 }
 
 static int64_t attn_work(const nf4b_attn& a, int split, void* base, AttnWork* w) {
-  const int64_t slots = at_slots(a.tokens, a.rows, 7), pairs = slots * a.kv_heads;
+  const int64_t slots = at_slots(a.tokens, a.rows), pairs = slots * a.kv_heads;
   char* b = static_cast<char*>(base);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -1263,7 +1231,7 @@ static int attn_bwd_launch(const nf4b_attn& a, const void* out, const float* lse
   static bool done[64] = {false};
   if (st == NF4B_OK) st = attn_smem(attn_bwd_kernel<T, DC>, AttnBwdSmem<DC>::ALLOC, done);
   if (st != NF4B_OK) return st;
-  const AttnParams p = attn_params(a, 7, AT_SINGLE);
+  const AttnParams p = attn_params(a);
   AttnWork w;
   attn_work(a, split, work, &w);
   T *tq = static_cast<T*>(dq), *tk = static_cast<T*>(dk), *tv = static_cast<T*>(dv);

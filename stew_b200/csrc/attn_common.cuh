@@ -21,16 +21,14 @@ struct AttnParams {
   int32_t tokens, rows, heads, kv_heads, head_dim;
   int32_t left, right;
   int32_t slots;       // tile slots of the packed rows, at_slots()
-  int32_t shift;       // log2 of a slot's tokens
-  int32_t pair;        // forward: what a CTA's two query tiles are, AT_SINGLE ...
   float scale;
 };
 
-// Tiles never cross a sequence.  Sequence s owns the slots of N = 2^shift tokens from floor(start_s / N) + s
-// on: that many hold its tiles for any lengths (floor(b/N) - floor(a/N) + 1 >= ceil((b-a)/N)), so the
-// launch needs only the token and row counts, and a CTA finds its sequence by searching a strictly
-// ascending function of s.  Slots from that of s = rows on cover the rows behind the last sequence.
-inline int64_t at_slots(int64_t tokens, int64_t rows, int shift) { return (tokens >> shift) + rows + 1; }
+// Tiles never cross a sequence.  Sequence s owns the tile slots from floor(start_s / 128) + s on: that many
+// hold its tiles for any lengths (floor(b/128) - floor(a/128) + 1 >= ceil((b-a)/128)), so the launch needs
+// only the token and row counts, and a CTA finds its sequence by searching a strictly ascending function
+// of s.  Slots from that of s = rows on cover the rows behind the last sequence.
+inline int64_t at_slots(int64_t tokens, int64_t rows) { return tokens / AT_TILE + rows + 1; }
 
 struct AttnTile {
   int a, len;   // the sequence's first token and length
@@ -42,7 +40,7 @@ struct AttnTile {
 __device__ __forceinline__ int at_start(const AttnParams& p, int s) {
   return s == 0 ? 0 : min(max(__ldg(p.cu + s), 0), p.tokens);
 }
-__device__ __forceinline__ int at_first_slot(const AttnParams& p, int s) { return (at_start(p, s) >> p.shift) + s; }
+__device__ __forceinline__ int at_first_slot(const AttnParams& p, int s) { return (at_start(p, s) >> 7) + s; }
 
 // Whole warp; 32 probes a step (one step for up to 31 sequences).
 __device__ __forceinline__ AttnTile at_find(const AttnParams& p, int slot) {
@@ -59,7 +57,7 @@ __device__ __forceinline__ AttnTile at_find(const AttnParams& p, int slot) {
   t.tail = lo == p.rows;
   t.a = at_start(p, lo);
   t.len = (t.tail ? p.tokens : max(at_start(p, lo + 1), t.a)) - t.a;
-  t.i0 = (slot - ((t.a >> p.shift) + lo)) << p.shift;
+  t.i0 = (slot - ((t.a >> 7) + lo)) << 7;
   return t;
 }
 
