@@ -129,9 +129,12 @@ def allreduce_lora_grads(params, local_labels: float, group=None) -> float:
     return total
 
 
-def allreduce_lora_grads_device(params, local_labels: torch.Tensor, group=None) -> torch.Tensor:
+def allreduce_lora_grads_device(params, local_labels: torch.Tensor, group=None, max_norm: float | None = None):
     """allreduce_lora_grads with the count as a device tensor and no host synchronisation,
     so the exchange can be captured in a CUDA graph.  Returns the global count (device).
+
+    max_norm: also clip the normalised gradients to this global 2-norm, in the pass that divides
+    them by the count (clip_grads); the return value is then (global count, norm before clipping).
 
     The gradients are gathered into the flat buffer with one concatenation and written back
     and normalised with multi-tensor (foreach) kernels, so the step's ~100 adapter tensors
@@ -148,13 +151,26 @@ def allreduce_lora_grads_device(params, local_labels: torch.Tensor, group=None) 
         dist.all_reduce(flat, op=dist.ReduceOp.SUM, group=group)
         total = flat[-1:].clamp_min(1.0)
         body = flat[:-1]
+        views = [v.view_as(g) for v, g in zip(body.split([g.numel() for g in grads]), grads)]
+        if max_norm is not None:
+            return total, _clip_views(views, grads, max_norm, total)
         body.div_(total)
-        sizes = [g.numel() for g in grads]
-        torch._foreach_copy_(grads, [v.view_as(g) for v, g in zip(body.split(sizes), grads)])
+        torch._foreach_copy_(grads, views)
         return total
     total = count.clamp_min(1.0)
+    if max_norm is not None:
+        return total, clip_grads(grads, max_norm, divisor=total)
     torch._foreach_div_(grads, total.reshape(()))
     return total
+
+
+def _clip_views(views, grads, max_norm, total):
+    """grads <- the all-reduced fp32 views / total, clipped; returns the norm."""
+    if all(g.dtype == torch.float32 for g in grads):
+        return clip_grads(views, max_norm, divisor=total, out=grads)
+    norm = clip_grads(views, max_norm, divisor=total)  # in the buffer; the copy rounds to the gradients' types
+    torch._foreach_copy_(grads, views)
+    return norm
 
 
 class BucketedGradAllReduce:
@@ -224,9 +240,10 @@ class BucketedGradAllReduce:
                 dist.all_reduce(flat, op=dist.ReduceOp.SUM, group=self.group)
         self._launched[i] = True
 
-    def finish(self) -> torch.Tensor:
+    def finish(self, max_norm: float | None = None):
         """Join the exchange, normalise by the global labelled-token count, write the grads.
-        Returns the global count (device tensor)."""
+        Returns the global count (device tensor); with max_norm the gradients are also clipped to
+        that global 2-norm in the same pass, and the return value is (count, norm before clipping)."""
         for i, b in enumerate(self.buckets):  # a bucket whose grads never came: zeros
             if not self._launched[i]:
                 for p in b:
@@ -240,14 +257,18 @@ class BucketedGradAllReduce:
         for i, b in enumerate(self.buckets):
             n = self.flat[i].numel() - (1 if i == 0 else 0)
             body = self.flat[i][:n]
-            body.div_(total)
+            if max_norm is None:
+                body.div_(total)
             for p, v in zip(b, body.split([p.numel() for p in b])):
                 grads.append(p.grad)
                 views.append(v.view_as(p))
-        torch._foreach_copy_(grads, views)
+        if max_norm is None:
+            torch._foreach_copy_(grads, views)
+        else:
+            norm = _clip_views(views, grads, max_norm, total)
         self._ready = [0] * len(self.buckets)
         self._launched = [False] * len(self.buckets)
-        return total
+        return total if max_norm is None else (total, norm)
 
     def remove(self):
         for h in self._handles:

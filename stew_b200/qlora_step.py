@@ -6,14 +6,14 @@ LoRA adapter on q and v, run on packed token rows.
 Scope: the reference patches this model (transformers' Qwen2 under peft/bitsandbytes) and runs
 it on packed real tokens (solution/unpad.py:278-345).  The NF4 projections and the LoRA
 adapters are this library's kernels (fused unpack + tcgen05 GEMMs, forward and backward), and
-so are the layer's RMSNorm (fused with the residual add), RoPE and SwiGLU (step_ops, the
-counterparts of solution/rmsnorm.py, rope.py, swiglu.py); attention is torch's variable-length
-flash attention over the packed rows, and the tied LM head + cross-entropy are torch.  Weights
+so are the layer's RMSNorm (fused with the residual add), RoPE, SwiGLU and the attention over the
+packed rows, forward and backward (step_ops, the counterparts of solution/rmsnorm.py, rope.py,
+swiglu.py and unpad.py's per-row attention); the tied LM head's GEMMs are torch.  Weights
 are random (seeded) and NF4-quantized on the GPU: no checkpoint is used.
 
 `train_step` = forward on the packed rows, backward (LoRA grads only: base weights, norms and
 embedding are frozen), one all-reduce of the LoRA grads across data-parallel ranks
-(stew_b200.dp), AdamW on the adapters.
+(stew_b200.dp), optionally clipping to a global norm, AdamW on the adapters.
 """
 from __future__ import annotations
 
@@ -25,7 +25,8 @@ import torch.nn.functional as F
 
 from . import dp
 from .lora import LORA_RANK, NF4Linear, NF4LoraLinear, grouped_projection, nf4_mlp
-from .step_ops import add_rms_norm, head_cross_entropy, rms_norm, rope_qk
+from .step_ops import (add_rms_norm, head_cross_entropy, packed_attention, packed_attention_supported, rms_norm,
+                       rope_qk)
 from .sweep import QWEN_PROJ, qwen_model_weights
 
 
@@ -70,11 +71,14 @@ def rope_tables(positions: torch.Tensor, head_dim: int, theta: float):
 
 def packed_causal_attention(q, k, v, rows):
     """Causal attention inside each packed row: q [N, H, D], k/v [N, KH, D] (grouped-query
-    heads, H a multiple of KH), rows = (cu_seqlens int32 [B+1], longest row).  The
-    variable-length flash kernel sees only the real tokens, no [N, N] mask, and reads the
-    shared k/v heads directly (no expanded copies, no head-sum in the backward)."""
-    from torch.nn.attention.varlen import varlen_attn
+    heads, H a multiple of KH), rows = (cu_seqlens int32 [B+1], longest row).  The kernels see
+    only the real tokens, no [N, N] mask, and read the shared k/v heads directly (no expanded
+    copies, no head-sum in the backward): step_ops.packed_attention for its types and head sizes,
+    torch's variable-length attention for others."""
     cu, longest = rows
+    if packed_attention_supported(q):
+        return packed_attention(q, k, v, cu)
+    from torch.nn.attention.varlen import varlen_attn
     return varlen_attn(q, k, v, cu, cu, longest, longest, window_size=(-1, 0))
 
 
@@ -253,6 +257,10 @@ def synthetic_batch(batch: int = 4, seq: int = 512, vocab: int = 151936, mean_fr
 class QLoRATrainer:
     """One QLoRA step per call: forward, backward, LoRA-grad all-reduce, AdamW.
 
+    max_grad_norm: clip the normalised LoRA gradients to this global 2-norm before AdamW (one pass
+    with the division by the label count, dp.clip_grads); `grad_norm` then holds the last step's
+    norm before clipping (0-d device tensor; read it before the next step).
+
     cuda_graph=True captures the whole step (forward, backward, the all-reduce and AdamW) in
     one CUDA graph per packed-batch shape and replays it: the step's ~3,000 kernel launches
     cost one graph launch on the host.  The packed batch is copied into the graph's static
@@ -261,7 +269,11 @@ class QLoRATrainer:
     call is exactly one optimizer step."""
 
     def __init__(self, model: QwenQLoRA, lr: float = 2e-4, group=None, cuda_graph: bool = False,
-                 buckets: int = 4, buckets_on_one_rank: bool = False):
+                 buckets: int = 4, buckets_on_one_rank: bool = False, max_grad_norm: float | None = None):
+        if max_grad_norm is not None and not max_grad_norm >= 0.0:
+            raise ValueError(f"max_grad_norm must be >= 0, got {max_grad_norm}")
+        self.max_grad_norm = max_grad_norm
+        self.grad_norm = None
         self.model = model
         self.params = model.lora_parameters()
         self.cuda_graph = cuda_graph
@@ -289,13 +301,31 @@ class QLoRATrainer:
         if self._reducer is not None:
             self._reducer.count = torch.full((1,), float(pb.n_labels), device=pb.ids.device)
             loss_sum.backward()
-            total = float(self._reducer.finish())
+            total = float(self._finish())
         else:
             loss_sum.backward()
-            total = dp.allreduce_lora_grads(self.params, pb.n_labels, self.group)
+            if self.max_grad_norm is None:
+                total = dp.allreduce_lora_grads(self.params, pb.n_labels, self.group)
+            else:
+                n_lab = torch.full((1,), float(pb.n_labels), device=pb.ids.device)
+                total = float(self._exchange(n_lab))
         self.opt.step()
         self.opt.zero_grad(set_to_none=True)
         return loss_sum.detach(), total
+
+    def _finish(self):
+        """The bucketed exchange's end; returns the global count."""
+        if self.max_grad_norm is None:
+            return self._reducer.finish()
+        total, self.grad_norm = self._reducer.finish(self.max_grad_norm)
+        return total
+
+    def _exchange(self, n_lab):
+        """The exchange in one buffer, on the device; returns the global count."""
+        if self.max_grad_norm is None:
+            return dp.allreduce_lora_grads_device(self.params, n_lab, self.group)
+        total, self.grad_norm = dp.allreduce_lora_grads_device(self.params, n_lab, self.group, self.max_grad_norm)
+        return total
 
     def _graph_body(self):
         loss = self.model.forward_packed(self._pb)
@@ -305,9 +335,9 @@ class QLoRATrainer:
         # keep no reference to this autograd graph: a later capture must not reuse its nodes
         self._loss = loss.detach()
         if self._reducer is not None:
-            self._total = self._reducer.finish()
+            self._total = self._finish()
         else:
-            self._total = dp.allreduce_lora_grads_device(self.params, self._n_lab, self.group)
+            self._total = self._exchange(self._n_lab)
         self.opt.step()
 
     def _capture(self, pb):
