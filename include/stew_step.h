@@ -91,11 +91,13 @@ typedef struct nf4b_attn {
   float scale;           /* > 0 */
 } nf4b_attn;
 
-/* out [tokens, heads, head_dim] contiguous, of q's type; lse fp32 [heads, tokens] (natural log).
- * Tokens at and behind cu[rows] get zeros (lse -inf).  */
-int nf4b_attn_fwd(const nf4b_attn* a, void* out, float* lse, void* stream);
+/* out [tokens, heads, head_dim] contiguous, of q's type; lse fp32 [heads, tokens] (natural log);
+ * rest (NULL: not wanted): what out's rounding left of the output, again in q's type, for the
+ * backward's do.o.  Tokens at and behind cu[rows] get zeros (lse -inf).  */
+int nf4b_attn_fwd(const nf4b_attn* a, void* out, void* rest, float* lse, void* stream);
 
-/* Gradients from dout, out (contiguous, as nf4b_attn_fwd wrote it) and lse:
+/* Gradients from dout, out, rest (contiguous, as nf4b_attn_fwd wrote them; rest may be NULL: do.o is
+ * then taken from the rounded output, whose error all of a row's ds share) and lse:
  *   dv_j = sum_i p_ij do_i,   ds_ij = p_ij (do_i.v_j - do_i.o_i),
  *   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,
  * k's and v's summed over the query heads that share them.  The probabilities are recomputed
@@ -104,8 +106,8 @@ int nf4b_attn_fwd(const nf4b_attn* a, void* out, float* lse, void* stream);
  * tokens at and behind cu[rows] get zeros.  work: nf4b_attn_bwd_work_bytes(a) bytes of device
  * scratch, 16-byte aligned, of any content; -1 for a call that would be refused.  */
 int64_t nf4b_attn_bwd_work_bytes(const nf4b_attn* a);
-int nf4b_attn_bwd(const nf4b_attn* a, const void* out, const float* lse, const void* dout, void* dq,
-                  void* dk, void* dv, void* work, int64_t work_bytes, void* stream);
+int nf4b_attn_bwd(const nf4b_attn* a, const void* out, const void* rest, const float* lse, const void* dout,
+                  void* dq, void* dk, void* dv, void* work, int64_t work_bytes, void* stream);
 
 /* Reads (and with reset != 0 clears) the device-side flag the attention kernels set when a pipeline
  * wait ran out of time (the kernel then ends early instead of hanging).  0 = no timeout since the

@@ -130,9 +130,9 @@ SIGNATURES = {
     "nf4b_ce_fwd": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p]),
     "nf4b_ce_bwd": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p]),
     # (the first argument is an nf4b_attn as a packed record)
-    "nf4b_attn_fwd": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p]),
+    "nf4b_attn_fwd": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "nf4b_attn_bwd_work_bytes": (c_int64, [c_void_p]),
-    "nf4b_attn_bwd": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+    "nf4b_attn_bwd": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                 c_void_p, c_void_p, c_int64, c_void_p]),
     "nf4b_attn_error_flag": (c_int32, [ctypes.POINTER(c_int32), c_int32]),
     "nf4b_clip_grads_work_bytes": (c_int64, [c_int32]),

@@ -51,7 +51,7 @@ template <typename T, int DC>
 __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttnParams p, T* __restrict__ out,
-                    float* __restrict__ lse) {
+                    T* __restrict__ rest, float* __restrict__ lse) {
   using L = AttnFwdSmem<DC>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -82,7 +82,9 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
     const int n = min(AT_TILE, t.len - t.i0), vec = p.head_dim / 8;
     for (int i = threadIdx.x; i < n * vec; i += AT_FWD_THREADS) {
       const int64_t row = t.a + t.i0 + i / vec;
-      *reinterpret_cast<uint4*>(out + (row * p.heads + h) * p.head_dim + (i % vec) * 8) = make_uint4(0, 0, 0, 0);
+      const int64_t off = (row * p.heads + h) * p.head_dim + (i % vec) * 8;
+      *reinterpret_cast<uint4*>(out + off) = make_uint4(0, 0, 0, 0);
+      if (rest != nullptr) *reinterpret_cast<uint4*>(rest + off) = make_uint4(0, 0, 0, 0);
     }
     if (threadIdx.x < n) lse[int64_t(h) * p.tokens + t.a + t.i0 + threadIdx.x] = -INFINITY;
     return;
@@ -272,6 +274,9 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
       // every MMA is done: the Q tile's memory is free
       at_store_rows<T, DC * 64>(t_o, smem + L::Q + w0 * DC * 128, out + (row * p.heads + h) * p.head_dim,
                                 int64_t(p.heads) * p.head_dim, t.len - t.i0 - w0, p.head_dim, inv);
+      if (rest != nullptr)
+        at_store_rows<T, DC * 64, true>(t_o, smem + L::Q + w0 * DC * 128, rest + (row * p.heads + h) * p.head_dim,
+                                        int64_t(p.heads) * p.head_dim, t.len - t.i0 - w0, p.head_dim, inv);
       if (i < t.len) lse[int64_t(h) * p.tokens + row + lane] = l == 0.f ? -INFINITY : m * p.scale + logf(l);
     }
     tc_fence_before();
@@ -282,7 +287,8 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
 
 // ------------------------------------------------------------------ backward
 // Two launches.  The first (attn_prep_kernel) writes, per (head, token), the row's log-sum-exp in
-// log2 units and delta = do.o, and zeros behind the last sequence.  The second's persistent CTAs work on two
+// log2 units and delta = do.o (o with what its rounding left, where the forward kept that), and zeros behind
+// the last sequence.  The second's persistent CTAs work on two
 // kinds of units with one structure, a resident pair of 128-token tiles X, Y against a ring of tile pairs
 // A, B (D = head_dim):
 //   keys    : X = K, Y = V of a key tile; A = Q, B = dO over the query tiles of the group's heads (or a share
@@ -326,7 +332,8 @@ __device__ __forceinline__ float at_half_warp_sum(float v) {
 // head) read V.
 template <typename T>
 __global__ void __launch_bounds__(AT_PREP_THREADS)
-    attn_prep_kernel(const __grid_constant__ AttnParams p, const T* __restrict__ out, const T* __restrict__ dout,
+    attn_prep_kernel(const __grid_constant__ AttnParams p, const T* __restrict__ out, const T* __restrict__ rest,
+                     const T* __restrict__ dout,
                      const float* __restrict__ lse, const T* __restrict__ v, int64_t v_stride, int64_t v_head_stride,
                      AttnWork w, T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dv) {
   grid_dep_wait();  // programmatic launch: no global access before the wait
@@ -360,11 +367,11 @@ __global__ void __launch_bounds__(AT_PREP_THREADS)
     return;
   }
   if (keys && !SCALED) return;
-  uint4 x4[N], d4[N];  // every load under way before the first sum
+  uint4 x4[N], y4[N], d4[N];  // every load under way before the first sum
   float l[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) {
-    x4[k] = d4[k] = make_uint4(0, 0, 0, 0);
+    x4[k] = y4[k] = d4[k] = make_uint4(0, 0, 0, 0);
     l[k] = 0.f;
     const int64_t row = row0 + k * STEP;
     if (!live(k)) continue;
@@ -374,6 +381,7 @@ __global__ void __launch_bounds__(AT_PREP_THREADS)
       const int64_t off = (row * p.heads + h) * p.head_dim + f;
       x4[k] = *reinterpret_cast<const uint4*>(out + off);
       d4[k] = *reinterpret_cast<const uint4*>(dout + off);
+      if (rest != nullptr) y4[k] = *reinterpret_cast<const uint4*>(rest + off);
       if (sub == 0) l[k] = lse[int64_t(h) * p.tokens + row];
     }
   }
@@ -381,12 +389,13 @@ __global__ void __launch_bounds__(AT_PREP_THREADS)
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     const uint32_t* x = reinterpret_cast<const uint32_t*>(&x4[k]);
+    const uint32_t* y = reinterpret_cast<const uint32_t*>(&y4[k]);
     const uint32_t* d = reinterpret_cast<const uint32_t*>(keys ? &x4[k] : &d4[k]);
     float dot = 0.f, nd = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 a = at_unpack<T>(x[i]), b = at_unpack<T>(d[i]);
-      dot = fmaf(a.x, b.x, fmaf(a.y, b.y, dot));
+      const float2 a = at_unpack<T>(x[i]), c = at_unpack<T>(y[i]), b = at_unpack<T>(d[i]);
+      dot = fmaf(a.x + c.x, b.x, fmaf(a.y + c.y, b.y, dot));
       nd = fmaf(b.x, b.x, fmaf(b.y, b.y, nd));
     }
     if (!keys) {
@@ -1111,7 +1120,7 @@ static int attn_smem(K kernel, int bytes, bool (&done)[64]) {
 }
 
 template <typename T, int DC>
-static int attn_fwd_launch(const nf4b_attn& a, void* out, float* lse, cudaStream_t s) {
+static int attn_fwd_launch(const nf4b_attn& a, void* out, void* rest, float* lse, cudaStream_t s) {
   CUtensorMap q, k, v;
   int st = attn_tmap(&q, a, a.q, a.heads, a.q_stride, a.q_head_stride, AT_TILE);
   if (st == NF4B_OK) st = attn_tmap(&k, a, a.k, a.kv_heads, a.k_stride, a.k_head_stride, AT_KEYS);
@@ -1121,24 +1130,24 @@ static int attn_fwd_launch(const nf4b_attn& a, void* out, float* lse, cudaStream
   if (st != NF4B_OK) return st;
   const AttnParams p = attn_params(a);
   NF4B_CUDA_TRY(launch_pdl(attn_fwd_kernel<T, DC>, dim3(unsigned(p.slots) * unsigned(a.heads)), dim3(AT_FWD_THREADS),
-                           size_t(AttnFwdSmem<DC>::ALLOC), s, q, k, v, p, static_cast<T*>(out), lse));
+                           size_t(AttnFwdSmem<DC>::ALLOC), s, q, k, v, p, static_cast<T*>(out), static_cast<T*>(rest), lse));
   return launch_status("attn_fwd_kernel launch");
 }
 
-extern "C" int nf4b_attn_fwd(const nf4b_attn* args, void* out, float* lse, void* stream) {
+extern "C" int nf4b_attn_fwd(const nf4b_attn* args, void* out, void* rest, float* lse, void* stream) {
   nf4b_attn a;
   int st = attn_checks(args, &a);
   if (st != NF4B_OK) return st;
   if (a.tokens == 0) return NF4B_OK;
   NF4B_RETURN_IF(!out || !lse, NF4B_ERR_INVALID_ARG);
-  NF4B_RETURN_IF(!aligned(out, 16) || !aligned(lse, 16), NF4B_ERR_ALIGNMENT);
+  NF4B_RETURN_IF(!aligned(out, 16) || !aligned(rest, 16) || !aligned(lse, 16), NF4B_ERR_ALIGNMENT);
   st = check_device();
   if (st != NF4B_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool wide = a.head_dim > 64;
   if (a.dtype == NF4B_F16)
-    return wide ? attn_fwd_launch<__half, 2>(a, out, lse, s) : attn_fwd_launch<__half, 1>(a, out, lse, s);
-  return wide ? attn_fwd_launch<__nv_bfloat16, 2>(a, out, lse, s) : attn_fwd_launch<__nv_bfloat16, 1>(a, out, lse, s);
+    return wide ? attn_fwd_launch<__half, 2>(a, out, rest, lse, s) : attn_fwd_launch<__half, 1>(a, out, rest, lse, s);
+  return wide ? attn_fwd_launch<__nv_bfloat16, 2>(a, out, rest, lse, s) : attn_fwd_launch<__nv_bfloat16, 1>(a, out, rest, lse, s);
 }
 
 extern "C" int nf4b_attn_error_flag(int* value, int reset) {
@@ -1221,7 +1230,7 @@ extern "C" int64_t nf4b_attn_bwd_work_bytes(const nf4b_attn* args) {
 }
 
 template <typename T, int DC>
-static int attn_bwd_launch(const nf4b_attn& a, const void* out, const float* lse, const void* dout, void* dq, void* dk,
+static int attn_bwd_launch(const nf4b_attn& a, const void* out, const void* rest, const float* lse, const void* dout, void* dq, void* dk,
                            void* dv, void* work, int split, cudaStream_t s) {
   AttnBwdMaps m;
   int st = attn_tmap(&m.q, a, a.q, a.heads, a.q_stride, a.q_head_stride, AT_TILE);
@@ -1237,7 +1246,7 @@ static int attn_bwd_launch(const nf4b_attn& a, const void* out, const float* lse
   T *tq = static_cast<T*>(dq), *tk = static_cast<T*>(dk), *tv = static_cast<T*>(dv);
   NF4B_CUDA_TRY(launch_pdl(attn_prep_kernel<T>, dim3(unsigned(p.slots) * unsigned(a.heads + a.kv_heads)),
                            dim3(AT_PREP_THREADS),
-                           size_t(0), s, p, static_cast<const T*>(out), static_cast<const T*>(dout), lse,
+                           size_t(0), s, p, static_cast<const T*>(out), static_cast<const T*>(rest), static_cast<const T*>(dout), lse,
                            static_cast<const T*>(a.v), a.v_stride, a.v_head_stride, w, tq, tk, tv));
   const int64_t units = int64_t(p.slots) * (int64_t(a.kv_heads) * (split > 1 ? split + AT_PIECES : 1) + a.heads);
   const int64_t sms = attn_sms();
@@ -1246,14 +1255,14 @@ static int attn_bwd_launch(const nf4b_attn& a, const void* out, const float* lse
   return launch_status("attn_bwd_kernel launch");
 }
 
-extern "C" int nf4b_attn_bwd(const nf4b_attn* args, const void* out, const float* lse, const void* dout, void* dq,
-                             void* dk, void* dv, void* work, int64_t work_bytes, void* stream) {
+extern "C" int nf4b_attn_bwd(const nf4b_attn* args, const void* out, const void* rest, const float* lse,
+                             const void* dout, void* dq, void* dk, void* dv, void* work, int64_t work_bytes, void* stream) {
   nf4b_attn a;
   int st = attn_checks(args, &a);
   if (st != NF4B_OK) return st;
   if (a.tokens == 0) return NF4B_OK;
   NF4B_RETURN_IF(!out || !lse || !dout || !dq || !dk || !dv || !work, NF4B_ERR_INVALID_ARG);
-  NF4B_RETURN_IF(!aligned(out, 16) || !aligned(lse, 16) || !aligned(dout, 16) || !aligned(dq, 16) || !aligned(dk, 16) ||
+  NF4B_RETURN_IF(!aligned(out, 16) || !aligned(rest, 16) || !aligned(lse, 16) || !aligned(dout, 16) || !aligned(dq, 16) || !aligned(dk, 16) ||
                      !aligned(dv, 16) || !aligned(work, 16),
                  NF4B_ERR_ALIGNMENT);
   const int split = attn_split(a);
@@ -1263,8 +1272,8 @@ extern "C" int nf4b_attn_bwd(const nf4b_attn* args, const void* out, const float
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool wide = a.head_dim > 64;
   if (a.dtype == NF4B_F16)
-    return wide ? attn_bwd_launch<__half, 2>(a, out, lse, dout, dq, dk, dv, work, split, s)
-                : attn_bwd_launch<__half, 1>(a, out, lse, dout, dq, dk, dv, work, split, s);
-  return wide ? attn_bwd_launch<__nv_bfloat16, 2>(a, out, lse, dout, dq, dk, dv, work, split, s)
-              : attn_bwd_launch<__nv_bfloat16, 1>(a, out, lse, dout, dq, dk, dv, work, split, s);
+    return wide ? attn_bwd_launch<__half, 2>(a, out, rest, lse, dout, dq, dk, dv, work, split, s)
+                : attn_bwd_launch<__half, 1>(a, out, rest, lse, dout, dq, dk, dv, work, split, s);
+  return wide ? attn_bwd_launch<__nv_bfloat16, 2>(a, out, rest, lse, dout, dq, dk, dv, work, split, s)
+              : attn_bwd_launch<__nv_bfloat16, 1>(a, out, rest, lse, dout, dq, dk, dv, work, split, s);
 }

@@ -218,11 +218,19 @@ __device__ __forceinline__ void at_hide(int lo, int hi, F kill) {
   }
 }
 
+// What is left of v after its rounding to T.
+template <typename T>
+__device__ __forceinline__ float at_rest(float v) {
+  const float2 r = at_unpack<T>(at_pack<T>(v, 0.f));
+  return v - r.x;
+}
+
 // Whole warp: `cols` fp32 columns (a multiple of 8, at most MAX) from TMEM column `taddr` on of the warp's 32
 // rows, row r times its thread's f, rounded to T and written to out + r * stride for r < rows.  The rows pass
 // through `buf` (32 x 2 MAX bytes of shared memory, the 16-byte pieces of a row permuted by its number against
-// bank conflicts), so that a warp writes whole rows instead of 16 bytes of each of 32.
-template <typename T, int MAX>
+// bank conflicts), so that a warp writes whole rows instead of 16 bytes of each of 32.  REST: what the rounding
+// left, instead.
+template <typename T, int MAX, bool REST = false>
 __device__ __forceinline__ void at_store_rows(uint32_t taddr, uint8_t* buf, T* out, int64_t stride, int rows, int cols, float f) {
   const int lane = threadIdx.x & 31;
   constexpr int VEC = MAX / 8;  // 16-byte pieces of a row: 4, 8 or 16
@@ -238,8 +246,10 @@ __device__ __forceinline__ void at_store_rows(uint32_t taddr, uint8_t* buf, T* o
       uint4 v;
       uint32_t* w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        w[e] = at_pack<T>(__uint_as_float(o[k * 8 + 2 * e]) * f, __uint_as_float(o[k * 8 + 2 * e + 1]) * f);
+      for (int e = 0; e < 4; ++e) {
+        const float a = __uint_as_float(o[k * 8 + 2 * e]) * f, b = __uint_as_float(o[k * 8 + 2 * e + 1]) * f;
+        w[e] = REST ? at_pack<T>(at_rest<T>(a), at_rest<T>(b)) : at_pack<T>(a, b);
+      }
       *reinterpret_cast<uint4*>(place(lane, c / 8 + k)) = v;
     }
   }

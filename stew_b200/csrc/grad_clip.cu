@@ -154,7 +154,7 @@ __device__ __forceinline__ void gc_scale_chunk(const T* src, T* dst, int n, floa
     T* x = reinterpret_cast<T*>(&v[k]);
 #pragma unroll
     for (int e = 0; e < V; ++e) x[e] = gc_from_f<T>(gc_to_f(x[e]) * f);
-    if (i < nv) to[i] = v[k];
+    if (i < nv) __stcs(to + i, v[k]);
   }
   const int rest = n - nv * V;
   if (threadIdx.x < rest) {

@@ -189,44 +189,45 @@ def _attn_record(q, qs, k, ks, v, vs, cu, left, right, scale) -> bytes:
                              cu.numel() - 1, hq, k.shape[1], d, _ATTN_DTYPE[q.dtype], left, right, scale)
 
 
-def _attn_forward(q, k, v, cu, left, right, scale):
-    """(out, lse, q, k, v as read, the call's nf4b_attn record)."""
+def _attn_forward(q, k, v, cu, left, right, scale, keep_rest=False):
+    """(out, what its rounding left or None, lse, q, k, v as read, the call's nf4b_attn record)."""
     q, *qs = _attn_layout(q)
     k, *ks = _attn_layout(k)
     v, *vs = _attn_layout(v)
-    n, hq, _ = q.shape
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((hq, n), dtype=torch.float32, device=q.device)
+    shape, dt, dev = q.shape, q.dtype, q.device
+    out = torch.empty(shape, dtype=dt, device=dev)
+    rest = torch.empty(shape, dtype=dt, device=dev) if keep_rest else None
+    lse = torch.empty((shape[1], shape[0]), dtype=torch.float32, device=dev)
     rec = _attn_record(q, qs, k, ks, v, vs, cu, left, right, scale)
-    if n:
-        _launch(_lib.lib().nf4b_attn_fwd, "nf4b_attn_fwd", q.device, rec, out.data_ptr(), lse.data_ptr())
-    return out, lse, q, k, v, rec
+    if shape[0]:
+        _launch(_lib.lib().nf4b_attn_fwd, "nf4b_attn_fwd", dev, rec, out.data_ptr(),
+                rest.data_ptr() if keep_rest else None, lse.data_ptr())
+    return out, rest, lse, q, k, v, rec
 
 
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu, left, right, scale):
-        out, lse, q, k, v, ctx.rec = _attn_forward(q, k, v, cu, left, right, scale)
-        ctx.save_for_backward(q, k, v, cu, out, lse)
+        out, rest, lse, q, k, v, ctx.rec = _attn_forward(q, k, v, cu, left, right, scale, True)
+        ctx.save_for_backward(q, k, v, cu, out, rest, lse)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, cu, out, lse = ctx.saved_tensors
+        q, k, v, _, out, rest, lse = ctx.saved_tensors
         dev, dt = q.device, q.dtype
-        n = q.shape[0]
         dout = _aligned_c(dout if dout.dtype == dt else dout.to(dt))
         dq = torch.empty(q.shape, dtype=dt, device=dev)
         dk = torch.empty(k.shape, dtype=dt, device=dev)
-        dv = torch.empty(v.shape, dtype=dt, device=dev)
-        if n:
+        dv = torch.empty(k.shape, dtype=dt, device=dev)
+        if q.shape[0]:
             L = _lib.lib()
+            # the record's addresses are those of the saved tensors, which the graph keeps alive
             wb = L.nf4b_attn_bwd_work_bytes(ctx.rec)
             work = torch.empty(wb, dtype=torch.uint8, device=dev)
-            # the record's addresses are those of the saved tensors, which the graph keeps alive
-            _launch(L.nf4b_attn_bwd, "nf4b_attn_bwd", dev, ctx.rec, out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
-                    dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), work.data_ptr(), wb)
+            _launch(L.nf4b_attn_bwd, "nf4b_attn_bwd", dev, ctx.rec, out.data_ptr(), rest.data_ptr(), lse.data_ptr(),
+                    dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), work.data_ptr(), wb)
         return dq, dk, dv, None, None, None, None
 
 
@@ -248,8 +249,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torc
     1 / sqrt(D).
     Returns [N, Hq, D]; tokens behind cu[B] get zeros, and zero gradients.  Any strides with
     contiguous features are read in place when they are multiples of 8 elements, else copied.
-    The backward recomputes the probabilities from the saved log-sum-exp; forward and backward
-    give the same bits on every run.  Second derivatives are refused."""
+    The backward recomputes the probabilities from the saved log-sum-exp; beside the output it
+    keeps what the output's rounding left (a second tensor of its size), from which the rows'
+    do.o are exact.  Forward and backward give the same bits on every run.  Second derivatives are
+    refused."""
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError("packed_attention: q, k and v must be [tokens, heads, head_dim]")
     if not (q.dtype == k.dtype == v.dtype and q.device == k.device == v.device):

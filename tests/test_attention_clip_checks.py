@@ -34,27 +34,28 @@ def test_attention_entry_refuses(change, status):
     from stew_b200 import _lib
     L = _lib.lib()
     a, want = _attn(**change), getattr(_lib, "NF4B_ERR_" + status)
-    assert L.nf4b_attn_fwd(ctypes.byref(a), 256, 256, None) == want
-    assert L.nf4b_attn_bwd(ctypes.byref(a), 256, 256, 256, 256, 256, 256, 256, 1 << 30, None) == want
+    assert L.nf4b_attn_fwd(ctypes.byref(a), 256, None, 256, None) == want
+    assert L.nf4b_attn_bwd(ctypes.byref(a), 256, None, 256, 256, 256, 256, 256, 256, 1 << 30, None) == want
 
 
 def test_attention_entry_refuses_buffers():
     from stew_b200 import _lib
     L = _lib.lib()
     a = ctypes.byref(_attn())
-    assert L.nf4b_attn_fwd(None, 256, 256, None) == _lib.NF4B_ERR_INVALID_ARG
-    assert L.nf4b_attn_fwd(a, None, 256, None) == _lib.NF4B_ERR_INVALID_ARG
-    assert L.nf4b_attn_fwd(a, 264, 256, None) == _lib.NF4B_ERR_ALIGNMENT
+    assert L.nf4b_attn_fwd(None, 256, None, 256, None) == _lib.NF4B_ERR_INVALID_ARG
+    assert L.nf4b_attn_fwd(a, None, None, 256, None) == _lib.NF4B_ERR_INVALID_ARG
+    assert L.nf4b_attn_fwd(a, 264, None, 256, None) == _lib.NF4B_ERR_ALIGNMENT
+    assert L.nf4b_attn_fwd(a, 256, 264, 256, None) == _lib.NF4B_ERR_ALIGNMENT
     need = L.nf4b_attn_bwd_work_bytes(a)
     assert need >= 10 * 4 * 8
     for bad in (dict(kv_heads=3), dict(tokens=-1), dict(head_dim=60), dict(k_stride=4)):
         assert L.nf4b_attn_bwd_work_bytes(ctypes.byref(_attn(**bad))) == -1
     assert L.nf4b_attn_bwd_work_bytes(None) == -1
-    assert L.nf4b_attn_bwd(a, 256, 256, 256, 256, 256, 256, 256, need - 1, None) == _lib.NF4B_ERR_INVALID_ARG
-    assert L.nf4b_attn_bwd(a, 256, 256, 256, 256, 256, 256, None, need, None) == _lib.NF4B_ERR_INVALID_ARG
-    assert L.nf4b_attn_bwd(a, 256, 256, 256, 256, 264, 256, 256, need, None) == _lib.NF4B_ERR_ALIGNMENT
+    assert L.nf4b_attn_bwd(a, 256, None, 256, 256, 256, 256, 256, 256, need - 1, None) == _lib.NF4B_ERR_INVALID_ARG
+    assert L.nf4b_attn_bwd(a, 256, None, 256, 256, 256, 256, 256, None, need, None) == _lib.NF4B_ERR_INVALID_ARG
+    assert L.nf4b_attn_bwd(a, 256, None, 256, 256, 256, 264, 256, 256, need, None) == _lib.NF4B_ERR_ALIGNMENT
     none = ctypes.byref(_attn(tokens=0, q=None, k=None, v=None, cu=None))
-    assert L.nf4b_attn_fwd(none, None, None, None) == _lib.NF4B_OK
+    assert L.nf4b_attn_fwd(none, None, None, None, None) == _lib.NF4B_OK
 
 
 def test_packed_attention_refuses():
