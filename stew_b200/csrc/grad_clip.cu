@@ -1,11 +1,16 @@
 // Global 2-norm of a list of gradients and clipping (C ABI include/stew_step.h):
 //   norm = sqrt(sum src^2) / divisor,   dst = src (1 / divisor) min(1, max_norm / (norm + 1e-6))
 //
-// Two launches: the list is cut into chunks of 16 KB, every CTA takes a contiguous run of them.  The first launch writes one 64-bit sum of squares per CTA; every CTA of
-// the second adds those sums up in the same order (so all of them use the same bits), forms the
-// factor and scales its run, last chunk first: what the first launch read last is still in the
-// 126 MB L2.  The tensors' pointers travel in the kernel's parameters, so a call needs no copy to
-// the device and can be captured; longer lists take several launches.
+// Two launches: the list is cut into chunks of 16 KB, every CTA takes a contiguous run of them.  The first
+// launch writes one 64-bit sum of squares per CTA; every CTA of the second adds those sums up in the same
+// order (so all of them use the same bits), forms the factor and scales its run.  The tensors' pointers
+// travel in the kernel's parameters, so a call needs no copy to the device and can be captured; longer lists
+// take several launches.
+//
+// Bound by memory: the list is read twice and written once (a list under the limit, in place, is read
+// once).  187 M bf16 values, out of place: 190 us, 5.9 TB/s of 6.5 measured for a copy.  Scaling from the
+// end of each run (to find what the first launch read last in the L2), stores that leave the L2 first and
+// fetching a chunk ahead all measured the same.  A step's 112 adapters (8.7 MB fp32, in the L2): 8.5 us.
 //
 // Squares are summed in 64 bits: a 32-bit sum overflows from |g| = 1.8e19 and drifts over a long
 // list.  A 16-bit value's square is exact in 32 bits, so two of them are added there (one
@@ -154,7 +159,7 @@ __device__ __forceinline__ void gc_scale_chunk(const T* src, T* dst, int n, floa
     T* x = reinterpret_cast<T*>(&v[k]);
 #pragma unroll
     for (int e = 0; e < V; ++e) x[e] = gc_from_f<T>(gc_to_f(x[e]) * f);
-    if (i < nv) __stcs(to + i, v[k]);
+    if (i < nv) to[i] = v[k];
   }
   const int rest = n - nv * V;
   if (threadIdx.x < rest) {
@@ -225,9 +230,9 @@ __global__ void __launch_bounds__(GC_THREADS, GC_SCALE_CTAS / 148)
   __syncthreads();
   const float f = s_factor;
   const int c0 = gc_first(l.chunks, blockIdx.x), c1 = gc_first(l.chunks, blockIdx.x + 1);
-  int g = c0 < c1 ? gc_find(l, c1 - 1) : 0;
-  for (int c = c1 - 1; c >= c0; --c) {
-    while (l.it[g].chunk0 > c) --g;
+  int g = c0 < c1 ? gc_find(l, c0) : 0;
+  for (int c = c0; c < c1; ++c) {
+    while (g + 1 < l.n && l.it[g + 1].chunk0 <= c) ++g;
     const GcItem& it = l.it[g];
     if (it.dst == nullptr || (it.dst == it.src && f == 1.f)) continue;
     gc_chunk(it, c, [&](auto* src, auto* dst, int n) { gc_scale_chunk(src, dst, n, f); });
