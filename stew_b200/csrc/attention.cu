@@ -498,8 +498,9 @@ __device__ __forceinline__ float4* at_part(float* parts, int join, int split, in
 // Persistent: every CTA takes units from a counter, the longest kind first (key tiles with a group's heads;
 // of a causal sequence the first key tiles, which the most queries see, and the last query tiles; then the
 // sums over shares), so that the next unit's tiles are on their way and its first scores done while this
-// unit's sums are stored.  A sum waits for its shares; they come before it in the order, so each is in the
-// hands of a CTA that runs and does not wait.
+// unit's sums are stored.  A sum waits for its shares; they come before it in the order, so each has been
+// taken by a CTA that runs and does not wait for it (no unit belongs to a CTA before that CTA takes it: one
+// that found no room yet holds nothing up).
 template <typename T, int DC>
 __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
     attn_bwd_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_constant__ AttnParams p, const AttnWork w,
@@ -586,17 +587,17 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
     const unsigned n_all = n_main + (split > 1 ? unsigned(p.slots) * unsigned(p.kv_heads) * AT_PIECES : 0u);
     unsigned loads = 0, issued = 0, aux = 0;  // ring items so far, also those under way
     int k = 0, tiles = 0;         // units so far; those of them with tiles
+    // the row starts into the L1 while the first unit's number is on its way
+    for (int i = lane * 32; i <= p.rows && i < 1024; i += 1024) asm volatile("prefetch.global.L1 [%0];" ::"l"(p.cu + i));
     for (;; ++k) {
-      // the next unit that is not empty; the first is the CTA's number
+      // the next unit that is not empty
       AttnUnit u;
       u.kind = AT_UNIT_END;
       int slot = 0;
-      for (bool start = k == 0;; start = false) {
-        unsigned at = blockIdx.x;
-        if (!start) {
-          if (lane == 0) at = gridDim.x + atomicAdd(w.next, 1u);
-          at = __shfl_sync(0xffffffffu, at, 0);
-        }
+      for (;;) {
+        unsigned at = 0;
+        if (lane == 0) at = atomicAdd(w.next, 1u);
+        at = __shfl_sync(0xffffffffu, at, 0);
         if (at >= n_all) break;
         if (at < n_keys) {
           u.kind = AT_UNIT_KEYS;
@@ -1053,9 +1054,9 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
   if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
-static bool attn_strides_ok(int64_t stride, int64_t head_stride, const nf4b_attn& a, int heads) {
-  return (a.tokens == 1 || stride >= a.head_dim) && (heads == 1 || head_stride >= a.head_dim) && stride % 8 == 0 &&
-         head_stride % 8 == 0 && stride < (int64_t(1) << 38) && head_stride < (int64_t(1) << 38);
+static bool attn_strides_ok(int64_t stride, int64_t head_stride, const nf4b_attn& a) {
+  return stride >= a.head_dim && head_stride >= a.head_dim && stride % 8 == 0 && head_stride % 8 == 0 &&
+         stride < (int64_t(1) << 38) && head_stride < (int64_t(1) << 38);
 }
 
 // Checks the call and writes its normalised form (window bounds cut to the token count, so that
@@ -1075,9 +1076,12 @@ static int attn_checks(const nf4b_attn* in, nf4b_attn* a) {
   if (a->tokens == 0) return NF4B_OK;
   NF4B_RETURN_IF(!a->q || !a->k || !a->v || !a->cu, NF4B_ERR_INVALID_ARG);
   NF4B_RETURN_IF(!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->cu, 4), NF4B_ERR_ALIGNMENT);
-  NF4B_RETURN_IF(!attn_strides_ok(a->q_stride, a->q_head_stride, *a, a->heads) ||
-                     !attn_strides_ok(a->k_stride, a->k_head_stride, *a, a->kv_heads) ||
-                     !attn_strides_ok(a->v_stride, a->v_head_stride, *a, a->kv_heads),
+  // a dimension of one element may carry any stride
+  if (a->tokens == 1) a->q_stride = a->k_stride = a->v_stride = int64_t(a->heads) * a->head_dim;
+  if (a->heads == 1) a->q_head_stride = a->head_dim;
+  if (a->kv_heads == 1) a->k_head_stride = a->v_head_stride = a->head_dim;
+  NF4B_RETURN_IF(!attn_strides_ok(a->q_stride, a->q_head_stride, *a) || !attn_strides_ok(a->k_stride, a->k_head_stride, *a) ||
+                     !attn_strides_ok(a->v_stride, a->v_head_stride, *a),
                  NF4B_ERR_ALIGNMENT);
   a->left = a->left < 0 || a->left >= a->tokens ? -1 : a->left;
   a->right = a->right < 0 || a->right >= a->tokens ? -1 : a->right;

@@ -10,6 +10,15 @@ from tests.attention_ref import assert_within, reference
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    """No pipeline wait of the kernels ran out of time in any test."""
+    from stew_b200 import _lib
+    yield
+    if torch.cuda.is_available():
+        assert _lib.attn_error_flag() == 0
+
+
 def _edges(lens):
     e = [0]
     for x in lens:
@@ -268,6 +277,61 @@ def test_two_streams_at_once(cuda_lib):
                 got[i].append(packed_attention(*s[:4]))
     torch.cuda.synchronize()
     assert all(torch.equal(o, w) for w, os in zip(want, got) for o in os)
+
+
+def test_two_backwards_at_once(cuda_lib, monkeypatch):
+    """Backward passes whose CTAs wait for sums over shares, on three streams at once: neither holds
+    the other up."""
+    from stew_b200 import _lib
+    from stew_b200.step_ops import packed_attention
+    monkeypatch.setenv("STEW_ATTN_SPLIT", "6")
+    sets = [_inputs([900, 400, 700], 12, 2, 128, torch.float16, seed=s) for s in (1, 2, 3)]
+
+    def run(s):
+        leaves = [t.detach().requires_grad_(True) for t in s[:3]]
+        return torch.autograd.grad(packed_attention(*leaves, s[3]), leaves, s[5])
+
+    want = [run(s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[] for _ in sets]
+    for _ in range(6):
+        for i, (s, st) in enumerate(zip(sets, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(run(s))
+    torch.cuda.synchronize()
+    for w, gs in zip(want, got):
+        assert all(torch.equal(a, b) for g in gs for a, b in zip(w, g))
+    assert _lib.attn_error_flag() == 0
+
+
+@pytest.mark.parametrize("split", ["1", "2", "3", "6"])
+@pytest.mark.parametrize("d", [64, 80, 128])
+def test_shares_of_a_group(cuda_lib, monkeypatch, split, d):
+    """A key tile's heads on one CTA or shared out over several."""
+    monkeypatch.setenv("STEW_ATTN_SPLIT", split)
+    q, k, v, cu, edges, dout = _inputs([300, 140, 1, 129], 6, 1, d, torch.float16, pad=5, seed=8)
+    _check(q, k, v, cu, edges, dout)
+
+
+def test_one_token_dimension_with_any_stride(cuda_lib):
+    from stew_b200.step_ops import packed_attention
+    q, k, v, cu, edges, dout = _inputs([1], 1, 1, 64, torch.float16)
+    want = packed_attention(q, k, v, cu)
+    odd = [t.as_strided((1, 1, 64), (3, 5, 1)) for t in (q, k, v)]
+    assert torch.equal(packed_attention(*odd, cu), want) and torch.equal(want, v)
+
+
+def test_changed_row_starts_are_noticed(cuda_lib):
+    """The row starts are saved for the backward; changing them in between is an error, not a wrong
+    gradient."""
+    from stew_b200.step_ops import packed_attention
+    q, k, v, cu, edges, dout = _inputs([20, 30], 1, 1, 64, torch.float16)
+    q.requires_grad_(True)
+    out = packed_attention(q, k, v, cu)
+    cu[1] = 10
+    with pytest.raises(RuntimeError):
+        out.backward(dout)
 
 
 def test_long_row_past_32_bit_offsets(cuda_lib):
