@@ -194,12 +194,14 @@ def _attn_forward(q, k, v, cu, left, right, scale, keep_rest=False):
     q, *qs = _attn_layout(q)
     k, *ks = _attn_layout(k)
     v, *vs = _attn_layout(v)
-    shape, dt, dev = q.shape, q.dtype, q.device
-    out = torch.empty(shape, dtype=dt, device=dev)
-    rest = torch.empty(shape, dtype=dt, device=dev) if keep_rest else None
-    lse = torch.empty((shape[1], shape[0]), dtype=torch.float32, device=dev)
+    n, hq, _ = q.shape
+    dev = q.device
+    # (empty_like with a memory format is less than half the host time of empty with a Size)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    rest = torch.empty_like(q, memory_format=torch.contiguous_format) if keep_rest else None
+    lse = torch.empty(hq, n, dtype=torch.float32, device=dev)
     rec = _attn_record(q, qs, k, ks, v, vs, cu, left, right, scale)
-    if shape[0]:
+    if n:
         _launch(_lib.lib().nf4b_attn_fwd, "nf4b_attn_fwd", dev, rec, out.data_ptr(),
                 rest.data_ptr() if keep_rest else None, lse.data_ptr())
     return out, rest, lse, q, k, v, rec
@@ -218,9 +220,9 @@ class _PackedAttention(torch.autograd.Function):
         q, k, v, _, out, rest, lse = ctx.saved_tensors
         dev, dt = q.device, q.dtype
         dout = _aligned_c(dout if dout.dtype == dt else dout.to(dt))
-        dq = torch.empty(q.shape, dtype=dt, device=dev)
-        dk = torch.empty(k.shape, dtype=dt, device=dev)
-        dv = torch.empty(k.shape, dtype=dt, device=dev)
+        dq = torch.empty_like(q, memory_format=torch.contiguous_format)
+        dk = torch.empty_like(k, memory_format=torch.contiguous_format)
+        dv = torch.empty_like(v, memory_format=torch.contiguous_format)
         if q.shape[0]:
             L = _lib.lib()
             # the record's addresses are those of the saved tensors, which the graph keeps alive
