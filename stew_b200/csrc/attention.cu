@@ -311,14 +311,17 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
 // beside 2,048 of MMAs; a launch per unit instead of persistent CTAs: 43 us and 694.
 //
 // fp16 range: dS is rounded to the operand type with a power-of-two scale 2^k that puts the largest
-// |dO||V| + |delta| of the sequence (the prep launch's maxima per tile) at 2^14, and P with 2^8:
+// |dO||V| + |delta| of the tiles a unit meets (the prep launch's maxima) at 2^14, and P with 2^8:
 // gradients of any size keep fp16's 11 bits, where unscaled products of small gradients would fall
-// into its subnormals.  bf16 has fp32's range and is not scaled.
+// into its subnormals (rows share their unit's scale: beside rows with gradients 2^20 times larger they still
+// do).  The whole sequence's maxima would do for one scale, but their scan grows with the sequence under a
+// window: 262,144 tokens, window 128, 14 heads of 64 on 2: 6,962 us against 2,046.  bf16 has fp32's range and
+// is not scaled.
 constexpr int AT_BWD_THREADS = 320;
 constexpr int AT_PREP_THREADS = 256;
 
 template <typename T>
-constexpr float at_p_shift() { return sizeof(T) == 2 && at_idesc<T>(16, false) == at_idesc<__half>(16, false) ? 8.f : 0.f; }
+constexpr float at_p_shift() { return std::is_same<T, __half>::value ? 8.f : 0.f; }
 
 // The backward's scratch.
 struct AttnWork {
@@ -433,18 +436,21 @@ __global__ void __launch_bounds__(AT_PREP_THREADS)
   }
 }
 
-// Whole warp: the exponent k of the dS scale for a tile (slot, at i0) of a sequence and a key/value head.
-__device__ __forceinline__ int at_ds_exponent(const AttnParams& p, const AttnWork& w, int slot, int i0, int len, int hk) {
-  const int lane = threadIdx.x & 31, grp = p.heads / p.kv_heads;
-  const int first = slot - (i0 >> 7), tiles = (len + AT_TILE - 1) >> 7;
+// Whole warp: the exponent k of a unit's dS scale, from the tiles it meets: nd query tiles from slot d0 on of
+// heads [h0, h0 + nh), nv key tiles from slot v0 on of key/value head hk.  (Any k is right that overflows
+// nothing: the sums are scaled back in fp32.  Only a unit's own tiles are read, so that under a window the
+// scan does not grow with the sequence.)
+__device__ __forceinline__ int at_ds_exponent(const AttnParams& p, const AttnWork& w, int h0, int nh, int d0, int nd, int hk,
+                                              int v0, int nv) {
+  const int lane = threadIdx.x & 31;
   float m_do = 0.f, m_dl = 0.f, m_v = 0.f;
-  for (int i = lane; i < grp * tiles; i += 32) {
-    const int g = i / tiles;
-    const float2 x = w.tile[int64_t(hk * grp + g) * p.slots + first + i - g * tiles];
+  for (int i = lane; i < nh * nd; i += 32) {
+    const int g = i / nd;
+    const float2 x = w.tile[int64_t(h0 + g) * p.slots + d0 + i - g * nd];
     m_do = fmaxf(m_do, x.x);
     m_dl = fmaxf(m_dl, x.y);
   }
-  for (int i = lane; i < tiles; i += 32) m_v = fmaxf(m_v, w.vmax[int64_t(hk) * p.slots + first + i]);
+  for (int i = lane; i < nv; i += 32) m_v = fmaxf(m_v, w.vmax[int64_t(hk) * p.slots + v0 + i]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     m_do = fmaxf(m_do, __shfl_xor_sync(0xffffffffu, m_do, o));
@@ -697,7 +703,9 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
       // slot is done)
       int k_exp = 0;
       if (at_p_shift<T>() != 0.f) {
-        k_exp = at_ds_exponent(p, w, slot, u.i0, u.len, u.hk);
+        const int other = slot - (u.i0 >> 7) + u.yt0;  // the ring's first tile
+        k_exp = keys ? at_ds_exponent(p, w, u.h0, grp / split, other, u.nt, u.hk, slot, 1)
+                     : at_ds_exponent(p, w, u.h, 1, slot, 1, u.hk, other, u.nt);
         if (lane == 0) {
           exponent[(tiles - 1) & 1] = k_exp;
           mbar_arrive(&exp_full[(tiles - 1) & 1]);
@@ -919,12 +927,6 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
           mbar_arrive(p_ready);  // the scores are in registers: the next tile's may overwrite them
         }
         uint64_t pv[32];
-        auto hide = [&] {  // 0 where the pair is not visible, whatever is there
-          at_hide(see_lo - y0, see_hi - y0, [&](int c) {
-            const float2 v = f2_unpack(pv[c >> 1]);
-            pv[c >> 1] = c & 1 ? f2_pack(v.x, 0.f) : f2_pack(0.f, v.y);
-          });
-        };
         const ulonglong2* la = reinterpret_cast<const ulonglong2*>(aux_lse + sa * AT_TILE + half * 64);
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
@@ -935,6 +937,12 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
           pv[2 * c] = f2_pack(at_exp2(f.x), at_exp2(f.y));
           pv[2 * c + 1] = f2_pack(at_exp2(g.x), at_exp2(g.y));
         }
+        auto hide = [&] {  // 0 where the pair is not visible, whatever is there
+          at_hide(see_lo - y0, see_hi - y0, [&](int c) {
+            const float2 v = f2_unpack(pv[c >> 1]);
+            pv[c >> 1] = c & 1 ? f2_pack(v.x, 0.f) : f2_pack(0.f, v.y);
+          });
+        };
         if (y0 < lo_max || y0 + 63 > hi_min) hide();
         if (!cut_tile()) return;
         auto put = [&](uint32_t taddr) {  // rounded to the MMA's operand type

@@ -193,10 +193,11 @@ __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap
       : "memory");
 }
 
-// N threads (this one `id`): zeros in the rows from `first` to the next multiple of 16 (the tokens of one MMA;
-// those behind it are not multiplied) of a [ROWS tokens][DC x 64 features] tile that has arrived, so that the rows of other sequences behind a ragged tile add nothing to a product over
-// tokens (0 x their NaN would).  The 128-byte swizzle permutes inside a row only.  (The caller makes the
-// writes visible to the MMAs: fence_proxy_async_smem.)
+// N threads (this one `id`): zeros in the rows from `first` to the next multiple of 16 (the tokens of one
+// MMA; those behind it are not multiplied) of a [ROWS tokens][DC x 64 features] tile that has arrived, so
+// that the rows of other sequences behind a ragged tile add nothing to a product over tokens (0 x their NaN
+// would).  The 128-byte swizzle permutes inside a row only.  (The caller makes the writes visible to the
+// MMAs: fence_proxy_async_smem.)
 template <int DC, int ROWS, int N>
 __device__ __forceinline__ void at_zero_rows(uint8_t* tile, int first, int id) {
 #pragma unroll

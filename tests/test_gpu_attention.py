@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from tests.attention_ref import assert_within, reference
+from tests.attention_ref import assert_within, reference, row_mask
 
 pytestmark = pytest.mark.gpu
 
@@ -119,6 +119,49 @@ def test_gradient_scales(cuda_lib, dscale, dtype):
     the type; fp16's 2^-25 is in the bound."""
     q, k, v, cu, edges, dout = _inputs([200, 310], 4, 2, 128, dtype, dscale=dscale)
     _check(q, k, v, cu, edges, dout)
+
+
+@pytest.mark.parametrize("window", [(64, 0), (0, 64)])
+def test_gradient_scales_under_a_window(cuda_lib, window):
+    """Rows whose gradients are 2^24 times smaller than those of a far part of their sequence, whose
+    tiles no window joins to theirs, keep their precision: scaled by the far rows' size, a ds of
+    about 2^-15 would be rounded to steps of 2^-20, where its bound here is 2^-26.
+
+    Where a window does join tiles, all ds of a 128-token tile share one scale 2^k, with
+    k = 14 - floor(log2 M) >= 14 - log2 M, M the largest |dO||V| + |delta| of the tiles that meet;
+    a scaled ds below fp16's normal range is off by up to 2^-25, so ds by 2^-25 / 2^k <= M 2^-39,
+    which the bounds of assert_within's reference (ds in the normal range) do not hold."""
+    from stew_b200.step_ops import packed_attention
+    n, hq, hk, d = 640, 4, 2, 64
+    q, k, v, cu, edges, dout = _inputs([n], hq, hk, d, torch.float16, seed=21, dscale=2.0 ** -12)
+    dout[:128] *= 2.0 ** 24
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    out = packed_attention(*leaves, cu, window=window)
+    grads = torch.autograd.grad(out, leaves, dout)
+    sc = 1 / math.sqrt(d)
+    ref = reference(q, k, v, edges, *window, sc, dout)
+    see = row_mask(n, *window, "cuda").double()
+    tiles = n // 128
+    n_do, n_v = dout.double().norm(dim=2), v.double().norm(dim=2)  # [n, hq], [n, hk]
+    delta = (dout.double() * ref["out"][0]).sum(2).abs()
+    size = lambda x, t, m: x[t * 128:(t + m) * 128].amax(0)  # of tiles [t, t + m), by head
+    for t in range(tiles):
+        mine = slice(t * 128, (t + 1) * 128)
+        for keys in (False, True):
+            back, ahead = window[::-1] if keys else window
+            lo, hi = max(0, t * 128 - back) // 128, min(n - 1, t * 128 + 127 + ahead) // 128
+            a, b = ((lo, hi - lo + 1), (t, 1)) if keys else ((t, 1), (lo, hi - lo + 1))
+            m = size(n_do, *a) * size(n_v, *b).repeat_interleave(hq // hk) + size(delta, *a)  # [hq]
+            lost = sc * m * 2.0 ** -39
+            if keys:  # over the group's heads, one scale for all of them at most
+                lost = lost.view(hk, -1).amax(1)[:, None]
+                x = q.double().abs().view(n, hk, hq // hk, d).sum(2)
+                ref["dk"][1][mine] += lost * torch.einsum("ij,ihd->jhd", see[:, mine], x)
+            else:
+                x = k.double().abs().repeat_interleave(hq // hk, 1)
+                ref["dq"][1][mine] += lost[:, None] * torch.einsum("ij,jhd->ihd", see[mine], x)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out, *grads)):
+        assert_within(got, *ref[name], name)
 
 
 def test_large_scores_and_values(cuda_lib):
