@@ -42,7 +42,8 @@ def clip_grads(grads, max_norm: float, divisor: torch.Tensor | None = None, out=
     all-reduced flat buffer); None scales in place, and an in-place list that is under the limit
     and has no divisor is only read.  divisor: one fp32 on the device (the labelled-token count),
     None for 1.  max_norm: >= 0; infinity never clips.  A norm that is not finite behaves as
-    max_norm / norm does: infinite gives zeros (NaN where g is infinite), NaN gives NaN."""
+    max_norm / norm does: infinite gives zeros (NaN where g is infinite, and everywhere under an
+    infinite max_norm), NaN gives NaN.  No output may overlap another gradient or output."""
     grads = list(grads)
     dst = grads if out is None else list(out)
     if not grads:
@@ -87,6 +88,7 @@ def clip_grads(grads, max_norm: float, divisor: torch.Tensor | None = None, out=
     work = torch.empty(wb, dtype=torch.uint8, device=dev)
     _launch(L.nf4b_clip_grads, "nf4b_clip_grads", dev, table.buffer_info()[0], n, max_norm,
             None if divisor is None else divisor.data_ptr(), norm.data_ptr(), work.data_ptr(), wb)
+    torch.autograd.graph.increment_version(dst)  # written: an autograd graph that saved one notices
     return norm
 
 

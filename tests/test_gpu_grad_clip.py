@@ -105,12 +105,29 @@ def test_not_finite(cuda_lib):
     g = [torch.tensor([1.0, float("nan")], device="cuda"), torch.ones(5, device="cuda")]
     assert math.isnan(float(clip_grads(g, 1.0)))
     assert torch.isnan(g[0]).all() and torch.isnan(g[1]).all()
+    g = [torch.tensor([1.0, float("inf")], device="cuda")]
+    assert math.isinf(float(clip_grads(g, math.inf))) and torch.isnan(g[0]).all()
     z = [torch.zeros(9, device="cuda")]
     assert float(clip_grads(z, 1.0)) == 0.0 and not z[0].any()
     z = [torch.ones(9, device="cuda")]
     assert float(clip_grads(z, math.inf)) == 3.0 and bool((z[0] == 1).all())
     assert float(clip_grads(z, 0.0)) == 3.0 and not z[0].any()
     assert float(clip_grads([torch.empty(0, device="cuda")], 1.0)) == 0.0
+
+
+def test_autograd_notices_the_write(cuda_lib):
+    """A gradient that an autograd graph saved and clip_grads then scaled ends that graph's backward
+    with torch's error; out of place only the outputs count as written."""
+    from stew_b200.dp import clip_grads
+    for out in (False, True):
+        g, a = torch.full((9,), 3.0, device="cuda"), torch.ones(9, device="cuda", requires_grad=True)
+        y = (a * g).sum()
+        clip_grads([g], 1.0, out=[torch.empty_like(g)] if out else None)
+        if out:
+            assert torch.equal(torch.autograd.grad(y, a)[0], g)
+        else:
+            with pytest.raises(RuntimeError, match="inplace operation"):
+                y.backward()
 
 
 def test_same_bits_and_matches_torch(cuda_lib):
