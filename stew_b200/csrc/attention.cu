@@ -310,6 +310,8 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
 // about 2,900 clocks, of them 1,150 exponentials and 1,250 other elementwise work and waits in one chain,
 // beside 2,048 of MMAs; a launch per unit instead of persistent CTAs: 43 us and 694.
 //
+// FINE: dS is kept as two 16-bit values, its rounding and what that leaves, each with its product (attn_fine()).
+//
 // fp16 range: dS is rounded to the operand type with a power-of-two scale 2^k that puts the largest
 // |dO||V| + |delta| of the tiles a unit meets (the prep launch's maxima) at 2^14, and P with 2^8:
 // gradients of any size keep fp16's 11 bits, where unscaled products of small gradients would fall
@@ -515,7 +517,7 @@ __device__ __forceinline__ float4* at_part(float* parts, int join, int split, in
 // unit's sums are stored.  A sum waits for its shares; they come before it in the order, so each has been
 // taken by a CTA that runs and does not wait for it (no unit belongs to a CTA before that CTA takes it: one
 // that found no room yet holds nothing up).
-template <typename T, int DC>
+template <typename T, int DC, bool FINE>
 __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
     attn_bwd_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_constant__ AttnParams p, const AttnWork w,
                     const int split, T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dv) {
@@ -820,6 +822,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
         if (!wait(ds_ready, r & 1, 21)) break;
         tc_fence_after();
         sum(tmem + AT_TM_DX, tmem + AT_TM_DP, ta + (r & 1) * STEP, it > 0, steps);
+        if (FINE) sum(tmem + AT_TM_DX, tmem + AT_TM_DP + 32, ta + (r & 1) * STEP, true, steps);
         at_commit(lead, &a_empty[r & 1]);
         if (more && !dp_of(r + 1, keys, next)) break;
         if (it + 2 == n) at_commit(lead, xy_empty);  // no more scores of this unit
@@ -909,6 +912,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
           if (!scale(it) || !wait(dp_full, r & 1, 24)) return;
           tc_fence_after();
           tmem_st_32x32b_x32(t_dp, zeros);
+          if (FINE) tmem_st_32x32b_x32(t_dp + 32, zeros);
           tmem_st_wait();
           tc_fence_before();
           mbar_arrive(ds_ready);
@@ -956,6 +960,15 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
           tmem_st_wait();
           tc_fence_before();
         };
+        auto put_rest = [&](uint32_t taddr) {  // what that rounding leaves, rounded again
+          uint32_t pk[32];
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            const float2 v = f2_unpack(pv[k]), w = at_unpack<T>(at_pack<T>(v.x, v.y));
+            pk[k] = at_pack<T>(v.x - w.x, v.y - w.y);
+          }
+          tmem_st_32x32b_x32(taddr, pk);
+        };
         if (KEYS) {
           put(t_s);
           mbar_arrive(p_ready);
@@ -976,6 +989,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
           pv[2 * c + 1] = f2_mul(pv[2 * c + 1], f2_fma(f2_pack_u(dpv[4 * c + 2], dpv[4 * c + 3]), scx2, d4.y));
         }
         if (y0 + 64 > u.len) hide();  // tokens of another sequence (inside this one p = 0 has done it)
+        if (FINE) put_rest(t_dp + 32);
         put(t_dp);
         mbar_arrive(ds_ready);
         if (KEYS) {
@@ -1223,6 +1237,17 @@ static int attn_split(const nf4b_attn& a) {
   return best;
 }
 
+// Whether dS goes into dQ and dK with what its rounding leaves: sequences of 256 tokens or fewer on average
+// (the padding counts), or windows of 128.  The ds of a row sum to zero, so over a few tokens their roundings
+// stay in the sums: with two to ten tokens a sequence dq and dk were 1.50 to 1.56 times as far off the 64-bit
+// result as values rounded once, with the rest 1.05 to 1.14 times; over some hundred tokens it was 1.43.  It
+// costs a second dS product: a backward of 63 tokens 17.6 -> 18.2 us, of 1,170 in 4 rows 31.9 -> 35.2, of
+// 8,192 670 -> 820.
+static bool attn_fine(const nf4b_attn& a) {
+  const bool window = a.left >= 0 && a.right >= 0 && int64_t(a.left) + a.right < AT_TILE;
+  return window || a.tokens <= int64_t(a.rows) * 2 * AT_TILE;
+}
+
 static int64_t attn_work(const nf4b_attn& a, int split, void* base, AttnWork* w) {
   const int64_t slots = at_slots(a.tokens, a.rows), pairs = slots * a.kv_heads;
   char* b = static_cast<char*>(base);
@@ -1249,7 +1274,7 @@ extern "C" int64_t nf4b_attn_bwd_work_bytes(const nf4b_attn* args) {
   return attn_work(a, attn_split(a), nullptr, nullptr);
 }
 
-template <typename T, int DC>
+template <typename T, int DC, bool FINE>
 static int attn_bwd_launch(const nf4b_attn& a, const void* out, const void* rest, const float* lse, const void* dout, void* dq, void* dk,
                            void* dv, void* work, int split, cudaStream_t s) {
   AttnBwdMaps m;
@@ -1258,7 +1283,7 @@ static int attn_bwd_launch(const nf4b_attn& a, const void* out, const void* rest
   if (st == NF4B_OK) st = attn_tmap(&m.v, a, a.v, a.kv_heads, a.v_stride, a.v_head_stride, AT_TILE);
   if (st == NF4B_OK) st = attn_tmap(&m.dout, a, dout, a.heads, int64_t(a.heads) * a.head_dim, a.head_dim, AT_TILE);
   static bool done[64] = {false};
-  if (st == NF4B_OK) st = attn_smem(attn_bwd_kernel<T, DC>, AttnBwdSmem<DC>::ALLOC, done);
+  if (st == NF4B_OK) st = attn_smem(attn_bwd_kernel<T, DC, FINE>, AttnBwdSmem<DC>::ALLOC, done);
   if (st != NF4B_OK) return st;
   const AttnParams p = attn_params(a);
   AttnWork w;
@@ -1270,7 +1295,7 @@ static int attn_bwd_launch(const nf4b_attn& a, const void* out, const void* rest
                            static_cast<const T*>(a.v), a.v_stride, a.v_head_stride, w, tq, tk, tv));
   const int64_t units = int64_t(p.slots) * (int64_t(a.kv_heads) * (split > 1 ? split + AT_PIECES : 1) + a.heads);
   const int64_t sms = attn_sms();
-  NF4B_CUDA_TRY(launch_pdl(attn_bwd_kernel<T, DC>, dim3(unsigned(units < sms ? units : sms)), dim3(AT_BWD_THREADS),
+  NF4B_CUDA_TRY(launch_pdl(attn_bwd_kernel<T, DC, FINE>, dim3(unsigned(units < sms ? units : sms)), dim3(AT_BWD_THREADS),
                            size_t(AttnBwdSmem<DC>::ALLOC), s, m, p, w, split, tq, tk, tv));
   return launch_status("attn_bwd_kernel launch");
 }
@@ -1290,10 +1315,15 @@ extern "C" int nf4b_attn_bwd(const nf4b_attn* args, const void* out, const void*
   st = check_device();
   if (st != NF4B_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool wide = a.head_dim > 64;
-  if (a.dtype == NF4B_F16)
-    return wide ? attn_bwd_launch<__half, 2>(a, out, rest, lse, dout, dq, dk, dv, work, split, s)
-                : attn_bwd_launch<__half, 1>(a, out, rest, lse, dout, dq, dk, dv, work, split, s);
-  return wide ? attn_bwd_launch<__nv_bfloat16, 2>(a, out, rest, lse, dout, dq, dk, dv, work, split, s)
-              : attn_bwd_launch<__nv_bfloat16, 1>(a, out, rest, lse, dout, dq, dk, dv, work, split, s);
+  auto launch = [&](auto tag, auto dc, auto fine) {
+    using T = decltype(tag);
+    return attn_bwd_launch<T, decltype(dc)::value, decltype(fine)::value>(a, out, rest, lse, dout, dq, dk, dv, work, split, s);
+  };
+  auto typed = [&](auto tag) {
+    const std::integral_constant<int, 1> one;
+    const std::integral_constant<int, 2> two;
+    if (attn_fine(a)) return a.head_dim > 64 ? launch(tag, two, std::true_type{}) : launch(tag, one, std::true_type{});
+    return a.head_dim > 64 ? launch(tag, two, std::false_type{}) : launch(tag, one, std::false_type{});
+  };
+  return a.dtype == NF4B_F16 ? typed(__half()) : typed(__nv_bfloat16());
 }

@@ -252,8 +252,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torc
     Returns [N, Hq, D]; tokens behind cu[B] get zeros, and zero gradients.  Any strides with
     contiguous features are read in place when they are multiples of 8 elements, else copied.
     The backward recomputes the probabilities from the saved log-sum-exp; beside the output it
-    keeps what the output's rounding left (a second tensor of its size), from which the rows'
-    do.o are exact.  Forward and backward give the same bits on every run.  Second derivatives are
+    keeps what the output's rounding left (a second tensor of its size), so that the rows' do.o
+    are free of it.  Forward and backward give the same bits on every run.  Second derivatives are
     refused."""
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError("packed_attention: q, k and v must be [tokens, heads, head_dim]")

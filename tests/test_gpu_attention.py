@@ -164,6 +164,33 @@ def test_gradient_scales_under_a_window(cuda_lib, window):
         assert_within(got, *ref[name], name)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens,window,d", [([2] * 40, (-1, 0), 128), ([1, 3, 5, 2, 70, 128, 0, 9], (-1, 0), 64),
+                                           ([128, 100], (-1, -1), 96), ([500, 131], (2, 0), 128), ([700], (60, 67), 64),
+                                           ([300] + [1] * 9, (-1, 0), 128)], ids=str)
+def test_few_tokens_keep_what_the_rounding_of_ds_leaves(cuda_lib, lens, window, d, dtype):
+    """Where the tokens see few others on average, dq and dk are as if ds were not rounded to the type:
+    1.3 times as far off as the output's own rounding at most, over all elements.
+
+    A rounding's error has the same relative size e on average, whatever is rounded, and e is what the
+    output's has.  ds rounded to the type would add a second independent e: sqrt(2) = 1.41 and more.
+    What stays is do.o: o = (V_m + sum_j r(p_j) V_j) / l holds the roundings of all p but the
+    largest (exp(0) = 1).  With two tokens, p_2 <= p_1, dO of size s and d features, that shifts do.o by
+    e p_2 s sqrt(d) and so dq by e p_2 s sqrt(d) sqrt(p_1^2 + p_2^2) |K|, against dq =
+    p_1 p_2 (dP_1 - dP_2) (K_1 - K_2) of size 2 p_1 p_2 s sqrt(d) |K|: e sqrt(p_1^2 + p_2^2) / (2 p_1)
+    <= 0.71 e, in all sqrt(1 + 0.5) = 1.22 (more tokens: smaller parts each); 6 % are for the sample."""
+    from stew_b200.step_ops import packed_attention
+    q, k, v, cu, edges, dout = _inputs(lens, 4, 2, d, dtype, seed=31)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    out = packed_attention(*leaves, cu, window=window)
+    grads = torch.autograd.grad(out, leaves, dout)
+    ref = reference(q, k, v, edges, *window, 1 / math.sqrt(d), dout)
+    for name, got in (("dq", grads[0]), ("dk", grads[1])):
+        want = ref[name][0]
+        own = (want.to(dtype).double() - want).norm()
+        assert float((got.double() - want).norm() / own) <= 1.3, name
+
+
 def test_large_scores_and_values(cuda_lib):
     """Scores up to some hundreds (one-hot rows), large values."""
     q, k, v, cu, edges, dout = _inputs([257, 140], 4, 2, 128, torch.float16, seed=9)
