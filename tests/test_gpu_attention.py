@@ -79,6 +79,24 @@ def test_windows(cuda_lib, window, dtype, d):
     _check(q, k, v, cu, edges, dout, window=window)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d", [8, 64, 72, 128])
+@pytest.mark.parametrize("lens,window", [([390, 128, 1, 633], (-1, -1)), ([390, 128, 1, 633], (5, -1)), ([257], (64, 64)),
+                                         ([700, 0, 333], (200, 300)), ([513, 512], (-1, 7)), ([260, 259], (-1, 0))], ids=str)
+def test_longer_rows(cuda_lib, lens, window, d, dtype):
+    """Sequences of more than 256 tokens on average (their ds is rounded once), with every kind of window."""
+    q, k, v, cu, edges, dout = _inputs(lens, 6, 2, d, dtype, seed=7)
+    assert edges[-1] > 256 * len(lens)
+    _check(q, k, v, cu, edges, dout, window=window)
+
+
+@pytest.mark.parametrize("split", ["1", "2", "3", "6"])
+def test_shares_of_a_group_in_longer_rows(cuda_lib, monkeypatch, split):
+    monkeypatch.setenv("STEW_ATTN_SPLIT", split)
+    q, k, v, cu, edges, dout = _inputs([300, 517], 12, 2, 96, torch.float16, seed=8, pad=5)
+    _check(q, k, v, cu, edges, dout)
+
+
 @pytest.mark.parametrize("pad", [0, 1, 200])
 def test_strided_projection_output_and_padding(cuda_lib, pad):
     q, k, v, cu, edges, dout = _inputs([77, 260], 6, 2, 64, torch.bfloat16, pad=pad, fused=True)
