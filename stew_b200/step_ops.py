@@ -190,7 +190,7 @@ def _attn_record(q, qs, k, ks, v, vs, cu, left, right, scale) -> bytes:
 
 
 def _attn_forward(q, k, v, cu, left, right, scale, keep_rest=False):
-    """(out, what its rounding left or None, lse, q, k, v as read, the call's nf4b_attn record)."""
+    """(out, what its rounding left or None, lse, q, k, v as read)."""
     q, *qs = _attn_layout(q)
     k, *ks = _attn_layout(k)
     v, *vs = _attn_layout(v)
@@ -200,35 +200,43 @@ def _attn_forward(q, k, v, cu, left, right, scale, keep_rest=False):
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     rest = torch.empty_like(q, memory_format=torch.contiguous_format) if keep_rest else None
     lse = torch.empty(hq, n, dtype=torch.float32, device=dev)
-    rec = _attn_record(q, qs, k, ks, v, vs, cu, left, right, scale)
     if n:
+        rec = _attn_record(q, qs, k, ks, v, vs, cu, left, right, scale)
         _launch(_lib.lib().nf4b_attn_fwd, "nf4b_attn_fwd", dev, rec, out.data_ptr(),
                 rest.data_ptr() if keep_rest else None, lse.data_ptr())
-    return out, rest, lse, q, k, v, rec
+    return out, rest, lse, q, k, v
 
 
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu, left, right, scale):
-        out, rest, lse, q, k, v, ctx.rec = _attn_forward(q, k, v, cu, left, right, scale, True)
+        out, rest, lse, q, k, v = _attn_forward(q, k, v, cu, left, right, scale, True)
         ctx.save_for_backward(q, k, v, cu, out, rest, lse)
+        ctx.scalars = left, right, scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, _, out, rest, lse = ctx.saved_tensors
+        # Under checkpointing, offload and other saved-tensor hooks these are not the tensors that the
+        # forward read: their addresses and strides are taken here, and nothing of the forward's.
+        q, k, v, cu, out, rest, lse = ctx.saved_tensors
         dev, dt = q.device, q.dtype
+        q, *qs = _attn_layout(q)
+        k, *ks = _attn_layout(k)
+        v, *vs = _attn_layout(v)
+        cu = cu.contiguous()
+        out, rest, lse = _aligned_c(out), _aligned_c(rest), _aligned_c(lse)
         dout = _aligned_c(dout if dout.dtype == dt else dout.to(dt))
         dq = torch.empty_like(q, memory_format=torch.contiguous_format)
         dk = torch.empty_like(k, memory_format=torch.contiguous_format)
         dv = torch.empty_like(v, memory_format=torch.contiguous_format)
         if q.shape[0]:
             L = _lib.lib()
-            # the record's addresses are those of the saved tensors, which the graph keeps alive
-            wb = L.nf4b_attn_bwd_work_bytes(ctx.rec)
+            rec = _attn_record(q, qs, k, ks, v, vs, cu, *ctx.scalars)
+            wb = L.nf4b_attn_bwd_work_bytes(rec)
             work = torch.empty(wb, dtype=torch.uint8, device=dev)
-            _launch(L.nf4b_attn_bwd, "nf4b_attn_bwd", dev, ctx.rec, out.data_ptr(), rest.data_ptr(), lse.data_ptr(),
+            _launch(L.nf4b_attn_bwd, "nf4b_attn_bwd", dev, rec, out.data_ptr(), rest.data_ptr(), lse.data_ptr(),
                     dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), work.data_ptr(), wb)
         return dq, dk, dv, None, None, None, None
 

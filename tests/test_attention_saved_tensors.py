@@ -1,0 +1,103 @@
+"""CPU: the attention's backward launches with the addresses and strides of the tensors that autograd
+hands back, which under checkpointing, offload and other saved-tensor hooks are not the forward's.
+The launches are recorded instead of run."""
+import ctypes
+
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """[(entry, nf4b_attn, the other arguments)] of every launch, which does nothing."""
+    from stew_b200 import _lib, step_ops
+    seen = []
+
+    def record(fn, what, device, rec, *args):
+        seen.append((what, _lib.AttnC.from_buffer_copy(rec), args))
+
+    monkeypatch.setattr(step_ops, "_launch", record)
+    monkeypatch.setattr(step_ops, "packed_attention_supported", lambda q: True)
+    return seen
+
+
+def _inputs(fused):
+    x = torch.zeros(24, 8, 64, dtype=torch.float16)
+    q, k, v = x.split([4, 2, 2], dim=1)
+    if not fused:
+        q, k, v = q.clone(), k.clone(), v.clone()
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    return leaves, torch.tensor([0, 10, 24], dtype=torch.int32)
+
+
+def _fields(a, names):
+    return tuple(getattr(a, n) for n in names.split())
+
+
+SCALARS = "tokens rows heads kv_heads head_dim dtype left right scale"
+
+
+@pytest.mark.parametrize("fused", [False, True])
+@pytest.mark.parametrize("odd", [False, True])
+def test_backward_reads_the_unpacked_tensors(launches, fused, odd):
+    """Hooks that move every saved tensor (odd: to an address that is not 16-byte aligned, so that it is
+    copied once more): the backward names the unpacked ones, with their strides."""
+    from stew_b200.step_ops import packed_attention
+    leaves, cu = _inputs(fused)
+    unpacked = []
+
+    def unpack(t):
+        if odd:
+            buf = torch.empty(t.numel() + 1, dtype=t.dtype)
+            buf[1:].view(t.shape).copy_(t)
+            t = buf[1:].view(t.shape)
+        unpacked.append(t)
+        return t
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().contiguous().clone(), unpack):
+        out = packed_attention(*leaves, cu, window=(7, 3), scale=0.25)
+    out.sum().backward()
+    (w0, fwd, _), (w1, bwd, args) = launches
+    assert (w0, w1) == ("nf4b_attn_fwd", "nf4b_attn_bwd")
+    assert _fields(fwd, SCALARS) == _fields(bwd, SCALARS)
+    assert _fields(bwd, "q_stride q_head_stride k_stride k_head_stride v_stride v_head_stride") == (256, 64, 128, 64, 128, 64)
+    read = [bwd.q, bwd.k, bwd.v, bwd.cu, *args[:3]]  # and out, rest, lse
+    if odd:
+        assert all(a % 16 == 0 for a in read if a != bwd.cu)
+        old = {fwd.q, fwd.k, fwd.v, fwd.cu}
+        assert not old & set(read)
+    else:
+        assert set(read) == {t.data_ptr() for t in unpacked} and len(unpacked) == 7
+
+
+@pytest.mark.parametrize("fused", [False, True])
+def test_backward_under_checkpointing(launches, fused):
+    """The recomputed forward's tensors are the ones that the backward reads."""
+    from stew_b200.step_ops import packed_attention
+    leaves, cu = _inputs(fused)
+    alive = []
+
+    def layer(q, k, v):
+        kept = [t * 1.0 for t in (q, k, v)]
+        alive.extend(kept)
+        return packed_attention(*kept, cu)
+
+    checkpoint(layer, *leaves, use_reentrant=False).sum().backward()
+    names = [what for what, *_ in launches]
+    assert names == ["nf4b_attn_fwd", "nf4b_attn_fwd", "nf4b_attn_bwd"]
+    first, again, bwd = (a for _, a, _ in launches)
+    assert _fields(bwd, "q k v cu") == _fields(again, "q k v cu")
+    assert not set(_fields(first, "q k v")) & set(_fields(bwd, "q k v"))
+    assert launches[2][2][0] == launches[1][2][0] and launches[2][2][2] == launches[1][2][2]  # out, lse
+
+
+def test_plain_backward_reads_the_inputs(launches):
+    """Without hooks nothing is copied: slices of one projection output are read in place."""
+    from stew_b200.step_ops import packed_attention
+    leaves, cu = _inputs(True)
+    packed_attention(*leaves, cu).sum().backward()
+    (_, fwd, _), (_, bwd, _) = launches
+    assert bytes(fwd) == bytes(bwd)
+    assert _fields(bwd, "q k v cu") == tuple(t.data_ptr() for t in (*leaves, cu))
+    assert bwd.q_stride == 512 and ctypes.sizeof(bwd) == ctypes.sizeof(fwd)
