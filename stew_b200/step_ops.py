@@ -12,6 +12,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -261,8 +262,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torc
     contiguous features are read in place when they are multiples of 8 elements, else copied.
     The backward recomputes the probabilities from the saved log-sum-exp; beside the output it
     keeps what the output's rounding left (a second tensor of its size), so that the rows' do.o
-    are free of it.  Forward and backward give the same bits on every run.  Second derivatives are
-    refused."""
+    are free of it.  Forward and backward give the same bits on every run.  Second derivatives and
+    forward-mode tangents are refused."""
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError("packed_attention: q, k and v must be [tokens, heads, head_dim]")
     if not (q.dtype == k.dtype == v.dtype and q.device == k.device == v.device):
@@ -286,7 +287,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torc
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"packed_attention: scale must be positive and finite, got {scale}")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    # (a forward-mode tangent goes there too, to be refused: the kernels on their own would drop it)
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+            or any(forward_ad.unpack_dual(t).tangent is not None for t in (q, k, v))):
         return _PackedAttention.apply(q, k, v, cu, left, right, scale)
     return _attn_forward(q, k, v, cu, left, right, scale)[0]
 

@@ -101,3 +101,21 @@ def test_plain_backward_reads_the_inputs(launches):
     assert bytes(fwd) == bytes(bwd)
     assert _fields(bwd, "q k v cu") == tuple(t.data_ptr() for t in (*leaves, cu))
     assert bwd.q_stride == 512 and ctypes.sizeof(bwd) == ctypes.sizeof(fwd)
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_tangents_are_refused(launches, which, grad):
+    """A dual tensor among q, k, v raises, with and without gradients: the result would carry no tangent."""
+    import torch.autograd.forward_ad as fwad
+
+    from stew_b200.step_ops import packed_attention
+    leaves, cu = _inputs(False)
+    qkv = [t.detach().requires_grad_(grad) for t in leaves]
+    with fwad.dual_level():
+        qkv[which] = fwad.make_dual(qkv[which], torch.ones_like(qkv[which]))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            packed_attention(*qkv, cu)
+        with torch.no_grad(), pytest.raises((RuntimeError, NotImplementedError)):
+            packed_attention(*qkv, cu)
+        packed_attention(*(t.detach() for t in leaves), cu)  # none of them dual: allowed
