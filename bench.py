@@ -733,8 +733,7 @@ def main():
                        "device -> pinned host copies (a third stream); groups overlap"}
         del host_in, host_out, pipe
 
-    if _lib.gemm_error_flag(reset=True) != 0:
-        raise RuntimeError("a GEMM pipeline wait timed out during the bench")
+    _lib.raise_if_wait_ran_out()
 
     cpu = None
     if rank == 0 and world == 1 and not args.no_cpu:

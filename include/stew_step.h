@@ -110,8 +110,8 @@ int nf4b_attn_bwd(const nf4b_attn* a, const void* out, const void* rest, const f
                   void* dq, void* dk, void* dv, void* work, int64_t work_bytes, void* stream);
 
 /* Reads (and with reset != 0 clears) the device-side flag the attention kernels set when a pipeline
- * wait ran out of time (the kernel then ends early instead of hanging).  0 = no timeout since the
- * last reset.  Synchronous.  */
+ * wait ran out of time (the kernel then ends early instead of hanging, with NaN in the output rows
+ * that it did not finish).  0 = no timeout since the last reset.  Synchronous.  */
 int nf4b_attn_error_flag(int* value, int reset);
 
 /* One gradient of a list: src and dst hold `numel` contiguous values of `dtype` (NF4B_F16,

@@ -223,6 +223,16 @@ def attn_error_flag(reset: bool = True) -> int:
     return int(v.value)
 
 
+def raise_if_wait_ran_out() -> None:
+    """Raises when a kernel of the GEMMs or the attention gave up a wait on the current device since
+    the flags were last read (the attention leaves NaN in the rows concerned).  Synchronises; clears
+    the flags."""
+    flags = {"GEMM": gemm_error_flag(), "attention": attn_error_flag()}
+    hit = [f"{name} (flag {v})" for name, v in flags.items() if v]
+    if hit:
+        raise RuntimeError("a wait inside a kernel ran out of time, its results are incomplete: " + ", ".join(hit))
+
+
 def gemm_geometry() -> tuple:
     """(SMs, resident 2-CTA clusters) the fused GEMMs plan with on the current device."""
     a, b = c_int32(0), c_int32(0)

@@ -75,6 +75,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
   uint64_t* o_full = o_done + 1;    // after the last
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC + 4);
+  const AttnWait aw{abort_flag, p.wait_cycles};
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 128) {
@@ -139,17 +140,16 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
       for (int c = 0; c < DC; ++c) tma_load_3d(sbase + L::Q + c * AT_BOX, &tm_q, q_full, c * 64, h, t.a + t.i0);
       for (int x = 0; x < 2 * nt; ++x, ++issued) {
         const int s = x % L::RING;
-        if (!at_wait(&empty[s], ((x / L::RING) & 1) ^ 1, abort_flag, 1)) break;
+        if (!at_wait(&empty[s], ((x / L::RING) & 1) ^ 1, aw, 1)) break;
         mbar_arrive_expect_tx(&full[s], L::TILE);
         for (int c = 0; c < DC; ++c)
           tma_load_3d(sbase + L::KV + s * L::TILE + c * AT_KBOX, x & 1 ? &tm_v : &tm_k, &full[s], c * 64, hk,
                       t.a + (jt0 + (x >> 1)) * AT_KEYS);
       }
-      // an abandoned CTA's loads must have landed before its shared memory goes
-      if (*abort_flag) {
-        at_drain(q_full, 0);
-        for (int x = max(0, issued - L::RING); x < issued; ++x) at_drain(&full[x % L::RING], (x / L::RING) & 1);
-      }
+      // The loads must have landed before the CTA's shared memory goes.  Whoever gives up may do so after the
+      // last of them was issued: always waited for (a finished CTA's have been).
+      at_drain(q_full, 0);
+      for (int x = max(0, issued - L::RING); x < issued; ++x) at_drain(&full[x % L::RING], (x / L::RING) & 1);
     }
   } else if (warp == 5) {
     // ---------------------------------------------------------------- MMA
@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
     const uint64_t dv0 = smem_desc_sw128(sbase + L::KV, AT_KBOX, 1024);
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
-      ok = __all_sync(0xffffffffu, ok && at_wait(bar, parity, abort_flag, where));
+      ok = __all_sync(0xffffffffu, ok && at_wait(bar, parity, aw, where));
       return ok;
     };
     auto arrived = [&](int x) { return wait(&full[x % L::RING], (x / L::RING) & 1, 4); };
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
     bool ok = true;
     for (int it = 0; it < nt; ++it) {
       const int j0 = (jt0 + it) * AT_KEYS, b = it & 1;
-      ok = at_wait(&s_full[b], (it >> 1) & 1, abort_flag, 7);
+      ok = at_wait(&s_full[b], (it >> 1) & 1, aw, 7);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       uint32_t s[2][32];
@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
       if (it > 0 && __any_sync(0xffffffffu, grow)) {
         const float f = grow ? at_exp2((m - top) * sl2) : 1.f;
         l *= f;
-        ok = at_wait(o_done, (it - 1) & 1, abort_flag, 9);  // the products so far
+        ok = at_wait(o_done, (it - 1) & 1, aw, 9);  // the products so far
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
 #pragma unroll 1
@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
       l += l2.x + l2.y;
       if (j0 + AT_KEYS > t.len) {  // the ragged last tile: V's rows behind the sequence's end
         const int x = 2 * it + 1;
-        ok = at_wait(&full[x % L::RING], (x / L::RING) & 1, abort_flag, 2);
+        ok = at_wait(&full[x % L::RING], (x / L::RING) & 1, aw, 2);
         if (!__all_sync(0xffffffffu, ok)) break;
         at_zero_rows<DC, AT_KEYS, 128>(smem + L::KV + (x % L::RING) * L::TILE, t.len - j0, threadIdx.x);
         fence_proxy_async_smem();
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
       tc_fence_before();
       mbar_arrive(&p_ready[b]);
     }
-    if (__all_sync(0xffffffffu, ok)) ok = at_wait(o_full, 0, abort_flag, 8);
+    if (__all_sync(0xffffffffu, ok)) ok = at_wait(o_full, 0, aw, 8);
     if (__all_sync(0xffffffffu, ok)) {
       tc_fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -289,10 +289,19 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
                                         int64_t(p.heads) * p.head_dim, t.len - t.i0 - w0, p.head_dim, inv);
       if (i < t.len) lse[int64_t(h) * p.tokens + row + lane] = l == 0.f ? -INFINITY : m * p.scale + logf(l * (1.f / float(1 << int(at_fwd_shift<T>()))));
     }
+    __syncwarp();
+    tmem_st_wait();  // (a warp that gave up may have stores under way)
     tc_fence_before();
   }
   __syncthreads();
   if (warp == 5) tmem_dealloc(tmem, 256);
+  if (*abort_flag) {  // a wait ran out somewhere: no row of the tile is an answer
+    const int n = min(AT_TILE, t.len - t.i0);
+    const int64_t off = (int64_t(t.a + t.i0) * p.heads + h) * p.head_dim, stride = int64_t(p.heads) * p.head_dim;
+    at_poison_rows(out + off, stride, n, p.head_dim, threadIdx.x, AT_FWD_THREADS);
+    if (rest != nullptr) at_poison_rows(rest + off, stride, n, p.head_dim, threadIdx.x, AT_FWD_THREADS);
+    if (threadIdx.x < n) lse[int64_t(h) * p.tokens + t.a + t.i0 + threadIdx.x] = __int_as_float(0x7fffffff);
+  }
 }
 
 // ------------------------------------------------------------------ backward
@@ -481,8 +490,8 @@ struct AttnBwdSmem {
   static constexpr int B = 4 * TILE;
   static constexpr int OUT = 6 * TILE;             // 2 KB per elementwise warp: rows on their way out
   static constexpr int AUX = OUT + 8 * 2048;       // [2][128] -lse, [2][128] -delta (scaled)
-  static constexpr int UNIT = AUX + 4 * AT_TILE * 4;  // [2] AttnUnit
-  static constexpr int BAR = UNIT + 2 * 64;
+  static constexpr int UNIT = AUX + 4 * AT_TILE * 4;  // [2] AttnUnit, and the last 4 taken
+  static constexpr int BAR = UNIT + 6 * 64;
   // a_full[2], a_empty[2], b_full[2], b_empty[2], aux_empty[2], unit_full[2], unit_empty[2], xy_full,
   // xy_empty, s_full, p_ready, dp_full, ds_ready, acc_full, acc_empty, drained, exp_full[2]
   static constexpr int NBAR = 25;
@@ -510,6 +519,56 @@ struct AttnUnit {
   int join;              // the key tile's number among those that are shared
 };
 static_assert(sizeof(AttnUnit) <= 64, "one slot of the unit ring");
+
+// Whole warp: unit number `at` of the order (below n_all), false for one without tokens.
+struct AttnUnits {
+  unsigned n_keys, n_main, n_all;
+  __device__ AttnUnits(const AttnParams& p, int split) {
+    n_keys = unsigned(p.slots) * unsigned(p.kv_heads) * unsigned(split);
+    n_main = n_keys + unsigned(p.slots) * unsigned(p.heads);
+    n_all = n_main + (split > 1 ? unsigned(p.slots) * unsigned(p.kv_heads) * AT_PIECES : 0u);
+  }
+};
+__device__ __forceinline__ bool at_unit(const AttnParams& p, const AttnUnits& order, int split, unsigned at, AttnUnit& u, int& slot) {
+  const int grp = p.heads / p.kv_heads;
+  if (at < order.n_keys) {
+    u.kind = AT_UNIT_KEYS;
+    u.rank = int(at % unsigned(split));
+    u.join = int(at / unsigned(split));
+  } else if (at < order.n_main) {
+    u.kind = AT_UNIT_QUERIES;
+    u.rank = u.join = 0;
+    slot = p.slots - 1 - int((at - order.n_keys) / unsigned(p.heads));
+    u.h = int((at - order.n_keys) % unsigned(p.heads));
+    u.hk = u.h / grp;
+    u.h0 = 0;
+  } else {
+    u.kind = AT_UNIT_JOIN;
+    u.rank = int((at - order.n_main) % AT_PIECES);
+    u.join = int((at - order.n_main) / AT_PIECES);
+  }
+  if (u.kind != AT_UNIT_QUERIES) {
+    slot = int(unsigned(u.join) / unsigned(p.kv_heads));
+    u.h = u.hk = int(unsigned(u.join) % unsigned(p.kv_heads));
+    u.h0 = u.h * grp + u.rank * (grp / split);
+  }
+  const AttnTile t = at_find(p, slot);
+  if (t.tail || t.i0 >= t.len) {  // rows behind the last sequence: the prep launch's
+    u.kind = AT_UNIT_END;
+    return false;
+  }
+  u.a = t.a;
+  u.len = t.len;
+  u.i0 = t.i0;
+  const bool keys = u.kind == AT_UNIT_KEYS;
+  const int back = keys ? p.right : p.left, ahead = keys ? p.left : p.right;  // the window seen from X's side
+  const int last = min(t.i0 + AT_TILE, t.len) - 1;
+  const int lo = back < 0 ? 0 : max(0, t.i0 - back), hi = ahead < 0 ? t.len - 1 : min(t.len - 1, last + ahead);
+  u.yt0 = lo >> 7;
+  u.nt = (hi >> 7) - u.yt0 + 1;
+  u.n = keys ? u.nt * (grp / split) : u.nt;
+  return true;
+}
 
 // A share's sums: groups of four features of [dK | dV], by rows.
 template <int DC>
@@ -551,8 +610,10 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
   float* aux_lse = reinterpret_cast<float*>(smem + L::AUX);
   float* aux_dl = aux_lse + 2 * AT_TILE;
   AttnUnit* units = reinterpret_cast<AttnUnit*>(smem + L::UNIT);
+  AttnUnit* taken = units + 2;  // [4]: the last units this CTA took
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC + 4);
+  const AttnWait aw{abort_flag, p.wait_cycles};
   int* exponent = reinterpret_cast<int*>(smem + L::MISC + 8);  // [2]
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int grp = p.heads / p.kv_heads;
@@ -578,6 +639,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
     mbar_init(acc_empty, 256);
     mbar_init(drained, 1);
     fence_barrier_init();
+    for (int i = 0; i < 4; ++i) taken[i].kind = AT_UNIT_END;
     *abort_flag = 0;
   }
   if (warp == 9) {
@@ -598,15 +660,13 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
 
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity, int where) {  // whole warp
-    ok = __all_sync(0xffffffffu, ok && at_wait(bar, parity, abort_flag, where));
+    ok = __all_sync(0xffffffffu, ok && at_wait(bar, parity, aw, where));
     return ok;
   };
 
   if (warp == 8) {
     // ---------------------------------------------------------------- units and TMA
-    const unsigned n_keys = unsigned(p.slots) * unsigned(p.kv_heads) * unsigned(split);
-    const unsigned n_main = n_keys + unsigned(p.slots) * unsigned(p.heads);
-    const unsigned n_all = n_main + (split > 1 ? unsigned(p.slots) * unsigned(p.kv_heads) * AT_PIECES : 0u);
+    const AttnUnits order(p, split);
     unsigned loads = 0, issued = 0, aux = 0;  // ring items so far, also those under way
     int k = 0, tiles = 0;         // units so far; those of them with tiles
     // the row starts into the L1 while the first unit's number is on its way
@@ -620,45 +680,9 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
         unsigned at = 0;
         if (lane == 0) at = atomicAdd(w.next, 1u);
         at = __shfl_sync(0xffffffffu, at, 0);
-        if (at >= n_all) break;
-        if (at < n_keys) {
-          u.kind = AT_UNIT_KEYS;
-          u.rank = int(at % unsigned(split));
-          u.join = int(at / unsigned(split));
-        } else if (at < n_main) {
-          u.kind = AT_UNIT_QUERIES;
-          u.rank = u.join = 0;
-          slot = p.slots - 1 - int((at - n_keys) / unsigned(p.heads));
-          u.h = int((at - n_keys) % unsigned(p.heads));
-          u.hk = u.h / grp;
-          u.h0 = 0;
-        } else {
-          u.kind = AT_UNIT_JOIN;
-          u.rank = int((at - n_main) % AT_PIECES);
-          u.join = int((at - n_main) / AT_PIECES);
-        }
-        if (u.kind != AT_UNIT_QUERIES) {
-          slot = int(unsigned(u.join) / unsigned(p.kv_heads));
-          u.h = u.hk = int(unsigned(u.join) % unsigned(p.kv_heads));
-          u.h0 = u.h * grp + u.rank * (grp / split);
-        }
-        const AttnTile t = at_find(p, slot);
-        if (t.tail || t.i0 >= t.len) {  // rows behind the last sequence: the prep launch's
-          u.kind = AT_UNIT_END;
-          continue;
-        }
-        u.a = t.a;
-        u.len = t.len;
-        u.i0 = t.i0;
-        const bool keys = u.kind == AT_UNIT_KEYS;
-        const int back = keys ? p.right : p.left, ahead = keys ? p.left : p.right;  // the window seen from X's side
-        const int last = min(t.i0 + AT_TILE, t.len) - 1;
-        const int lo = back < 0 ? 0 : max(0, t.i0 - back), hi = ahead < 0 ? t.len - 1 : min(t.len - 1, last + ahead);
-        u.yt0 = lo >> 7;
-        u.nt = (hi >> 7) - u.yt0 + 1;
-        u.n = keys ? u.nt * (grp / split) : u.nt;
-        break;
+        if (at >= order.n_all || at_unit(p, order, split, at, u, slot)) break;
       }
+      if (lane == 0) taken[k & 3] = u;
       const bool keys = u.kind == AT_UNIT_KEYS, main = keys || u.kind == AT_UNIT_QUERIES;
       auto load = [&](int hy, int y0) {  // ring item `loads`
         const int s = loads & 1;
@@ -691,7 +715,9 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
         const long long t0 = clock64();
         const volatile unsigned* done = w.tickets + u.join;
         while (ok && *done < 8u * unsigned(split)) {  // every elementwise warp of every share
-          if (*abort_flag || clock64() - t0 > kAttnWaitCycles) {
+          if (*abort_flag) {
+            ok = false;
+          } else if (clock64() - t0 >= p.wait_cycles) {
             *abort_flag = 1;
             atomicExch(&g_attn_error, 27);
             ok = false;
@@ -747,8 +773,8 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
       }
       if (!ok) break;
     }
-    // an abandoned CTA's loads must have landed before its shared memory goes
-    if (!ok && lane == 0) {
+    // the loads must have landed before the CTA's shared memory goes (see the forward)
+    if (lane == 0) {
       if (tiles > 0) at_drain(xy_full, (tiles - 1) & 1);
       if (issued > loads) mbar_arrive(&a_full[loads & 1]);
       for (unsigned i = issued > 2 ? issued - 2 : 0; i < issued; ++i) {
@@ -838,10 +864,8 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
       at_commit(lead, acc_full);
       ++m;
     }
-    if (!ok) {  // nothing in flight when TMEM and shared memory go
-      at_commit(lead, drained);
-      at_drain(drained, 0);
-    }
+    at_commit(lead, drained);  // nothing in flight when TMEM and shared memory go
+    at_drain(drained, 0);
   } else {
     // ---------------------------------------------------------------- elementwise
     const int half = warp >> 2;  // columns [64 half, 64 half + 64)
@@ -1084,10 +1108,38 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
         if (lane == 0) atomicAdd(w.tickets + u.join, 1u);
       }
     }
+    __syncwarp();
+    tmem_st_wait();  // (a warp that gave up may have stores under way)
     tc_fence_before();
   }
   __syncthreads();
   if (warp == 9) tmem_dealloc(tmem, 512);
+  if (warp == 8 && *abort_flag) {
+    // A wait ran out: NaN in the rows of the units under way (four at most: the one whose sums are read, one
+    // with its MMAs, one published, one just taken), and of all that this CTA can still take, so that
+    // none is left unwritten.  A lost share of a key tile's heads lets the wait of its sum run out.
+    auto poison = [&](const AttnUnit& u) {
+      const int64_t row = u.a + u.i0, n = min(AT_TILE, u.len - u.i0);
+      if (u.kind == AT_UNIT_QUERIES) {
+        at_poison_rows(dq + (row * p.heads + u.h) * p.head_dim, int64_t(p.heads) * p.head_dim, n, p.head_dim, lane, 32);
+      } else if (u.kind == AT_UNIT_JOIN || (u.kind == AT_UNIT_KEYS && split == 1)) {
+        const int64_t off = (row * p.kv_heads + u.h) * p.head_dim, stride = int64_t(p.kv_heads) * p.head_dim;
+        at_poison_rows(dk + off, stride, n, p.head_dim, lane, 32);
+        at_poison_rows(dv + off, stride, n, p.head_dim, lane, 32);
+      }
+    };
+    for (int i = 0; i < 4; ++i) poison(taken[i]);
+    const AttnUnits order(p, split);
+    for (;;) {
+      unsigned at = 0;
+      if (lane == 0) at = atomicAdd(w.next, 1u);
+      at = __shfl_sync(0xffffffffu, at, 0);
+      if (at >= order.n_all) break;
+      AttnUnit u;
+      int slot = 0;
+      if (at_unit(p, order, split, at, u, slot)) poison(u);
+    }
+  }
 }
 
 static bool attn_strides_ok(int64_t stride, int64_t head_stride, const nf4b_attn& a) {
@@ -1139,9 +1191,18 @@ static int attn_tmap(CUtensorMap* m, const nf4b_attn& a, const void* base, int h
                          base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// Clocks after which a wait of the kernels gives up.  STEW_ATTN_WAIT_CYCLES sets another limit (0: a wait that
+// is not over when it begins gives up), to see what a caller gets then.
+static long long attn_wait_cycles() {
+  const char* v = std::getenv("STEW_ATTN_WAIT_CYCLES");
+  if (v == nullptr || v[0] < '0' || v[0] > '9') return kAttnWaitCycles;
+  const long long c = std::atoll(v);
+  return c < kAttnWaitCycles ? c : kAttnWaitCycles;
+}
+
 static AttnParams attn_params(const nf4b_attn& a) {
   return AttnParams{a.cu,       int32_t(a.tokens), a.rows,  a.heads, a.kv_heads,
-                    a.head_dim, a.left,            a.right, int32_t(at_slots(a.tokens, a.rows)), a.scale};
+                    a.head_dim, a.left,            a.right, int32_t(at_slots(a.tokens, a.rows)), a.scale, attn_wait_cycles()};
 }
 
 // Dynamic shared memory of a kernel, set once per device.

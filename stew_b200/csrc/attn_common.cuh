@@ -22,6 +22,7 @@ struct AttnParams {
   int32_t left, right;
   int32_t slots;       // tile slots of the packed rows, at_slots()
   float scale;
+  long long wait_cycles;  // limit of a wait, in clocks
 };
 
 // Tiles never cross a sequence.  Sequence s owns the tile slots from floor(start_s / 128) + s on: that many
@@ -262,29 +263,34 @@ __device__ __forceinline__ void at_store_rows(uint32_t taddr, uint8_t* buf, T* o
   }
 }
 
-// Bounded waits: after about two seconds the CTA's abort flag is raised, g_attn_error records where,
-// and every role winds down.
+// Bounded waits: after `limit` clocks (about two seconds) the CTA's abort flag is raised, g_attn_error records
+// where, and every role winds down.
 __device__ int g_attn_error;
 
 constexpr long long kAttnWaitCycles = 4000000000ll;
 
-__device__ __forceinline__ bool at_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int where) {
+struct AttnWait {
+  volatile int* abort;  // in shared memory, of the CTA
+  long long limit;
+};
+
+__device__ __forceinline__ bool at_wait_slow(uint64_t* bar, uint32_t parity, const AttnWait& w, int where) {
   const long long t0 = clock64();
   for (;;) {
-    if (mbar_try_wait_sleep(bar, parity, 1000000u)) return true;
-    if (*abort_flag) return false;
-    if (clock64() - t0 > kAttnWaitCycles) {
-      *abort_flag = 1;
+    if (w.limit > 0 && mbar_try_wait_sleep(bar, parity, 1000000u)) return true;
+    if (*w.abort) return false;
+    if (clock64() - t0 >= w.limit) {
+      *w.abort = 1;
       atomicExch(&g_attn_error, where);
       return false;
     }
   }
 }
-__device__ __forceinline__ bool at_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int where) {
+__device__ __forceinline__ bool at_wait(uint64_t* bar, uint32_t parity, const AttnWait& w, int where) {
   if (mbar_test_wait(bar, parity)) return true;
-  return at_wait_slow(bar, parity, abort_flag, where);
+  return at_wait_slow(bar, parity, w, where);
 }
-// Waits for work in flight whatever the abort flag says.
+// Waits for work in flight whatever the abort flag and the limit say.
 __device__ __forceinline__ void at_drain(uint64_t* bar, uint32_t parity) {
   const long long t0 = clock64();
   while (!mbar_try_wait_sleep(bar, parity, 1000000u)) {
@@ -293,6 +299,16 @@ __device__ __forceinline__ void at_drain(uint64_t* bar, uint32_t parity) {
       return;
     }
   }
+}
+
+// NaN in `rows` rows of head_dim values: what a CTA whose wait ran out leaves of the rows that are its own.
+// Thread `id` of `n`.
+template <typename T>
+__device__ __forceinline__ void at_poison_rows(T* to, int64_t stride, int rows, int head_dim, int id, int n) {
+  const int vec = head_dim / 8;
+  const uint32_t nan2 = 0x7fff7fffu;  // two NaN of either 16-bit type
+  for (int i = id; i < rows * vec; i += n)
+    *reinterpret_cast<uint4*>(to + (i / vec) * stride + (i % vec) * 8) = make_uint4(nan2, nan2, nan2, nan2);
 }
 
 }  // namespace nf4b

@@ -23,7 +23,7 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 
-from . import dp
+from . import _lib, dp
 from .lora import LORA_RANK, NF4Linear, NF4LoraLinear, grouped_projection, nf4_mlp
 from .step_ops import (add_rms_norm, head_cross_entropy, packed_attention, packed_attention_supported, rms_norm,
                        rope_qk)
@@ -266,7 +266,11 @@ class QLoRATrainer:
     cost one graph launch on the host.  The packed batch is copied into the graph's static
     input buffers each step; a new shape (token count, rows, longest row, labels) re-captures.
     The capture's warm-up steps are undone (adapters and optimizer state restored), so every
-    call is exactly one optimizer step."""
+    call is exactly one optimizer step.
+
+    A wait inside a GEMM or attention kernel that runs out of time raises before the optimizer's step.
+    A captured step has no place on the host to look: there check() raises when it is called (the
+    attention leaves NaN, so the loss tells too)."""
 
     def __init__(self, model: QwenQLoRA, lr: float = 2e-4, group=None, cuda_graph: bool = False,
                  buckets: int = 4, buckets_on_one_rank: bool = False, max_grad_norm: float | None = None):
@@ -309,6 +313,7 @@ class QLoRATrainer:
             else:
                 n_lab = torch.full((1,), float(pb.n_labels), device=pb.ids.device)
                 total = float(self._exchange(n_lab))
+        self.check()  # (the host has waited for the count) no step on gradients that were never finished
         self.opt.step()
         self.opt.zero_grad(set_to_none=True)
         return loss_sum.detach(), total
@@ -395,6 +400,13 @@ class QLoRATrainer:
             dst.copy_(src)
         self._graph.replay()
         return self._loss.detach() / max(n_lab, 1), n_lab, self._total
+
+    def check(self) -> None:
+        """Raises if a kernel gave up a wait since the last check (synchronises)."""
+        dev = self.params[0].device
+        if dev.type == "cuda":
+            with torch.cuda.device(dev):
+                _lib.raise_if_wait_ran_out()
 
     def release(self):
         """Drop the captured graph (it holds NCCL work: release before destroying the group)."""
