@@ -1264,7 +1264,10 @@ extern "C" int nf4b_attn_error_flag(int* value, int reset) {
 static int attn_sms() {
   static int cached[64] = {0};
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+    cudaGetLastError();  // (no device: the scratch may be asked for all the same)
+    return 148;
+  }
   if (cached[dev] == 0) {
     int v = 0;
     cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
@@ -1273,8 +1276,8 @@ static int attn_sms() {
   return cached[dev];
 }
 
-// CTAs that share a key tile's heads: the divisor of the group with the shortest estimated time on 148 SMs,
-// from an average sequence: the longer of all units' work shared out and the longest key-tile unit.  In
+// CTAs that share a key tile's heads: the divisor of the group with the shortest estimated time on the device's
+// SMs, from an average sequence: the longer of all units' work shared out and the longest key-tile unit.  In
 // microseconds, as measured: about 3 of start and store for a unit, 2 more for a shared one, 1.6 a key-tile
 // step, 1.2 a query-tile step.
 static int attn_split(const nf4b_attn& a) {
@@ -1284,15 +1287,17 @@ static int attn_split(const nf4b_attn& a) {
   const double most = (seen_max < len ? seen_max : len) / AT_TILE + 1;                          // tiles a key tile meets
   const double mean = (a.left < 0) != (a.right < 0) && most * AT_TILE > len ? (most + 1) / 2 : most;
   const double tiles = double(a.tokens) / AT_TILE + 0.5 * a.rows;
+  // (the shares' sums take 128 KB each: half a GB at most)
+  auto fits = [&](int c) { return grp % c == 0 && (c == 1 || at_slots(a.tokens, a.rows) * a.kv_heads * c <= 4096); };
+  const int sms = attn_sms();
   int best = 1;
   double best_us = 0;
   for (int c = 1; c <= grp; ++c) {
-    // (the shares' sums: 1 KB a key row, share and 128 features)
-    if (grp % c != 0 || (c > 1 && double(at_slots(a.tokens, a.rows)) * a.kv_heads * c > 4096)) continue;
+    if (!fits(c)) continue;
     const double one = 3.0 + (c > 1 ? 2.0 : 0.0);
     const double keys = tiles * a.kv_heads * c * (one + 1.6 * mean * (grp / c));
     const double queries = tiles * a.heads * (3.0 + 1.2 * mean);
-    const double all = (keys + queries) / 148, longest = one + 1.6 * most * (grp / c);
+    const double all = (keys + queries) / sms, longest = one + 1.6 * most * (grp / c);
     const double us = all > longest ? all : longest;
     if (c == 1 || us < best_us) {
       best = c;
@@ -1300,7 +1305,7 @@ static int attn_split(const nf4b_attn& a) {
     }
   }
   const char* v = std::getenv("STEW_ATTN_SPLIT");
-  if (v != nullptr && v[0] >= '1' && v[0] <= '9' && grp % (v[0] - '0') == 0) best = v[0] - '0';
+  if (v != nullptr && v[0] >= '1' && v[0] <= '9' && fits(v[0] - '0')) best = v[0] - '0';
   return best;
 }
 
