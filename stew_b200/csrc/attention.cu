@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
 // about 2,900 clocks, of them 1,150 exponentials and 1,250 other elementwise work and waits in one chain,
 // beside 2,048 of MMAs; a launch per unit instead of persistent CTAs: 43 us and 694.
 //
-// FINE: dS is kept as two 16-bit values, its rounding and what that leaves, each with its product (attn_fine()).
+// Fine units keep dS as two 16-bit values, its rounding and what that leaves, each with its product (at_fine()).
 //
 // fp16 range: dS is rounded to the operand type with a power-of-two scale 2^k that puts the largest
 // |dO||V| + |delta| of the tiles a unit meets (the prep launch's maxima) at 2^14, and P with 2^8:
@@ -517,8 +517,23 @@ struct AttnUnit {
   int yt0, nt, n;        // the ring's first tile, its tiles per head, ring items
   int h0;                // first query head of a key tile's share
   int join;              // the key tile's number among those that are shared
+  int fine;              // dS as two 16-bit values
 };
 static_assert(sizeof(AttnUnit) <= 64, "one slot of the unit ring");
+
+// Whether dS goes into dQ and dK with what its rounding leaves: sequences of one tile, windows of 128, and
+// batches whose sequences have 256 tokens or fewer on average (the tokens behind the last one do not count).  The
+// ds of a row sum to zero, so over a few tokens their roundings stay in the sums: with two to ten tokens a
+// sequence dq and dk were 1.50 to 1.56 times as far off the 64-bit result as values rounded once, with the rest
+// 1.05 to 1.14 times; over some hundred tokens it was 1.43.  It costs a second dS product: a backward of 1,170
+// tokens in 4 rows 33 -> 36 us where all of them take it, of 8,192 670 -> 820.  The choice is a unit's own, so
+// that a short sequence's gradients do not depend on what is packed beside it: that took 1,170 tokens from 32 to
+// 33 us, a window of 255 over 8,192 from 90.5 to 94.5, 8,192 causal ones from 666 to 676 (against a kernel of
+// each kind, chosen for the whole call).
+__device__ __forceinline__ bool at_fine(const AttnParams& p, int len) {
+  return len <= AT_TILE || (p.left >= 0 && p.right >= 0 && p.left + p.right < AT_TILE) ||
+         (at_start(p, p.rows) + 255) >> 8 <= p.rows;
+}
 
 // Whole warp: unit number `at` of the order (below n_all), false for one without tokens.
 struct AttnUnits {
@@ -567,6 +582,7 @@ __device__ __forceinline__ bool at_unit(const AttnParams& p, const AttnUnits& or
   u.yt0 = lo >> 7;
   u.nt = (hi >> 7) - u.yt0 + 1;
   u.n = keys ? u.nt * (grp / split) : u.nt;
+  u.fine = at_fine(p, t.len);
   return true;
 }
 
@@ -582,7 +598,7 @@ __device__ __forceinline__ float4* at_part(float* parts, int join, int split, in
 // unit's sums are stored.  A sum waits for its shares; they come before it in the order, so each has been
 // taken by a CTA that runs and does not wait for it (no unit belongs to a CTA before that CTA takes it: one
 // that found no room yet holds nothing up).
-template <typename T, int DC, bool FINE>
+template <typename T, int DC>
 __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
     attn_bwd_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_constant__ AttnParams p, const AttnWork w,
                     const int split, T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dv) {
@@ -824,45 +840,50 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
       if (!keys) at_commit(lead, &b_empty[i & 1]);
       return true;
     };
-    for (int k = 0;; ++k) {
-      if (!wait(&unit_full[k & 1], (k >> 1) & 1, 15)) break;
-      auto of_unit = [&](int v) { return __shfl_sync(0xffffffffu, v, 0); };
-      const int kind = of_unit(units[k & 1].kind), n = of_unit(units[k & 1].n), nt = of_unit(units[k & 1].nt);
-      const int tokens = of_unit(units[k & 1].len - units[k & 1].yt0 * AT_TILE);  // from the ring's first tile on
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&unit_empty[k & 1]);
-      if (kind == AT_UNIT_END) break;
-      if (kind == AT_UNIT_JOIN) continue;
-      const bool keys = kind == AT_UNIT_KEYS;
+    // One unit's MMAs; a copy for each kind of dS (a test around the second product cost 5 % of a short backward).
+    auto unit = [&](auto fine_tag, bool keys, int n, int nt, int tokens) {
       // MMAs over 16 tokens each: nothing behind the sequence's end
       int yt = 0, steps = (min(tokens, AT_TILE) + 15) >> 4;
-      if (!wait(xy_full, m & 1, 18) || !s_of(r, steps) || !dp_of(r, keys, steps)) break;
+      if (!wait(xy_full, m & 1, 18) || !s_of(r, steps) || !dp_of(r, keys, steps)) return;
       if (n == 1) at_commit(lead, xy_empty);
       for (int it = 0; it < n; ++it, ++r) {
         const bool more = it + 1 < n;
         if (++yt == nt) yt = 0;
         const int next = (min(tokens - yt * AT_TILE, AT_TILE) + 15) >> 4;
-        if (!wait(p_ready, r & 1, 19)) break;
+        if (!wait(p_ready, r & 1, 19)) return;
         // the sums of the unit before have been read
-        if (it == 0 && !wait(acc_empty, (m & 1) ^ 1, 20)) break;
+        if (it == 0 && !wait(acc_empty, (m & 1) ^ 1, 20)) return;
         tc_fence_after();
         if (keys) {
           sum(tmem + AT_TM_DV, tmem + AT_TM_S, tb + (r & 1) * STEP, it > 0, steps);
           at_commit(lead, &b_empty[r & 1]);
         }
-        if (more && !s_of(r + 1, next)) break;
-        if (!wait(ds_ready, r & 1, 21)) break;
+        if (more && !s_of(r + 1, next)) return;
+        if (!wait(ds_ready, r & 1, 21)) return;
         tc_fence_after();
         sum(tmem + AT_TM_DX, tmem + AT_TM_DP, ta + (r & 1) * STEP, it > 0, steps);
-        if (FINE) sum(tmem + AT_TM_DX, tmem + AT_TM_DP + 32, ta + (r & 1) * STEP, true, steps);
+        if (decltype(fine_tag)::value) sum(tmem + AT_TM_DX, tmem + AT_TM_DP + 32, ta + (r & 1) * STEP, true, steps);
         at_commit(lead, &a_empty[r & 1]);
-        if (more && !dp_of(r + 1, keys, next)) break;
+        if (more && !dp_of(r + 1, keys, next)) return;
         if (it + 2 == n) at_commit(lead, xy_empty);  // no more scores of this unit
         steps = next;
       }
-      if (!ok) break;
       at_commit(lead, acc_full);
       ++m;
+    };
+    for (int k = 0;; ++k) {
+      if (!wait(&unit_full[k & 1], (k >> 1) & 1, 15)) break;
+      auto of_unit = [&](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+      const int kind = of_unit(units[k & 1].kind), n = of_unit(units[k & 1].n), nt = of_unit(units[k & 1].nt);
+      const int fine = of_unit(units[k & 1].fine);
+      const int tokens = of_unit(units[k & 1].len - units[k & 1].yt0 * AT_TILE);  // from the ring's first tile on
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&unit_empty[k & 1]);
+      if (kind == AT_UNIT_END) break;
+      if (kind == AT_UNIT_JOIN) continue;
+      if (fine) unit(std::true_type{}, kind == AT_UNIT_KEYS, n, nt, tokens);
+      else unit(std::false_type{}, kind == AT_UNIT_KEYS, n, nt, tokens);
+      if (!ok) break;
     }
     at_commit(lead, drained);  // nothing in flight when TMEM and shared memory go
     at_drain(drained, 0);
@@ -878,8 +899,8 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
     unsigned r = 0, aux = 0, m = 0;
     // One unit's ring items.
     int k_exp = 0;
-    auto items = [&](auto keys_tag, const AttnUnit& u) {
-      constexpr bool KEYS = decltype(keys_tag)::value;
+    auto items = [&](auto keys_tag, auto fine_tag, const AttnUnit& u) {
+      constexpr bool KEYS = decltype(keys_tag)::value, FINE = decltype(fine_tag)::value;
       const int x = u.i0 + row;  // this thread's row, relative to a
       float sc = 1.f;
       const int back = KEYS ? p.right : p.left, ahead = KEYS ? p.left : p.right;
@@ -1064,8 +1085,13 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1)
         continue;
       }
       const bool keys = u.kind == AT_UNIT_KEYS;
-      if (keys) items(std::true_type{}, u);
-      else items(std::false_type{}, u);
+      if (keys) {
+        if (u.fine) items(std::true_type{}, std::true_type{}, u);
+        else items(std::true_type{}, std::false_type{}, u);
+      } else {
+        if (u.fine) items(std::false_type{}, std::true_type{}, u);
+        else items(std::false_type{}, std::false_type{}, u);
+      }
       if (!ok || !wait(acc_full, m & 1, 26)) break;
       ++m;
       tc_fence_after();
@@ -1309,17 +1335,6 @@ static int attn_split(const nf4b_attn& a) {
   return best;
 }
 
-// Whether dS goes into dQ and dK with what its rounding leaves: sequences of 256 tokens or fewer on average
-// (the padding counts), or windows of 128.  The ds of a row sum to zero, so over a few tokens their roundings
-// stay in the sums: with two to ten tokens a sequence dq and dk were 1.50 to 1.56 times as far off the 64-bit
-// result as values rounded once, with the rest 1.05 to 1.14 times; over some hundred tokens it was 1.43.  It
-// costs a second dS product: a backward of 63 tokens 17.6 -> 18.2 us, of 1,170 in 4 rows 31.9 -> 35.2, of
-// 8,192 670 -> 820.
-static bool attn_fine(const nf4b_attn& a) {
-  const bool window = a.left >= 0 && a.right >= 0 && int64_t(a.left) + a.right < AT_TILE;
-  return window || a.tokens <= int64_t(a.rows) * 2 * AT_TILE;
-}
-
 static int64_t attn_work(const nf4b_attn& a, int split, void* base, AttnWork* w) {
   const int64_t slots = at_slots(a.tokens, a.rows), pairs = slots * a.kv_heads;
   char* b = static_cast<char*>(base);
@@ -1346,7 +1361,7 @@ extern "C" int64_t nf4b_attn_bwd_work_bytes(const nf4b_attn* args) {
   return attn_work(a, attn_split(a), nullptr, nullptr);
 }
 
-template <typename T, int DC, bool FINE>
+template <typename T, int DC>
 static int attn_bwd_launch(const nf4b_attn& a, const void* out, const void* rest, const float* lse, const void* dout, void* dq, void* dk,
                            void* dv, void* work, int split, cudaStream_t s) {
   AttnBwdMaps m;
@@ -1355,7 +1370,7 @@ static int attn_bwd_launch(const nf4b_attn& a, const void* out, const void* rest
   if (st == NF4B_OK) st = attn_tmap(&m.v, a, a.v, a.kv_heads, a.v_stride, a.v_head_stride, AT_TILE);
   if (st == NF4B_OK) st = attn_tmap(&m.dout, a, dout, a.heads, int64_t(a.heads) * a.head_dim, a.head_dim, AT_TILE);
   static bool done[64] = {false};
-  if (st == NF4B_OK) st = attn_smem(attn_bwd_kernel<T, DC, FINE>, AttnBwdSmem<DC>::ALLOC, done);
+  if (st == NF4B_OK) st = attn_smem(attn_bwd_kernel<T, DC>, AttnBwdSmem<DC>::ALLOC, done);
   if (st != NF4B_OK) return st;
   const AttnParams p = attn_params(a);
   AttnWork w;
@@ -1367,7 +1382,7 @@ static int attn_bwd_launch(const nf4b_attn& a, const void* out, const void* rest
                            static_cast<const T*>(a.v), a.v_stride, a.v_head_stride, w, tq, tk, tv));
   const int64_t units = int64_t(p.slots) * (int64_t(a.kv_heads) * (split > 1 ? split + AT_PIECES : 1) + a.heads);
   const int64_t sms = attn_sms();
-  NF4B_CUDA_TRY(launch_pdl(attn_bwd_kernel<T, DC, FINE>, dim3(unsigned(units < sms ? units : sms)), dim3(AT_BWD_THREADS),
+  NF4B_CUDA_TRY(launch_pdl(attn_bwd_kernel<T, DC>, dim3(unsigned(units < sms ? units : sms)), dim3(AT_BWD_THREADS),
                            size_t(AttnBwdSmem<DC>::ALLOC), s, m, p, w, split, tq, tk, tv));
   return launch_status("attn_bwd_kernel launch");
 }
@@ -1387,15 +1402,12 @@ extern "C" int nf4b_attn_bwd(const nf4b_attn* args, const void* out, const void*
   st = check_device();
   if (st != NF4B_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  auto launch = [&](auto tag, auto dc, auto fine) {
+  auto launch = [&](auto tag, auto dc) {
     using T = decltype(tag);
-    return attn_bwd_launch<T, decltype(dc)::value, decltype(fine)::value>(a, out, rest, lse, dout, dq, dk, dv, work, split, s);
+    return attn_bwd_launch<T, decltype(dc)::value>(a, out, rest, lse, dout, dq, dk, dv, work, split, s);
   };
   auto typed = [&](auto tag) {
-    const std::integral_constant<int, 1> one;
-    const std::integral_constant<int, 2> two;
-    if (attn_fine(a)) return a.head_dim > 64 ? launch(tag, two, std::true_type{}) : launch(tag, one, std::true_type{});
-    return a.head_dim > 64 ? launch(tag, two, std::false_type{}) : launch(tag, one, std::false_type{});
+    return a.head_dim > 64 ? launch(tag, std::integral_constant<int, 2>()) : launch(tag, std::integral_constant<int, 1>());
   };
   return a.dtype == NF4B_F16 ? typed(__half()) : typed(__nv_bfloat16());
 }
