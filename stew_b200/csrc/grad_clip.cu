@@ -1,5 +1,5 @@
 // Global 2-norm of a list of gradients and clipping (C ABI include/stew_step.h):
-//   norm = sqrt(sum src^2) / divisor,   dst = src (1 / divisor) min(1, max_norm / (norm + 1e-6))
+//   norm = sqrt(sum src^2) / |divisor|,   dst = src (1 / divisor) min(1, max_norm / (norm + 1e-6))
 //
 // Two launches: the list is cut into chunks of 16 KB, every CTA takes a contiguous run of them.  The first
 // launch writes one 64-bit sum of squares per CTA; every CTA of the second adds those sums up in the same
@@ -168,6 +168,12 @@ __device__ __forceinline__ void gc_scale_chunk(const T* src, T* dst, int n, floa
   }
 }
 
+// The same with a factor that fp32 holds only with less precision, or not at all.
+template <typename T>
+__device__ __forceinline__ void gc_scale_chunk_wide(const T* src, T* dst, int n, double f) {
+  for (int i = threadIdx.x; i < n; i += GC_THREADS) dst[i] = gc_from_f<T>(float(double(gc_to_f(src[i])) * f));
+}
+
 // Calls f(typed src, typed dst, count) for chunk c of gradient `it`.
 template <typename F>
 __device__ __forceinline__ void gc_chunk(const GcItem& it, int c, F f) {
@@ -216,7 +222,7 @@ __global__ void __launch_bounds__(GC_THREADS, GC_SCALE_CTAS / 148)
     grad_scale_kernel(const __grid_constant__ GcList<CAP> l, const double* __restrict__ part, int parts, float max_norm,
                       const float* __restrict__ divisor, float* __restrict__ norm_out) {
   grid_dep_wait();  // programmatic launch: no global access before the wait
-  __shared__ float s_factor;
+  __shared__ double s_factor;
   double acc = 0.0;
   for (int i = threadIdx.x; i < parts; i += GC_THREADS) acc += part[i];
   acc = gc_cta_sum(acc);
@@ -224,18 +230,25 @@ __global__ void __launch_bounds__(GC_THREADS, GC_SCALE_CTAS / 148)
     const double div = divisor ? double(*divisor) : 1.0;
     const double norm = sqrt(acc) / fabs(div);
     const double q = double(max_norm) / (norm + 1e-6);
-    s_factor = float((q >= 1.0 ? 1.0 : q) / div);  // a NaN norm stays one
+    s_factor = (q >= 1.0 ? 1.0 : q) / div;  // a NaN norm stays one
     if (blockIdx.x == 0 && norm_out) *norm_out = float(norm);
   }
   __syncthreads();
-  const float f = s_factor;
+  const double wide = s_factor;
+  const float f = float(wide);
+  // outside fp32's normal range (gradients of 1e30 and a limit of 1e-10, a divisor of 1e-39) the results may still
+  // be inside
+  const bool normal = wide == 0.0 || !(fabs(wide) < 0x1p-126 || (isinf(f) && !isinf(wide)));
   const int c0 = gc_first(l.chunks, blockIdx.x), c1 = gc_first(l.chunks, blockIdx.x + 1);
   int g = c0 < c1 ? gc_find(l, c0) : 0;
   for (int c = c0; c < c1; ++c) {
     while (g + 1 < l.n && l.it[g + 1].chunk0 <= c) ++g;
     const GcItem& it = l.it[g];
     if (it.dst == nullptr || (it.dst == it.src && f == 1.f)) continue;
-    gc_chunk(it, c, [&](auto* src, auto* dst, int n) { gc_scale_chunk(src, dst, n, f); });
+    gc_chunk(it, c, [&](auto* src, auto* dst, int n) {
+      if (normal) gc_scale_chunk(src, dst, n, f);
+      else gc_scale_chunk_wide(src, dst, n, wide);
+    });
   }
 }
 
