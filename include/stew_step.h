@@ -88,7 +88,7 @@ typedef struct nf4b_attn {
   int32_t rows, heads, kv_heads, head_dim;
   int32_t dtype;         /* NF4B_F16 or NF4B_BF16 */
   int32_t left, right;
-  float scale;           /* > 0 */
+  float scale;           /* > 0, below 2^127 */
 } nf4b_attn;
 
 /* out [tokens, heads, head_dim] contiguous, of q's type; lse fp32 [heads, tokens] (natural log);

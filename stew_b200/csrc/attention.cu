@@ -1181,7 +1181,7 @@ static int attn_checks(const nf4b_attn* in, nf4b_attn* a) {
   NF4B_RETURN_IF(a->tokens < 0 || a->rows < 0 || a->heads <= 0 || a->kv_heads <= 0 || a->head_dim <= 0,
                  NF4B_ERR_INVALID_ARG);
   NF4B_RETURN_IF(a->heads % a->kv_heads != 0, NF4B_ERR_INVALID_ARG);
-  NF4B_RETURN_IF(!(a->scale > 0.f) || !isfinite(a->scale), NF4B_ERR_INVALID_ARG);
+  NF4B_RETURN_IF(!(a->scale > 0.f && a->scale < 0x1p127f), NF4B_ERR_INVALID_ARG);  // scale log2(e) is fp32, too
   NF4B_RETURN_IF(a->dtype != NF4B_F16 && a->dtype != NF4B_BF16, NF4B_ERR_UNSUPPORTED);
   NF4B_RETURN_IF(a->head_dim % 8 != 0 || a->head_dim > AT_MAX_DIM, NF4B_ERR_UNSUPPORTED);
   NF4B_RETURN_IF(a->tokens > 0x3FFFFFFF || a->rows > 0x3FFFFFFF || a->heads > 65535, NF4B_ERR_UNSUPPORTED);

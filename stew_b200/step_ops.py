@@ -285,8 +285,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torc
         raise ValueError(f"packed_attention: window {tuple(window)}: bounds are >= 0, or -1 for none")
     left, right = min(left, n), min(right, n)  # further than the longest sequence: no bound
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not (scale > 0.0 and math.isfinite(scale)):
-        raise ValueError(f"packed_attention: scale must be positive and finite, got {scale}")
+    if not 2.0 ** -149 <= scale < 2.0 ** 127:  # (fp32, and so is scale log2(e))
+        raise ValueError(f"packed_attention: scale must be positive and below 2^127, got {scale}")
     # (a forward-mode tangent goes there too, to be refused: the kernels on their own would drop it)
     if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
             or any(forward_ad.unpack_dual(t).tangent is not None for t in (q, k, v))):

@@ -119,3 +119,28 @@ def test_forward_mode_tangents_are_refused(launches, which, grad):
         with torch.no_grad(), pytest.raises((RuntimeError, NotImplementedError)):
             packed_attention(*qkv, cu)
         packed_attention(*(t.detach() for t in leaves), cu)  # none of them dual: allowed
+
+
+@pytest.mark.parametrize("scale", [3.5e38, 1e39, 1e300, 2.0 ** 127, 0.0, 1e-46, 5e-324, float("inf"), float("nan"), -1.0])
+def test_scales_that_the_kernels_cannot_hold_are_refused(launches, scale):
+    """The kernels take scale log2(e) in fp32."""
+    from stew_b200.step_ops import packed_attention
+    leaves, cu = _inputs(False)
+    with pytest.raises(ValueError, match="scale"):
+        packed_attention(*leaves, cu, scale=scale)
+    assert not launches
+    packed_attention(*leaves, cu, scale=1e38)
+    assert len(launches) == 1
+
+
+def test_scale_in_the_entry():
+    from stew_b200 import _lib
+    a = _lib.AttnC()
+    a.q = a.k = a.v = a.cu = 256
+    a.tokens, a.rows, a.heads, a.kv_heads, a.head_dim = 10, 1, 4, 2, 64
+    a.q_stride, a.k_stride, a.v_stride = 256, 128, 128
+    a.q_head_stride = a.k_head_stride = a.v_head_stride = 64
+    a.dtype, a.left, a.right = _lib.NF4B_F16, -1, 0
+    for scale, ok in ((1e38, True), (2.0 ** 127, False), (3.4e38, False)):
+        a.scale = scale
+        assert (_lib.lib().nf4b_attn_bwd_work_bytes(bytes(a)) > 0) == ok
