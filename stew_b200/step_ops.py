@@ -242,6 +242,11 @@ class _PackedAttention(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None
 
 
+def _dual_level() -> bool:
+    """Whether a forward-mode level is open (1 us less than asking three tensors)."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
+
+
 def packed_attention_supported(q: torch.Tensor) -> bool:
     """Whether packed_attention's kernels take q's type and head size."""
     return (q.is_cuda and q.dtype in _ATTN_DTYPE and q.shape[-1] % 8 == 0
@@ -289,7 +294,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torc
         raise ValueError(f"packed_attention: scale must be positive and below 2^127, got {scale}")
     # (a forward-mode tangent goes there too, to be refused: the kernels on their own would drop it)
     if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
-            or any(forward_ad.unpack_dual(t).tangent is not None for t in (q, k, v))):
+            or _dual_level() and any(forward_ad.unpack_dual(t).tangent is not None for t in (q, k, v))):
         return _PackedAttention.apply(q, k, v, cu, left, right, scale)
     return _attn_forward(q, k, v, cu, left, right, scale)[0]
 
