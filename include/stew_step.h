@@ -128,7 +128,8 @@ typedef struct nf4b_grad {
 /* Global 2-norm of a list of gradients and clipping to max_norm (>= 0, or infinity):
  *   *norm = || src / *divisor ||_2 over all n gradients (device fp32; divisor: device fp32, NULL = 1)
  *   dst   = src * (1 / *divisor) * min(1, max_norm / (*norm + 1e-6))
- * The squares are summed in 64 bits in a fixed order.  A norm that is infinite gives zeros (NaN
+ * The squares are summed in 64 bits in a fixed order (16-bit values' exact squares in pairs, rounded to
+ * fp32, before that).  A norm that is infinite gives zeros (NaN
  * where src is infinite), a NaN norm gives NaN everywhere.  An in-place list under the limit with
  * no divisor is not written.  No dst may overlap another gradient's src or dst.  `grads` is a host
  * array, read before the call returns.  work: nf4b_clip_grads_work_bytes(n) bytes of device

@@ -31,8 +31,8 @@ namespace nf4b {
 // fp16: P holds 2^7 exp(s - m), at most 2^15 (l and O carry the factor, lse drops it), so that fp16's
 // subnormals begin at 2^-21 of the row's maximum and zeros at 2^-32.  l sums P before its rounding: without
 // the factor 65,536 keys at 2^-25.1 of the maximum, 1.8e-3 of the row's weight, were in l and not in O.
-// Measured, 12 query / 2 key-value heads of 128, fp16: 16,384 causal tokens 780-800 us, 1,031-1,058 TFLOP/s (the
-// power cap: cuBLAS sustains 1,371); 1,170 tokens in 4 rows 11.4 us, bound by a key tile's chain (scores,
+// Measured, 12 query / 2 key-value heads of 128, fp16: 16,384 causal tokens 780-830 us over boxes, 993-1,058 TFLOP/s
+// (the power cap: cuBLAS sustains 1,371); 1,170 tokens in 4 rows 11.7 us, bound by a key tile's chain (scores,
 // exponentials, product: about 1.1 us).  128-key tiles with one buffer of scores: 909 us; two query tiles per
 // CTA that share K and V: 813.
 constexpr int AT_KEYS = 64;                  // keys of a tile
@@ -320,8 +320,8 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 2)
 //   warps 0-7  elementwise: thread (row = TMEM lane, half of the columns)
 //   warp 8     takes units, TMA; for key tiles also the query rows' (lse, delta) into shared memory
 //   warp 9     TMEM allocation, MMA issue
-// Measured, heads as above: 8,192 causal tokens 655-680 us, 758-790 TFLOP/s of the formula's five products (the
-// power cap again); 1,170 tokens in 4 rows 29-32 us with six shares a key tile (one: 62).  A key tile's step takes
+// Measured, heads as above: 8,192 causal tokens 660-695 us over boxes, 741-780 TFLOP/s of the formula's five products
+// (the power cap again); 1,170 tokens in 4 rows 33 us with six shares a key tile (one: 62).  A key tile's step takes
 // about 2,900 clocks, of them 1,150 exponentials and 1,250 other elementwise work and waits in one chain,
 // beside 2,048 of MMAs; a launch per unit instead of persistent CTAs: 43 us and 694.
 //

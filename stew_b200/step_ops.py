@@ -263,12 +263,16 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torc
     window = (left, right): token i sees the tokens i - left <= j <= i + right of its sequence, -1
     for no bound; (-1, 0) is causal, (-1, -1) sees everything.  scale: of the scores, default
     1 / sqrt(D).
-    Returns [N, Hq, D]; tokens behind cu[B] get zeros, and zero gradients.  Any strides with
-    contiguous features are read in place when they are multiples of 8 elements, else copied.
+    Returns [N, Hq, D]; tokens behind cu[B] get zeros, and zero gradients.  What other sequences hold,
+    NaN too, does not reach a token; a NaN or infinity in v or in the output's gradient may reach
+    tokens of its own sequence that do not see it.  Any strides with contiguous features are read in
+    place when they are multiples of 8 elements, else copied.
     The backward recomputes the probabilities from the saved log-sum-exp; beside the output it
     keeps what the output's rounding left (a second tensor of its size), so that the rows' do.o
-    are free of it.  Forward and backward give the same bits on every run.  Second derivatives and
-    forward-mode tangents are refused."""
+    are free of it.  Forward and backward give the same bits on every run (the order of the fp32
+    sums goes by the counts of tokens, sequences and heads).  Second derivatives and forward-mode
+    tangents are refused.  A wait inside a kernel that runs out of time leaves NaN in the rows
+    concerned; _lib.raise_if_wait_ran_out() tells."""
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError("packed_attention: q, k and v must be [tokens, heads, head_dim]")
     if not (q.dtype == k.dtype == v.dtype and q.device == k.device == v.device):
