@@ -17,7 +17,7 @@ def _inputs(dtype, d, pad=7):
 
 
 def _fill_free_memory():
-    """What torch.empty will find: 123 in any 16-bit type's bytes, no NaN."""
+    """What torch.empty will find: 0x5555, no NaN of any type."""
     kept = [torch.full((1 << s,), 0x5555, dtype=torch.int16, device="cuda") for s in range(9, 22) for _ in range(6)]
     del kept
 
